@@ -6,7 +6,8 @@ reference's op interface (``brovisionml::dsine::ray_relu`` /
 ``angmf_propagate`` in include/brovisionml/dsine_ops.h:25-54, plus the
 brotensor convex-upsample / L2-normalise / slice calls of
 src/dsine_refine.cpp:277-292) for Python callers, with torch tensors as the
-device-memory carrier. Every op runs in the CUDA library; there is no CPU or
+device-memory carrier. Beside it, libbvml_blocks.so (``include/bvml_blocks.h``) holds the
+feed-forward operators over rows of features (``blocks.py``). Every op runs in the CUDA library; there is no CPU or
 PyTorch fallback, and importing the package fails loudly when the library is
 missing.
 
@@ -19,8 +20,13 @@ from ._capi import (BVML_F16, BVML_F32, LIB_PATH, abi_version, check, lib,  # no
                     loaded_library)
 from .ops import (angmf_propagate, conv2d_nhwc, convex_upsample, l2_normalize_nchw,  # noqa: F401
                   pack_conv_weight, ray_relu, refine, refine_workspace_bytes, slice2d)
+from .blocks import (BLOCKS_LIB_PATH, blocks_status, gated_linear,  # noqa: F401
+                     gated_linear_backward, linear, linear_backward, pack_weight_e4m3, rms_norm,
+                     rms_norm_backward, rms_norm_e4m3)
 
 __all__ = ["ray_relu", "angmf_propagate", "convex_upsample", "l2_normalize_nchw", "slice2d",
            "conv2d_nhwc", "pack_conv_weight",
-           "refine", "refine_workspace_bytes", "lib", "abi_version", "loaded_library",
+           "rms_norm", "rms_norm_e4m3", "rms_norm_backward", "linear", "linear_backward",
+           "gated_linear", "gated_linear_backward", "pack_weight_e4m3", "blocks_status",
+           "BLOCKS_LIB_PATH", "refine", "refine_workspace_bytes", "lib", "abi_version", "loaded_library",
            "LIB_PATH", "BVML_F32", "BVML_F16"]

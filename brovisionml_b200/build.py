@@ -7,7 +7,9 @@ or missing before this script has run.)
 
 Compiles each brovisionml_b200/csrc/*.cu with nvcc for
 ``-gencode arch=compute_100a,code=sm_100a`` (B200 only) and links them into
-``brovisionml_b200/_lib/libbvml_dsine.so``. The C++ drop-in bridge
+``brovisionml_b200/_lib/libbvml_dsine.so``, and csrc/blocks/*.cu (the
+feed-forward operators, include/bvml_blocks.h) into ``_lib/libbvml_blocks.so``.
+The C++ drop-in bridge
 (csrc/dsine_ops_b200.cpp) is compiled into ``_lib/libbvml_dsine_bridge.so``
 against the stand-in brotensor header, to prove that it builds.
 Rebuilds only what changed (source / header mtimes).
@@ -31,6 +33,8 @@ LIB = os.path.join(LIB_DIR, "libbvml_dsine.so")
 # coordinates before each access and records failures (bvml_check_word); the
 # GPU tests run the odd shapes through it.
 CHECKED_LIB = os.path.join(LIB_DIR, "libbvml_dsine_checked.so")
+BLOCKS = os.path.join(CSRC, "blocks")
+BLOCKS_LIB = os.path.join(LIB_DIR, "libbvml_blocks.so")
 BRIDGE = os.path.join(LIB_DIR, "libbvml_dsine_bridge.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -75,6 +79,18 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
         if _stale(cobj, [src] + headers):
             jobs.append([nvcc] + ARCH + NVCC_FLAGS + ["-DBVML_CHECKED", "-c", src, "-o", cobj])
 
+    # the feed-forward operators: a library of their own, so that the ABI of
+    # libbvml_dsine.so stays as it is
+    bheaders = headers + glob.glob(os.path.join(BLOCKS, "*.cuh")) + \
+        glob.glob(os.path.join(BLOCKS, "*.h"))
+    bobjs = []
+    for src in sorted(glob.glob(os.path.join(BLOCKS, "*.cu"))):
+        obj = os.path.join(OBJ_DIR, "blocks_" + os.path.basename(src)[:-3] + ".o")
+        bobjs.append(obj)
+        if _stale(obj, [src] + bheaders) or ptxas_info:
+            jobs.append([nvcc] + ARCH + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) +
+                        ["-c", src, "-o", obj])
+
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
@@ -85,6 +101,9 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
         for out in ex.map(run, jobs):
             if verbose or ptxas_info:
                 sys.stdout.write(out)
+    if _stale(BLOCKS_LIB, bobjs + [__file__]):
+        run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_LIB] + bobjs +
+            ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
     if _stale(LIB, objs + [__file__]):
         # Shared cudart: callers (torch, or a brotensor runtime) hand in stream
         # handles created by THEIR CUDA runtime; one shared runtime instance

@@ -1,0 +1,547 @@
+// RMS norm over rows of K features, with the residual's addition before it,
+// a 16 / 32-bit or an 8-bit output, and its backward pass.
+//
+//   forward   s = x + r,  q = sum_k s^2,  y = s * rsqrt(q / K + eps) * w
+//   8 bits    max_k |y| = rstd * max_k |s w|, so the row's scale comes out of
+//             the same reduction as q: one pass over the row
+//   backward  n = s rstd:  dx = rstd (dy w - n mean(dy w n)) + ds, dw = sum_t dy n
+//
+// Bound by HBM: every row is read once into registers (G threads a row, VPT
+// groups of eight elements a thread), reduced, and written from there. Rows of
+// up to 1024 features belong to a warp or part of one (no block barrier), longer
+// ones to a block; beyond 16 Ki features a block walks the row twice, the second
+// time out of L2. A block keeps its weights in registers over its rows, and the
+// backward pass its sums of dw, which it writes once: the sums over blocks
+// are a second small kernel, in a fixed order (no atomics).
+#include "blocks_common.cuh"
+#include "blocks_internal.h"
+
+namespace bvml {
+namespace blocks {
+namespace {
+
+constexpr int kNormThreads = 256;  // rows of at most a warp share a block of this size
+constexpr int kLongThreads = 512;
+// Below this a row's largest value counts as zero: 448 / max would overflow.
+constexpr float kTinyMax = 7.7e-34f;  // 2^-110
+
+struct NormArgs {
+    const void *x, *r, *w;
+    void *y, *sum;
+    float* scale;
+    long long ldx, ldr, ldy, lds;
+    int T, K;
+    int w32;  // weights are fp32 (else the rows' type)
+    int vec;  // every row starts on 16 bytes and K is a multiple of 8
+    float eps;
+};
+
+struct NormBwdArgs {
+    const void *dy, *s, *w, *ds;
+    void* dx;
+    float* partial;
+    long long lddy, lds, ldds, lddx;
+    int T, K, w32, vec;
+    float eps;
+};
+
+// the larger of two magnitudes, NaN if either is (fmaxf would drop it)
+__device__ __forceinline__ float max_nan(float m, float a) { return (a > m || a != a) ? a : m; }
+
+// Feature index of element e of group v of lane l: eight consecutive features
+// where vectors can be used, otherwise lanes side by side.
+template <int G>
+__device__ __forceinline__ int feature(int vec, int v, int e, int l) {
+    return vec ? (v * G + l) * 8 + e : (v * 8 + e) * G + l;
+}
+
+template <typename T, int G, int VPT>
+__device__ __forceinline__ void load_row(const T* p, int K, int vec, int l, float (&o)[VPT][8]) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        if (vec) {
+            const int k = (v * G + l) * 8;
+            if (k < K) {
+                load8(p + k, o[v]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[v][e] = 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = (v * 8 + e) * G + l;
+                o[v][e] = k < K ? to_f(p[k]) : 0.0f;
+            }
+        }
+    }
+}
+
+template <typename T, int G, int VPT>
+__device__ __forceinline__ void store_row(T* p, int K, int vec, int l, const float (&o)[VPT][8]) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        if (vec) {
+            const int k = (v * G + l) * 8;
+            if (k < K) store8(p + k, o[v]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = (v * 8 + e) * G + l;
+                if (k < K) p[k] = from_f<T>(o[v][e]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+    return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+
+template <int G, int VPT>
+__device__ __forceinline__ void store_row_e4m3(uint8_t* p, int K, int vec, int l,
+                                               const float (&o)[VPT][8]) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        if (vec) {
+            const int k = (v * G + l) * 8;
+            if (k < K) {
+                uint2 u;
+                uint16_t* h = reinterpret_cast<uint16_t*>(&u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    h[e] = __nv_cvt_float2_to_fp8x2(make_float2(o[v][2 * e], o[v][2 * e + 1]),
+                                                    __NV_SATFINITE, __NV_E4M3);
+                *reinterpret_cast<uint2*>(p + k) = u;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = (v * 8 + e) * G + l;
+                if (k < K) p[k] = to_e4m3(o[v][e]);
+            }
+        }
+    }
+}
+
+// Sum of a and (MAX) largest of b, or sum of both, over the G threads of a
+// row; every thread gets the result. G > 32: the whole block takes part;
+// `slot` alternates between rows, so that one barrier a row is enough.
+template <int G, bool MAX>
+__device__ __forceinline__ void row_reduce(float& a, float& b, float (*slots)[2][16], int slot) {
+    constexpr int kW = G < 32 ? G : 32;
+#pragma unroll
+    for (int d = kW / 2; d > 0; d >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, d);
+        const float o = __shfl_xor_sync(0xffffffffu, b, d);
+        b = MAX ? max_nan(b, o) : b + o;
+    }
+    if constexpr (G > 32) {
+        constexpr int kN = G / 32;
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) {
+            slots[slot][0][warp] = a;
+            slots[slot][1][warp] = b;
+        }
+        __syncthreads();
+        a = slots[slot][0][0];
+        b = slots[slot][1][0];
+#pragma unroll
+        for (int i = 1; i < kN; ++i) {
+            a += slots[slot][0][i];
+            b = MAX ? max_nan(b, slots[slot][1][i]) : b + slots[slot][1][i];
+        }
+    }
+}
+
+template <typename T, int G, int VPT, bool Q>
+__global__ void __launch_bounds__(G > 32 ? G : kNormThreads)
+rms_norm_kernel(const NormArgs a) {
+    constexpr int kThreads = G > 32 ? G : kNormThreads;
+    constexpr int kRows = kThreads / G;
+    __shared__ float slots[2][2][16];
+    const int l = threadIdx.x % G, g = threadIdx.x / G;
+    float w[VPT][8];
+    if (a.w32) load_row<float, G, VPT>(static_cast<const float*>(a.w), a.K, a.vec, l, w);
+    else load_row<T, G, VPT>(static_cast<const T*>(a.w), a.K, a.vec, l, w);
+    const float inv_k = 1.0f / (float)a.K;
+    int slot = 0;
+    // every thread of the block makes the same number of turns (barriers, shuffles)
+    for (long long t0 = (long long)blockIdx.x * kRows; t0 < a.T;
+         t0 += (long long)gridDim.x * kRows, slot ^= 1) {
+        const long long t = t0 + g;
+        const bool in = t < a.T;
+        float s[VPT][8];
+        if (in) {
+            load_row<T, G, VPT>(static_cast<const T*>(a.x) + t * a.ldx, a.K, a.vec, l, s);
+            if (a.r) {
+                float r[VPT][8];
+                load_row<T, G, VPT>(static_cast<const T*>(a.r) + t * a.ldr, a.K, a.vec, l, r);
+#pragma unroll
+                for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[v][e] += r[v][e];
+            }
+            if (a.sum) store_row<T, G, VPT>(static_cast<T*>(a.sum) + t * a.lds, a.K, a.vec, l, s);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[v][e] = 0.0f;
+        }
+        float q = 0.0f, m = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                q = fmaf(s[v][e], s[v][e], q);
+                s[v][e] *= w[v][e];
+                if constexpr (Q) m = max_nan(m, fabsf(s[v][e]));
+            }
+        }
+        row_reduce<G, true>(q, m, slots, slot);
+        if (!in) continue;
+        const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
+        float f = rstd;
+        if constexpr (Q) {
+            const float top = m * rstd;
+            const bool zero = top < kTinyMax;  // false for NaN, which goes through
+            if (l == 0) a.scale[t] = zero ? 1.0f : top * (1.0f / 448.0f);
+            f = zero ? 0.0f : rstd * (448.0f / top);
+        }
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[v][e] *= f;
+        if constexpr (Q)
+            store_row_e4m3<G, VPT>(static_cast<uint8_t*>(a.y) + t * a.ldy, a.K, a.vec, l, s);
+        else
+            store_row<T, G, VPT>(static_cast<T*>(a.y) + t * a.ldy, a.K, a.vec, l, s);
+    }
+}
+
+// Rows of more than 16 Ki features: a block a row, two walks over it.
+template <typename T, bool Q>
+__global__ void __launch_bounds__(kLongThreads)
+rms_norm_long_kernel(const NormArgs a) {
+    __shared__ float slots[2][2][16];
+    const float inv_k = 1.0f / (float)a.K;
+    int slot = 0;
+    auto wt = [&](int k) {
+        return a.w32 ? static_cast<const float*>(a.w)[k] : to_f(static_cast<const T*>(a.w)[k]);
+    };
+    for (long long t = blockIdx.x; t < a.T; t += gridDim.x, slot ^= 1) {
+        const T* x = static_cast<const T*>(a.x) + t * a.ldx;
+        const T* r = a.r ? static_cast<const T*>(a.r) + t * a.ldr : nullptr;
+        float q = 0.0f, m = 0.0f;
+        for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
+            const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
+            if (a.sum) static_cast<T*>(a.sum)[t * a.lds + k] = from_f<T>(s);
+            q = fmaf(s, s, q);
+            if constexpr (Q) m = max_nan(m, fabsf(s * wt(k)));
+        }
+        row_reduce<kLongThreads, true>(q, m, slots, slot);
+        const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
+        float f = rstd;
+        if constexpr (Q) {
+            const float top = m * rstd;
+            const bool zero = top < kTinyMax;
+            if (threadIdx.x == 0) a.scale[t] = zero ? 1.0f : top * (1.0f / 448.0f);
+            f = zero ? 0.0f : rstd * (448.0f / top);
+        }
+        for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
+            const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
+            const float y = s * wt(k) * f;
+            if constexpr (Q) static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(y);
+            else static_cast<T*>(a.y)[t * a.ldy + k] = from_f<T>(y);
+        }
+    }
+}
+
+template <typename T, int G, int VPT>
+__global__ void __launch_bounds__(G > 32 ? G : kNormThreads)
+rms_norm_backward_kernel(const NormBwdArgs a) {
+    constexpr int kThreads = G > 32 ? G : kNormThreads;
+    constexpr int kRows = kThreads / G;
+    __shared__ float slots[2][2][16];
+    __shared__ float part[kRows > 1 ? kThreads * VPT * 8 : 1];
+    const int l = threadIdx.x % G, g = threadIdx.x / G;
+    float w[VPT][8], dw[VPT][8];
+    if (a.w32) load_row<float, G, VPT>(static_cast<const float*>(a.w), a.K, a.vec, l, w);
+    else load_row<T, G, VPT>(static_cast<const T*>(a.w), a.K, a.vec, l, w);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[v][e] = 0.0f;
+    const float inv_k = 1.0f / (float)a.K;
+    int slot = 0;
+    for (long long t0 = (long long)blockIdx.x * kRows; t0 < a.T;
+         t0 += (long long)gridDim.x * kRows, slot ^= 1) {
+        const long long t = t0 + g;
+        const bool in = t < a.T;
+        float s[VPT][8], dy[VPT][8];
+        if (in) {
+            load_row<T, G, VPT>(static_cast<const T*>(a.s) + t * a.lds, a.K, a.vec, l, s);
+            load_row<T, G, VPT>(static_cast<const T*>(a.dy) + t * a.lddy, a.K, a.vec, l, dy);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[v][e] = dy[v][e] = 0.0f;
+        }
+        float q = 0.0f, p = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                q = fmaf(s[v][e], s[v][e], q);
+                p = fmaf(dy[v][e] * w[v][e], s[v][e], p);
+            }
+        }
+        row_reduce<G, false>(q, p, slots, slot);
+        if (!in) continue;
+        const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
+        const float c = p * inv_k * rstd * rstd;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                dw[v][e] = fmaf(dy[v][e], s[v][e] * rstd, dw[v][e]);
+                s[v][e] = rstd * fmaf(dy[v][e], w[v][e], -s[v][e] * c);
+            }
+        }
+        if (a.ds) {
+            load_row<T, G, VPT>(static_cast<const T*>(a.ds) + t * a.ldds, a.K, a.vec, l, dy);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[v][e] += dy[v][e];
+        }
+        store_row<T, G, VPT>(static_cast<T*>(a.dx) + t * a.lddx, a.K, a.vec, l, s);
+    }
+    float* out = a.partial + (long long)blockIdx.x * a.K;
+    if constexpr (kRows > 1) {
+        // the block's rows side by side: part[g][feature], summed in the order of g
+        constexpr int kPer = G * VPT * 8;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) part[g * kPer + feature<G>(a.vec, v, e, l)] = dw[v][e];
+        __syncthreads();
+        for (int k = threadIdx.x; k < a.K; k += kThreads) {
+            float v = part[k];
+#pragma unroll 4
+            for (int i = 1; i < kRows; ++i) v += part[i * kPer + k];
+            out[k] = v;
+        }
+    } else {
+        store_row<float, G, VPT>(out, a.K, a.vec, l, dw);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads)
+rms_norm_backward_long_kernel(const NormBwdArgs a) {
+    __shared__ float slots[2][2][16];
+    const float inv_k = 1.0f / (float)a.K;
+    float* out = a.partial + (long long)blockIdx.x * a.K;
+    auto wt = [&](int k) {
+        return a.w32 ? static_cast<const float*>(a.w)[k] : to_f(static_cast<const T*>(a.w)[k]);
+    };
+    int slot = 0;
+    bool first = true;
+    for (long long t = blockIdx.x; t < a.T; t += gridDim.x, slot ^= 1) {
+        const T* s = static_cast<const T*>(a.s) + t * a.lds;
+        const T* dy = static_cast<const T*>(a.dy) + t * a.lddy;
+        float q = 0.0f, p = 0.0f;
+        for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
+            const float sv = to_f(s[k]);
+            q = fmaf(sv, sv, q);
+            p = fmaf(to_f(dy[k]) * wt(k), sv, p);
+        }
+        row_reduce<kLongThreads, false>(q, p, slots, slot);
+        const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
+        const float c = p * inv_k * rstd * rstd;
+        for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
+            const float sv = to_f(s[k]), d = to_f(dy[k]);
+            float o = rstd * fmaf(d, wt(k), -sv * c);
+            if (a.ds) o += to_f(static_cast<const T*>(a.ds)[t * a.ldds + k]);
+            static_cast<T*>(a.dx)[t * a.lddx + k] = from_f<T>(o);
+            out[k] = fmaf(d, sv * rstd, first ? 0.0f : out[k]);  // a thread's own columns
+        }
+        first = false;
+    }
+}
+
+// 32 columns a block, 16 rows side by side
+template <typename T>
+__global__ void __launch_bounds__(512)
+column_sum_kernel(const float* __restrict__ part, int rows, int cols, T* __restrict__ out) {
+    __shared__ float sh[16][33];
+    const int c = blockIdx.x * 32 + threadIdx.x % 32, r0 = threadIdx.x / 32;
+    float v = 0.0f;
+    if (c < cols)
+        for (int r = r0; r < rows; r += 16) v += part[(long long)r * cols + c];
+    sh[r0][threadIdx.x % 32] = v;
+    __syncthreads();
+    if (r0 == 0 && c < cols) {
+        for (int i = 1; i < 16; ++i) v += sh[i][threadIdx.x];
+        out[c] = from_f<T>(v);
+    }
+}
+
+// Threads a row and groups of eight a thread, by the row's length: the fewest
+// registers that hold it.
+enum class Shape { G8, G16, G32x1, G32x2, G32x4, G256x1, G256x2, G512x2, G512x4, Long };
+Shape shape_of(int K) {
+    if (K <= 64) return Shape::G8;
+    if (K <= 128) return Shape::G16;
+    if (K <= 256) return Shape::G32x1;
+    if (K <= 512) return Shape::G32x2;
+    if (K <= 1024) return Shape::G32x4;
+    if (K <= 2048) return Shape::G256x1;
+    if (K <= 4096) return Shape::G256x2;
+    if (K <= 8192) return Shape::G512x2;
+    if (K <= 16384) return Shape::G512x4;
+    return Shape::Long;
+}
+int block_threads(Shape h) {
+    switch (h) {
+        case Shape::G512x2:
+        case Shape::G512x4:
+        case Shape::Long: return 512;
+        default: return 256;
+    }
+}
+int block_rows(Shape h) {
+    switch (h) {
+        case Shape::G8: return 32;
+        case Shape::G16: return 16;
+        case Shape::G32x1:
+        case Shape::G32x2:
+        case Shape::G32x4: return 8;
+        default: return 1;
+    }
+}
+
+template <typename T, bool Q>
+void norm_by_shape(Shape h, int grid, const NormArgs& a, cudaStream_t s) {
+    switch (h) {
+        case Shape::G8: rms_norm_kernel<T, 8, 1, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G16: rms_norm_kernel<T, 16, 1, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G32x1: rms_norm_kernel<T, 32, 1, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G32x2: rms_norm_kernel<T, 32, 2, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G32x4: rms_norm_kernel<T, 32, 4, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G256x1: rms_norm_kernel<T, 256, 1, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G256x2: rms_norm_kernel<T, 256, 2, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G512x2: rms_norm_kernel<T, 512, 2, Q><<<grid, 512, 0, s>>>(a); break;
+        case Shape::G512x4: rms_norm_kernel<T, 512, 4, Q><<<grid, 512, 0, s>>>(a); break;
+        case Shape::Long: rms_norm_long_kernel<T, Q><<<grid, kLongThreads, 0, s>>>(a); break;
+    }
+}
+
+template <typename T>
+void norm_backward_by_shape(Shape h, int grid, const NormBwdArgs& a, cudaStream_t s) {
+    switch (h) {
+        case Shape::G8: rms_norm_backward_kernel<T, 8, 1><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G16: rms_norm_backward_kernel<T, 16, 1><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G32x1: rms_norm_backward_kernel<T, 32, 1><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G32x2: rms_norm_backward_kernel<T, 32, 2><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G32x4: rms_norm_backward_kernel<T, 32, 4><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G256x1: rms_norm_backward_kernel<T, 256, 1><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G256x2: rms_norm_backward_kernel<T, 256, 2><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G512x2: rms_norm_backward_kernel<T, 512, 2><<<grid, 512, 0, s>>>(a); break;
+        case Shape::G512x4: rms_norm_backward_kernel<T, 512, 4><<<grid, 512, 0, s>>>(a); break;
+        case Shape::Long:
+            rms_norm_backward_long_kernel<T><<<grid, kLongThreads, 0, s>>>(a);
+            break;
+    }
+}
+
+}  // namespace
+
+cudaError_t sm_count(int* sms) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+}
+
+cudaError_t launch_rms_norm(const NormLaunch& L, cudaStream_t s) {
+    if (L.T == 0) return cudaSuccess;
+    int sms = 0;
+    cudaError_t e = sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    const size_t es = elem_size(L.type);
+    NormArgs a{L.x, L.r, L.w, L.y, L.sum, L.scale, L.ldx, L.ldr, L.ldy, L.lds, L.T, L.K};
+    a.w32 = L.wtype == BVML_F32;
+    a.eps = L.eps;
+    const bool y_ok = L.scale ? ((reinterpret_cast<uintptr_t>(L.y) | (uintptr_t)L.ldy) & 7) == 0
+                              : on16(L.y, L.ldy, es);
+    a.vec = L.K % 8 == 0 && on16(L.x, L.ldx, es) && (!L.r || on16(L.r, L.ldr, es)) &&
+            on16(L.w, 0, 1) && y_ok && (!L.sum || on16(L.sum, L.lds, es));
+    const Shape h = shape_of(L.K);
+    const int rows = block_rows(h);
+    const long long want = ((long long)L.T + rows - 1) / rows;
+    const long long most = (long long)sms * (2048 / block_threads(h));
+    const int grid = (int)(want < most ? want : most);
+    const bool q = L.scale != nullptr;
+    if (L.type == BVML_F32) {
+        if (q) norm_by_shape<float, true>(h, grid, a, s);
+        else norm_by_shape<float, false>(h, grid, a, s);
+    } else if (L.type == BVML_F16) {
+        if (q) norm_by_shape<__half, true>(h, grid, a, s);
+        else norm_by_shape<__half, false>(h, grid, a, s);
+    } else {
+        if (q) norm_by_shape<__nv_bfloat16, true>(h, grid, a, s);
+        else norm_by_shape<__nv_bfloat16, false>(h, grid, a, s);
+    }
+    return cudaGetLastError();
+}
+
+// Blocks of the backward pass, each with a row of partial sums: four blocks of
+// 256 threads an SM (half its threads) on 148 SMs at most. A constant and not
+// the device's count, so that the workspace's size needs no device.
+int norm_backward_parts(int T, int K) {
+    const Shape h = shape_of(K);
+    const long long rows = block_rows(h);
+    const long long want = ((long long)T + rows - 1) / rows;
+    const long long most = 148LL * (1024 / block_threads(h));
+    return (int)(want < most ? want : most);
+}
+
+cudaError_t launch_rms_norm_backward(const NormBackwardLaunch& L, cudaStream_t s) {
+    const int parts = norm_backward_parts(L.T, L.K);
+    if (parts > 0) {
+        const size_t es = elem_size(L.type);
+        NormBwdArgs a{L.dy, L.s, L.w, L.ds, L.dx, L.partial, L.lddy, L.lds, L.ldds, L.lddx,
+                      L.T, L.K};
+        a.w32 = L.wtype == BVML_F32;
+        a.eps = L.eps;
+        a.vec = L.K % 8 == 0 && on16(L.dy, L.lddy, es) && on16(L.s, L.lds, es) &&
+                (!L.ds || on16(L.ds, L.ldds, es)) && on16(L.w, 0, 1) && on16(L.dx, L.lddx, es);
+        const Shape h = shape_of(L.K);
+        if (L.type == BVML_F32) norm_backward_by_shape<float>(h, parts, a, s);
+        else if (L.type == BVML_F16) norm_backward_by_shape<__half>(h, parts, a, s);
+        else norm_backward_by_shape<__nv_bfloat16>(h, parts, a, s);
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    return launch_column_sum(L.partial, parts, L.K, L.dw, L.wtype, s);
+}
+
+cudaError_t launch_column_sum(const float* part, int rows, int cols, void* out, int type,
+                              cudaStream_t s) {
+    const int grid = (cols + 31) / 32;
+    if (type == BVML_F32)
+        column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols, static_cast<float*>(out));
+    else if (type == BVML_F16)
+        column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols, static_cast<__half*>(out));
+    else
+        column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols,
+                                               static_cast<__nv_bfloat16*>(out));
+    return cudaGetLastError();
+}
+
+}  // namespace blocks
+}  // namespace bvml
