@@ -1,104 +1,340 @@
-// Matrix products of the feed-forward operators, the simplest form: a 64 x 64
-// tile a block, 4 x 4 outputs a thread, fp32 FMAs over 16-wide slices of K in
-// shared memory. Takes every layout and stride.
+// Planning of the feed-forward operators' matrix products: which kernel, tile and
+// share of K, the tensor maps, the operands that have to be laid out anew, and the
+// sum over shares of K.
+#include <cudaTypedefs.h>
+
+#include <atomic>
+
 #include "blocks_common.cuh"
-#include "blocks_internal.h"
+#include "gemm_internal.h"
 
 namespace bvml {
 namespace blocks {
 namespace {
 
-__device__ __forceinline__ float fetch(const void* p, long long i, int type) {
-    switch (type) {
-        case BVML_F16: return to_f(static_cast<const __half*>(p)[i]);
-        case BVML_BF16: return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
-        case BVML_E4M3:
-            return float(*(reinterpret_cast<const __nv_fp8_e4m3*>(p) + i));
-        default: return static_cast<const float*>(p)[i];
-    }
+// The pairs of SMs that the plans count on (B200: 148 SMs). A constant, so that
+// a workspace's size needs no device; the launch takes the device's own count.
+constexpr int kPairs = 74;
+
+// An operand as stored: rows x cols, cols contiguous.
+struct Stored {
+    const void* p;
+    long long ld;
+    int rows, cols;
+    bool pack;         // its rows do not start on 16 bytes: copied to the workspace
+    size_t at;         // ... there
+    long long ld_packed;
+};
+
+struct Plan {
+    bool skinny;
+    int bn;        // tile: columns of a pair
+    int tok;       // skinny: tokens of a CTA
+    int splits;    // shares of K
+    int steps[2];
+    int tiles_m, tiles_n;
+    Stored a[2], b[2];
+    long long ldslab;
+    size_t slab;   // offset of the partial sums
+    size_t bytes;  // workspace
+};
+
+int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+
+// A product's cost in K steps of a 256-column tile, by the number of turns that the
+// pairs take. A narrower tile loads more bytes a flop and keeps the tensor cores
+// less busy, which the weights carry (measured on square products: 128 columns
+// run at about 0.9, 64 at about 0.7 of the rate of 256); `tail` is what a turn costs
+// beside its K steps (filling the ring, draining the last accumulator).
+double tile_cost(int tiles, int steps, int splits, int bn) {
+    const double rate = bn == 256 ? 1.0 : bn == 128 ? 0.56 : 0.36;
+    const double tail = bn == 256 ? 5.0 : bn == 128 ? 3.5 : 2.5;
+    const long long works = (long long)tiles * splits;
+    const long long turns = (works + kPairs - 1) / kPairs;
+    // joining the shares reads and writes the output once more for each
+    const double join = splits > 1 ? 4.0 + 0.5 * splits * tiles * bn / (256.0 * kPairs) : 0.0;
+    return turns * (rate * steps / splits + tail) + join;
 }
-__device__ __forceinline__ void put(void* p, long long i, int type, float v) {
-    switch (type) {
-        case BVML_F16: static_cast<__half*>(p)[i] = from_f<__half>(v); break;
-        case BVML_BF16: static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v); break;
-        default: static_cast<float*>(p)[i] = v;
+
+Plan plan_of(const GemmLaunch& L) {
+    Plan p{};
+    const bool f8 = L.in_type == BVML_E4M3;
+    const size_t es = elem_size(L.in_type);
+    const int step = f8 ? 128 : 64;
+    const int segs = L.k[1] > 0 ? 2 : 1;
+    for (int i = 0; i < 2; ++i) p.steps[i] = i < segs ? cdiv(L.k[i], step) : 0;
+    const int steps = p.steps[0] + p.steps[1];
+
+    // operands: A by segment, B by segment or gate and up
+    size_t off = 0;
+    auto stored = [&](const void* ptr, long long ld, int rows, int cols) {
+        Stored s{ptr, ld, rows, cols};
+        if (rows == 1) s.ld = cols;  // one row has no pitch
+        // (one row's pitch is made up where the tensor map is)
+        s.pack = rows == 1 ? (reinterpret_cast<uintptr_t>(ptr) & 15) != 0 : !on16(ptr, ld, es);
+        s.ld_packed = ((long long)cols * (long long)es + 15) / 16 * 16 / (long long)es;
+        if (s.pack) {
+            s.at = off;
+            off += round256((size_t)rows * s.ld_packed * es);
+        }
+        return s;
+    };
+    for (int i = 0; i < segs; ++i)
+        p.a[i] = L.a_t ? stored(L.a[i], L.lda[i], L.k[i], L.M)
+                       : stored(L.a[i], L.lda[i], L.M, L.k[i]);
+    for (int i = 0; i < (L.gated ? 2 : segs); ++i) {
+        const int k = L.gated ? L.k[0] : L.k[i];
+        p.b[i] = L.b_t ? stored(L.b[i], L.ldb[i], k, L.N) : stored(L.b[i], L.ldb[i], L.N, k);
+    }
+
+    p.splits = 1;
+    if (!L.a_t && !L.b_t && L.M <= 128) {
+        p.skinny = true;
+        p.tok = L.M <= 16 ? 16 : L.M <= 32 ? 32 : L.M <= 64 ? 64 : 128;
+        const int tiles = cdiv(L.N, L.gated ? 64 : 128);
+        while (p.splits < 8 && (long long)tiles * p.splits * 2 <= 4 * kPairs &&
+               steps >= 4 * p.splits)
+            p.splits *= 2;
+        p.bytes = off;
+        return p;
+    }
+    p.tiles_m = cdiv(L.M, 256);
+    // K is shared out only where nothing but the sum is wanted (the gradients):
+    // long sums over few output tiles
+    const bool plain = !L.gated && !L.bias && !L.residual && !L.save[0] && !L.row_scale &&
+                       L.act == BVML_ACT_NONE;
+    double best = 1e300;
+    for (int bn = 256; bn >= (L.b_t ? 128 : 64); bn /= 2) {
+        const int tn = cdiv(L.N, L.gated ? bn / 2 : bn);
+        for (int sp = 1; sp <= (plain ? 32 : 1) && (sp == 1 || steps / sp >= 8); sp *= 2) {
+            const double c = tile_cost(p.tiles_m * tn, steps, sp, bn);
+            if (c < best * 0.999) {
+                best = c;
+                p.bn = bn;
+                p.splits = sp;
+                p.tiles_n = tn;
+            }
+        }
+    }
+    p.slab = off;
+    if (p.splits > 1) {
+        p.ldslab = ((long long)L.N + 7) / 8 * 8;
+        off += round256((size_t)p.splits * L.M * p.ldslab * 4);
+    }
+    p.bytes = off;
+    return p;
+}
+
+// ------------------------------------------------------- operands laid out anew
+
+// Rows of `cols` elements to a pitch of 16-byte units, eight (16-bit) or sixteen
+// (8-bit) elements a thread; what pads a row's last unit is zeros.
+template <typename T>
+__global__ void __launch_bounds__(256)
+pack_kernel(const T* __restrict__ src, long long ld, int rows, int cols, T* __restrict__ dst,
+            int units) {
+    constexpr int kE = 16 / sizeof(T);
+    const long long total = (long long)rows * units;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (long long)gridDim.x * 256) {
+        const long long r = i / units;
+        const int c = (int)(i - r * units) * kE;
+        const T* s = src + r * ld + c;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int j = 0; j < kE; ++j)
+            if (c + j < cols) e[j] = s[j];
+        *reinterpret_cast<uint4*>(dst + i * kE) = u;
     }
 }
 
-__global__ void __launch_bounds__(256) gemm_kernel(const GemmLaunch L) {
-    __shared__ float sa[16][65], sb[2][16][65];
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[2][4][4] = {};
-    for (int seg = 0; seg < 2; ++seg) {
-        const int nb = L.gated ? 2 : 1;
-        for (int k0 = 0; k0 < L.k[seg]; k0 += 16) {
-            for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-                const int r = L.a_t ? i % 64 : i / 16, c = L.a_t ? i / 64 : i % 16;
-                const int m = m0 + r, k = k0 + c;
-                const long long at = L.a_t ? (long long)k * L.lda[seg] + m
-                                           : (long long)m * L.lda[seg] + k;
-                sa[c][r] = m < L.M && k < L.k[seg] ? fetch(L.a[seg], at, L.in_type) : 0.0f;
-            }
-            for (int q = 0; q < nb; ++q) {
-                const int src = L.gated ? q : seg;
-                for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-                    const int r = L.b_t ? i % 64 : i / 16, c = L.b_t ? i / 64 : i % 16;
-                    const int n = n0 + r, k = k0 + c;
-                    const long long at = L.b_t ? (long long)k * L.ldb[src] + n
-                                               : (long long)n * L.ldb[src] + k;
-                    sb[q][c][r] = n < L.N && k < L.k[seg] ? fetch(L.b[src], at, L.in_type) : 0.0f;
-                }
-            }
-            __syncthreads();
-            for (int q = 0; q < nb; ++q)
-                for (int c = 0; c < 16; ++c)
-                    for (int i = 0; i < 4; ++i)
-                        for (int j = 0; j < 4; ++j)
-                            acc[q][i][j] = fmaf(sa[c][ty * 4 + i], sb[q][c][tx * 4 + j],
-                                                acc[q][i][j]);
-            __syncthreads();
+cudaError_t pack(const Stored& s, size_t es, void* ws, cudaStream_t st) {
+    const int units = (int)(s.ld_packed * (long long)es / 16);
+    const long long total = (long long)s.rows * units;
+    const long long want = (total + 255) / 256;
+    const int grid = (int)(want < 148 * 16 ? want : 148 * 16);
+    void* d = static_cast<char*>(ws) + s.at;
+    if (es == 1)
+        pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(s.p), s.ld, s.rows, s.cols,
+                                          static_cast<uint8_t*>(d), units);
+    else
+        pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(s.p), s.ld, s.rows, s.cols,
+                                          static_cast<uint16_t*>(d), units);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------ the shares' sum
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_kernel(const float* __restrict__ slab, long long stride, long long lds, int splits, int N,
+            T* __restrict__ out, long long ldo, T* __restrict__ out2, long long ldo2, int rows0,
+            int rows1, bool vec) {
+    const long long m = blockIdx.x;
+    T* o;
+    if (!out2 || m < rows0) o = out + m * ldo;
+    else if (m >= rows1) o = out2 + (m - rows1) * ldo2;
+    else return;
+    for (int n = (blockIdx.y * 256 + threadIdx.x) * 8; n < N; n += gridDim.y * 256 * 8) {
+        float v[8], t[8];
+        load8(slab + m * lds + n, v);
+        for (int s = 1; s < splits; ++s) {
+            load8(slab + s * stride + m * lds + n, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += t[e];
+        }
+        if (vec && n + 8 <= N) {
+            store8(o + n, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < N) o[n + e] = from_f<T>(v[e]);
         }
     }
-    for (int i = 0; i < 4; ++i) {
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= L.M || n >= L.N) continue;
-            const float rs = L.row_scale ? L.row_scale[m] : 1.0f;
-            float v = acc[0][i][j] * rs * (L.col_scale[0] ? L.col_scale[0][n] : 1.0f);
-            if (L.gated) {
-                const float u = acc[1][i][j] * rs * (L.col_scale[1] ? L.col_scale[1][n] : 1.0f);
-                if (L.save[0]) {
-                    put(L.save[0], m * L.lds[0] + n, L.out_type, v);
-                    put(L.save[1], m * L.lds[1] + n, L.out_type, u);
-                }
-                v = act_f(v, L.act) * u;
-            } else {
-                if (L.bias) v += L.bias[n];
-                if (L.save[0]) put(L.save[0], m * L.lds[0] + n, L.out_type, v);
-                v = act_f(v, L.act);
-                if (L.residual) v += fetch(L.residual, m * L.ldr + n, L.out_type);
-            }
-            if (!L.out2 || m < L.rows0) put(L.out, m * L.ldo + n, L.out_type, v);
-            else if (m >= L.rows1) put(L.out2, (m - L.rows1) * L.ldo2 + n, L.out_type, v);
+}
+
+template <typename T>
+cudaError_t join(const GemmLaunch& L, const Plan& p, const float* slab, bool vec, cudaStream_t s) {
+    const dim3 grid(L.M, cdiv(L.N, 256 * 8));
+    join_kernel<<<grid, 256, 0, s>>>(slab, (long long)L.M * p.ldslab, p.ldslab, p.splits, L.N,
+                                     static_cast<T*>(L.out), L.ldo, static_cast<T*>(L.out2),
+                                     L.ldo2, L.rows0, L.rows1, vec);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ tensor maps
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> cached{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 fn = cached.load(std::memory_order_acquire);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess) {
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+            cached.store(fn, std::memory_order_release);
         }
     }
+    return fn;
+}
+
+// Boxes of 128 bytes x box_rows in the 128-byte swizzle; what lies outside the
+// matrix reads zeros.
+cudaError_t encode(CUtensorMap* m, const Stored& s, const void* ws, int type, int box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn = encoder();
+    if (!fn) return cudaErrorNotSupported;
+    const size_t es = elem_size(type);
+    const void* base = s.pack ? static_cast<const char*>(ws) + s.at : s.p;
+    const long long ld = s.pack || s.rows == 1 ? s.ld_packed : s.ld;
+    const cuuint64_t dims[2] = {(cuuint64_t)s.cols, (cuuint64_t)s.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * es};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
+    const cuuint32_t es1[2] = {1, 1};
+    const CUtensorMapDataType dt = type == BVML_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : type == BVML_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, es1,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+// MMA instruction descriptor: fp32 D; A and B bf16 (1), f16 or e4m3 (0);
+// transpose bits; N / 8 and M / 16.
+uint32_t idesc_of(int type, bool a_t, bool b_t, int M, int N) {
+    const uint32_t f = type == BVML_BF16 ? 1 : 0;
+    return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_t << 15) | ((uint32_t)b_t << 16) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 }  // namespace
 
-size_t gemm_workspace_bytes(const GemmLaunch&) { return 0; }
+size_t gemm_workspace_bytes(const GemmLaunch& L) {
+    if (L.M == 0 || L.N == 0 || L.k[0] == 0) return 0;
+    return plan_of(L).bytes;
+}
 
-cudaError_t launch_gemm(const GemmLaunch& L, void*, cudaStream_t s) {
+cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     if (L.M == 0 || L.N == 0) return cudaSuccess;
-    const dim3 grid((L.N + 63) / 64, (L.M + 63) / 64);
-    if (grid.y > 65535) return cudaErrorInvalidValue;
-    gemm_kernel<<<grid, 256, 0, s>>>(L);
-    return cudaGetLastError();
+    const Plan p = plan_of(L);
+    const size_t es = elem_size(L.in_type), eo = elem_size(L.out_type);
+    const int segs = p.steps[1] > 0 ? 2 : 1, nb = L.gated ? 2 : segs;
+    cudaError_t e = cudaSuccess;
+    TileMaps maps{};
+    const int rows_b = p.skinny ? (L.gated ? 64 : 128) : p.bn / 2;
+    for (int i = 0; i < segs && e == cudaSuccess; ++i) {
+        if (p.a[i].pack) e = pack(p.a[i], es, ws, s);
+        if (e == cudaSuccess)
+            e = encode(&maps.a[i], p.a[i], ws, L.in_type,
+                       L.a_t ? 64 : p.skinny ? p.tok : 128);
+    }
+    for (int i = 0; i < nb && e == cudaSuccess; ++i) {
+        if (p.b[i].pack) e = pack(p.b[i], es, ws, s);
+        if (e == cudaSuccess)
+            e = encode(&maps.b[i], p.b[i], ws, L.in_type, L.b_t ? 64 : rows_b);
+    }
+    if (e != cudaSuccess) return e;
+    SkinnyArgs k{};
+    TileArgs& a = k.t;
+    a.M = L.M, a.N = L.N;
+    a.steps[0] = p.steps[0], a.steps[1] = p.steps[1];
+    a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n;
+    a.splits = p.splits;
+    a.row_scale = L.row_scale;
+    for (int i = 0; i < 2; ++i) {
+        a.col_scale[i] = L.col_scale[i];
+        a.save[i] = L.save[i];
+        a.lds[i] = L.lds[i];
+    }
+    a.bias = L.bias, a.residual = L.residual, a.out = L.out, a.out2 = L.out2;
+    a.ldr = L.ldr, a.ldo = L.ldo, a.ldo2 = L.ldo2;
+    a.rows0 = L.rows0, a.rows1 = L.rows1;
+    a.out_type = L.out_type, a.act = L.act;
+    if (p.skinny) {
+        k.split = p.splits;
+        a.idesc = idesc_of(L.in_type, false, false, 128, p.tok);
+        return launch_skinny(p.tok, L.in_type == BVML_E4M3, L.gated, maps, k, s);
+    }
+    const bool out_ok = on16(L.out, L.ldo, eo), out2_ok = !L.out2 || on16(L.out2, L.ldo2, eo);
+    if (out_ok) a.vec |= kVecOut;
+    if (out2_ok) a.vec |= kVecOut2;
+    if (L.residual && on16(L.residual, L.ldr, eo)) a.vec |= kVecRes;
+    if (L.save[0] && on16(L.save[0], L.lds[0], eo) &&
+        (!L.save[1] || on16(L.save[1], L.lds[1], eo)))
+        a.vec |= kVecSave;
+    a.idesc = idesc_of(L.in_type, L.a_t, L.b_t, 256, p.bn);
+    if (p.splits > 1) {
+        a.slab = reinterpret_cast<float*>(static_cast<char*>(ws) + p.slab);
+        a.ldslab = p.ldslab;
+    }
+    int sms = 0;
+    if ((e = sm_count(&sms)) != cudaSuccess) return e;
+    const long long works = (long long)p.tiles_m * p.tiles_n * p.splits;
+    const int pairs = (int)(works < sms / 2 ? works : sms / 2);
+    if (L.b_t) e = launch_tile_grad(p.bn, L.a_t, maps, a, pairs, s);
+    else if (L.in_type == BVML_E4M3) e = launch_tile_nt_f8(p.bn, L.gated, maps, a, pairs, s);
+    else e = launch_tile_nt(p.bn, L.gated, maps, a, pairs, s);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    const bool vec = out_ok && out2_ok;
+    if (L.out_type == BVML_F16) return join<__half>(L, p, a.slab, vec, s);
+    if (L.out_type == BVML_BF16) return join<__nv_bfloat16>(L, p, a.slab, vec, s);
+    return join<float>(L, p, a.slab, vec, s);
 }
 
 cudaError_t gemm_errors(int* word) {
     *word = 0;
+    cudaError_t (*readers[])(int*) = {tile_nt_error, tile_nt_f8_error, tile_grad_error,
+                                      skinny_error};
+    for (auto r : readers) {
+        int w = 0;
+        const cudaError_t e = r(&w);
+        if (e != cudaSuccess) return e;
+        if (w) *word = w;
+    }
     return cudaSuccess;
 }
 

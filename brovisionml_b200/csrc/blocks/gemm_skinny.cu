@@ -1,0 +1,240 @@
+// Products with few rows (decoding: one to 128 tokens), bound by reading the
+// weights once: out[t, n] = sum_k w[n, k] x[t, k].
+//
+// The weights are the MMA's 128 rows and the tokens its columns (16 to 128), so
+// that one token costs no more tensor-core time than sixteen and every byte that a
+// CTA loads is weight. To have enough loads in flight with few weight rows, K is
+// shared out over a cluster of up to eight CTAs; each leaves its 128 x tokens fp32
+// partial sums in its shared memory, and every CTA adds up a share of the rows over
+// the cluster through distributed shared memory, in the order of the ranks
+// (no atomics, no workspace, one launch). Gated: a CTA takes 64 rows of each
+// projection, and pairs them up where it adds.
+#include "gemm_tile.cuh"
+
+namespace bvml {
+namespace blocks {
+namespace {
+
+constexpr int kSkinnyThreads = 256;
+constexpr int kSkinnyPitch = 132;  // floats between two tokens' partial sums
+
+template <int TOK> constexpr int skinny_stage_bytes() { return (128 + TOK) * 128; }
+template <int TOK> constexpr int skinny_stages() {
+    // three CTAs an SM with few tokens, two with more: 72 and 96 KB
+    return (TOK <= 16 ? 73728 : 98304) / skinny_stage_bytes<TOK>();
+}
+template <int TOK> constexpr int skinny_smem_bytes() {
+    // 1024-aligned ring (the partial sums take its place), barriers
+    return 1024 + skinny_stages<TOK>() * skinny_stage_bytes<TOK>() + 256;
+}
+
+__device__ __forceinline__ void put1(void* p, long long i, int type, float v) {
+    if (type == BVML_BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
+    else if (type == BVML_F16) static_cast<__half*>(p)[i] = from_f<__half>(v);
+    else static_cast<float*>(p)[i] = v;
+}
+__device__ __forceinline__ float get1(const void* p, long long i, int type) {
+    if (type == BVML_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
+    if (type == BVML_F16) return to_f(static_cast<const __half*>(p)[i]);
+    return static_cast<const float*>(p)[i];
+}
+
+template <int TOK, bool F8, bool GATED>
+__global__ void __launch_bounds__(kSkinnyThreads)
+skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
+    constexpr int kStage = skinny_stage_bytes<TOK>();
+    constexpr int kStages = skinny_stages<TOK>();
+    static_assert(TOK * kSkinnyPitch * 4 <= kStages * kStage, "partial sums fit the ring");
+    constexpr int kStep = F8 ? 128 : 64;
+    constexpr uint32_t kCols = TOK < 32 ? 32 : TOK;
+    constexpr int kFeatures = GATED ? 64 : 128;
+    const TileArgs& a = sa.t;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const uint32_t sbase = tc::smem_u32(smem);
+    uint8_t* bar_mem = smem + kStages * kStage;
+    const uint32_t bar_full = tc::smem_u32(bar_mem), bar_empty = bar_full + 64,
+                   bar_acc = bar_full + 128;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 136);
+    int* abort_flag = reinterpret_cast<int*>(bar_mem + 140);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = sa.split;
+    const int rank = blockIdx.x % split;  // the cluster's CTAs are neighbours in x
+    const int f0 = (blockIdx.x / split) * kFeatures, t0 = blockIdx.y * TOK;
+    const int k0 = (int)((long long)a.steps[0] * rank / split);
+    const int k1 = (int)((long long)a.steps[0] * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            tc::mbar_init(bar_full + 8 * s, 1);
+            tc::mbar_init(bar_empty + 8 * s, 1);
+        }
+        tc::mbar_init(bar_acc, 1);
+        *abort_flag = 0;
+        tc::mbar_fence_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tc::smem_u32(tmem_slot), kCols);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    auto fail = [&](int code) {
+        atomicExch(&g_tile_error, code);
+        *reinterpret_cast<volatile int*>(abort_flag) = 1;
+    };
+    if (warp == 0 && lane == 0) {
+        int i = 0;
+        for (int k = k0; k < k1; ++k, ++i) {
+            const int s = i % kStages, j = i / kStages;
+            if (j > 0 &&
+                !tc::mbar_wait_pipe(bar_empty + 8 * s, (j - 1) & 1, kTileWaitLimit)) {
+                fail(11);
+                break;
+            }
+            if (*reinterpret_cast<volatile int*>(abort_flag)) break;
+            tc::mbar_expect_tx(bar_full + 8 * s, kStage);
+            const uint32_t d = sbase + s * kStage;
+            tc::tma_load_2d(d, &maps.b[0], bar_full + 8 * s, k * kStep, f0);
+            if constexpr (GATED)
+                tc::tma_load_2d(d + 8192, &maps.b[1], bar_full + 8 * s, k * kStep, f0);
+            tc::tma_load_2d(d + 128 * 128, &maps.a[0], bar_full + 8 * s, k * kStep, t0);
+        }
+        // no copy may still be landing when the ring is used anew
+        for (int q = i > kStages ? i - kStages : 0; q < i; ++q)
+            if (!tc::mbar_wait(bar_full + 8 * (q % kStages), (q / kStages) & 1, kTileWaitLimit)) {
+                fail(12);
+                break;
+            }
+    } else if (warp == 1 && lane == 0) {
+        int i = 0;
+        for (int k = k0; k < k1; ++k, ++i) {
+            const int s = i % kStages;
+            if (!tc::mbar_wait_pipe(bar_full + 8 * s, (i / kStages) & 1, kTileWaitLimit) ||
+                *reinterpret_cast<volatile int*>(abort_flag)) {
+                fail(13);
+                break;
+            }
+            tc::tc_fence_after();
+            const uint64_t dw = tc::umma_desc_k_sw128(sbase + s * kStage);
+            const uint64_t dx = tc::umma_desc_k_sw128(sbase + s * kStage + 128 * 128);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                tc::umma_single<F8>(tmem, dw + 2 * q, dx + 2 * q, a.idesc, i > 0 || q > 0);
+            tc::umma_commit(bar_empty + 8 * s);
+        }
+        tc::umma_commit(bar_acc);
+    }
+    __syncwarp();
+    // the accumulator, and with it every copy and MMA, is complete
+    if (!tc::mbar_wait(bar_acc, 0, kTileWaitLimit)) fail(14);
+    __syncthreads();  // ... also the producer's look at its last copies
+    tc::tc_fence_after();
+    // partial[token][row]: a lane is a row, so a warp writes 32 neighbours
+    float* partial = reinterpret_cast<float*>(smem);
+    {
+        const int quarter = warp & 3, half = warp >> 2;
+        constexpr int kPer = TOK < 32 ? 16 : TOK / 2;  // columns of a warp
+        if (half * kPer < TOK) {
+#pragma unroll
+            for (int c = 0; c < kPer; c += 16) {
+                uint32_t v[16];
+                tc::tmem_ld_16cols(tmem + ((uint32_t)(quarter * 32) << 16) + half * kPer + c, v);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    partial[(half * kPer + c + e) * kSkinnyPitch + quarter * 32 + lane] =
+                        __uint_as_float(v[e]);
+            }
+        }
+        tc::tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) tc::tmem_dealloc(tmem, kCols);
+    __syncwarp();
+    tc::cluster_sync();
+    const int share = kFeatures / split;  // features this CTA adds up
+    const int toks = a.M - t0 < TOK ? a.M - t0 : TOK;
+    for (int i = threadIdx.x; i < share * toks; i += kSkinnyThreads) {
+        const int f = rank * share + i % share, t = i / share;
+        const uint32_t at = sbase + 4 * (t * kSkinnyPitch + f);
+        float v = 0.0f, u = 0.0f;
+        for (int r = 0; r < split; ++r) {
+            v += tc::ld_cluster(tc::map_to(at, r));
+            if constexpr (GATED) u += tc::ld_cluster(tc::map_to(at + 4 * 64, r));
+        }
+        const int n = f0 + f;
+        const long long m = t0 + t;
+        if (n >= a.N) continue;
+        if (a.col_scale[0]) {
+            const float rs = a.row_scale[m];
+            v *= rs * a.col_scale[0][n];
+            if constexpr (GATED) u *= rs * a.col_scale[1][n];
+        }
+        if constexpr (GATED) {
+            if (a.save[0]) {
+                put1(a.save[0], m * a.lds[0] + n, a.out_type, v);
+                put1(a.save[1], m * a.lds[1] + n, a.out_type, u);
+            }
+            v = act_f(v, a.act) * u;
+        } else {
+            if (a.bias) v += a.bias[n];
+            if (a.save[0]) put1(a.save[0], m * a.lds[0] + n, a.out_type, v);
+            v = act_f(v, a.act);
+            if (a.residual) v += get1(a.residual, m * a.ldr + n, a.out_type);
+        }
+        put1(a.out, m * a.ldo + n, a.out_type, v);
+    }
+    tc::cluster_sync();  // no CTA leaves while another still reads its sums
+}
+
+template <int TOK, bool F8, bool GATED>
+cudaError_t launch_one(const TileMaps& m, const SkinnyArgs& a, cudaStream_t s) {
+    auto kern = skinny_kernel<TOK, F8, GATED>;
+    constexpr int smem = skinny_smem_bytes<TOK>();
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    constexpr int kFeatures = GATED ? 64 : 128;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((a.t.N + kFeatures - 1) / kFeatures * a.split),
+                       (unsigned)((a.t.M + TOK - 1) / TOK));
+    cfg.blockDim = dim3(kSkinnyThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)a.split;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, m, a);
+}
+
+template <bool F8, bool GATED>
+cudaError_t by_tokens(int tok, const TileMaps& m, const SkinnyArgs& a, cudaStream_t s) {
+    switch (tok) {
+        case 16: return launch_one<16, F8, GATED>(m, a, s);
+        case 32: return launch_one<32, F8, GATED>(m, a, s);
+        case 64: return launch_one<64, F8, GATED>(m, a, s);
+        default: return launch_one<128, F8, GATED>(m, a, s);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_skinny(int tok, bool f8, bool gated, const TileMaps& m, const SkinnyArgs& a,
+                          cudaStream_t s) {
+    if (f8) return gated ? by_tokens<true, true>(tok, m, a, s) : by_tokens<true, false>(tok, m, a, s);
+    return gated ? by_tokens<false, true>(tok, m, a, s) : by_tokens<false, false>(tok, m, a, s);
+}
+
+BVML_TILE_ERROR_READER(skinny_error)
+
+}  // namespace blocks
+}  // namespace bvml
