@@ -206,6 +206,11 @@ def _vec(op: str, t: torch.Tensor | None, name: str, n: int, dtype: torch.dtype 
     return t.data_ptr()
 
 
+# The current stream's handle without a Stream object around it (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _On:
     """Makes `dev` the current device for a launch, when it is not."""
     __slots__ = ("guard",)
@@ -228,7 +233,7 @@ def _run(fn, ws_fn, args, dev: torch.device, need: int | None = None) -> None:
     call needs none)."""
     p = ctypes.byref(args)
     with _On(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
+        stream = _raw_stream(dev.index)
         if need is None:
             rc = fn(p, None, 0, stream)
             if rc != BVML_EWORKSPACE:
@@ -237,6 +242,12 @@ def _run(fn, ws_fn, args, dev: torch.device, need: int | None = None) -> None:
             need = ws_fn(p)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _check(fn(p, None if ws is None else ws.data_ptr(), need, stream))
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor like t."""
+    return torch.empty_like(t) if t.is_contiguous() else \
+        torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _new(rows_of: torch.Tensor, cols: int, dtype: torch.dtype, dev: torch.device):
@@ -269,12 +280,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     is taken of the unrounded sum."""
     op = "rms_norm"
     dev, px, ldx, T, K, ty, wt, pw, pr, ldr = _norm_inputs(op, x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    s = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    y = _like(x)
+    s = _like(x) if residual is not None else None
     with _On(dev):
         _check(_norm(px, ldx, pr, ldr, pw, T, K, ty, wt, eps, y.data_ptr(), K,
                      None if s is None else s.data_ptr(), K,
-                     torch.cuda.current_stream(dev).cuda_stream))
+                     _raw_stream(dev.index)))
     return y if s is None else (y, s)
 
 
@@ -288,11 +299,11 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     dev, px, ldx, T, K, ty, wt, pw, pr, ldr = _norm_inputs(op, x, weight, residual)
     q = torch.empty(x.shape, dtype=_E4M3, device=dev)
     scale = torch.empty(x.shape[:-1], dtype=_F32, device=dev)
-    s = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    s = _like(x) if residual is not None else None
     with _On(dev):
         _check(_norm_e4m3(px, ldx, pr, ldr, pw, T, K, ty, wt, eps, q.data_ptr(), K,
                           scale.data_ptr(), None if s is None else s.data_ptr(), K,
-                          torch.cuda.current_stream(dev).cuda_stream))
+                          _raw_stream(dev.index)))
     return (q, scale) if s is None else (q, scale, s)
 
 
@@ -314,14 +325,14 @@ def rms_norm_backward(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor,
     if dsum is not None:
         pr, ldr, _, _ = _rows(op, dsum, "dsum", K, T, s.dtype)
     ty = _type(op, s.dtype)
-    dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
+    dx = _like(s)
     dw = torch.empty((K,), dtype=weight.dtype, device=dev)
     need = _norm_bwd_ws(T, K)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     with _On(dev):
         _check(_norm_bwd(pd, ldd, ps, lds, pw, pr, ldr, T, K, ty, _TYPES[weight.dtype], eps,
                          dx.data_ptr(), K, dw.data_ptr(), ws.data_ptr(), need,
-                         torch.cuda.current_stream(dev).cuda_stream))
+                         _raw_stream(dev.index)))
     return dx, dw
 
 
@@ -400,7 +411,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         if z.shape != dy.shape:
             raise _err(op, "z must have dy's shape")
         pz, ldz, _, _ = _rows(op, z, "z", N, T, x.dtype)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if dx else None
+    gx = _like(x) if dx else None
     gw = torch.empty((N, K), dtype=x.dtype, device=dev) if dw else None
     gb = torch.empty((N,), dtype=_F32, device=dev) if bias else None
     a = LinearBackwardArgs(pd, pz, px, pw, None if gx is None else gx.data_ptr(),
@@ -453,7 +464,7 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
     pd, ldd, _, _ = _rows(op, dh, "dh", F, T, x.dtype)
     pgv, ldgv, _, _ = _rows(op, g, "g", F, T, x.dtype)
     puv, lduv, _, _ = _rows(op, u, "u", F, T, x.dtype)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if dx else None
+    gx = _like(x) if dx else None
     gg, gu = (torch.empty((F, K), dtype=x.dtype, device=dev) for _ in range(2)) if dw \
         else (None, None)
     a = GatedBackwardArgs(pd, pgv, puv, px, pg, pu, None if gx is None else gx.data_ptr(),

@@ -77,27 +77,55 @@ act_backward_kernel(const ActBackwardLaunch L, bool vec_dy, bool vec_z, bool vec
     }
 }
 
+// g, u <- dh u act'(g), dh act(g); the activation is chosen outside the loops
+__device__ __forceinline__ void grad_rows(int act, const float (&dh)[2][8], float (&g)[2][8],
+                                          float (&u)[2][8]) {
+    switch (act) {
+#define BVML_GRAD_ROWS(code)                                  \
+    case code:                                                \
+        _Pragma("unroll") for (int i = 0; i < 2; ++i)         \
+            _Pragma("unroll") for (int e = 0; e < 8; ++e) {   \
+                float f, d;                                   \
+                act_grad_f(g[i][e], code, f, d);              \
+                g[i][e] = dh[i][e] * u[i][e] * d;             \
+                u[i][e] = dh[i][e] * f;                       \
+            }                                                 \
+        break;
+        BVML_GRAD_ROWS(BVML_ACT_RELU)
+        BVML_GRAD_ROWS(BVML_ACT_SIGMOID)
+        BVML_GRAD_ROWS(BVML_ACT_TANH)
+        BVML_GRAD_ROWS(BVML_ACT_SILU)
+        BVML_GRAD_ROWS(BVML_ACT_GELU)
+#undef BVML_GRAD_ROWS
+        default: break;
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kCols)
 gated_backward_kernel(const GatedBackwardLaunch L, bool vec_h, bool vec_g, bool vec_u, bool vec_d) {
     const int lane = threadIdx.x % 32, ry = threadIdx.x / 32;
     const int c = blockIdx.x * kCols + lane * 8;
     if (c >= L.F) return;
-    for (long long t = (long long)blockIdx.y * kRowThreads + ry; t < L.T;
-         t += (long long)gridDim.y * kRowThreads) {
-        float dh[8], g[8], u[8];
-        load_cols(static_cast<const T*>(L.dh) + t * L.lddh, c, L.F, vec_h, dh);
-        load_cols(static_cast<const T*>(L.g) + t * L.ldg, c, L.F, vec_g, g);
-        load_cols(static_cast<const T*>(L.u) + t * L.ldu, c, L.F, vec_u, u);
+    // two rows at a time: six loads in flight a thread
+    const long long stride = (long long)gridDim.y * kRowThreads;
+    for (long long t0 = (long long)blockIdx.y * kRowThreads + ry; t0 < L.T; t0 += 2 * stride) {
+        float dh[2][8], g[2][8], u[2][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float f, d;
-            act_grad_f(g[e], L.act, f, d);
-            g[e] = dh[e] * u[e] * d;
-            u[e] = dh[e] * f;
+        for (int i = 0; i < 2; ++i) {
+            const long long t = t0 + i * stride < L.T ? t0 + i * stride : t0;
+            load_cols(static_cast<const T*>(L.dh) + t * L.lddh, c, L.F, vec_h, dh[i]);
+            load_cols(static_cast<const T*>(L.g) + t * L.ldg, c, L.F, vec_g, g[i]);
+            load_cols(static_cast<const T*>(L.u) + t * L.ldu, c, L.F, vec_u, u[i]);
         }
-        store_cols(static_cast<T*>(L.dg) + t * L.ldd, c, L.F, vec_d, g);
-        store_cols(static_cast<T*>(L.du) + t * L.ldd, c, L.F, vec_d, u);
+        grad_rows(L.act, dh, g, u);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const long long t = t0 + i * stride;
+            if (t >= L.T) continue;
+            store_cols(static_cast<T*>(L.dg) + t * L.ldd, c, L.F, vec_d, g[i]);
+            store_cols(static_cast<T*>(L.du) + t * L.ldd, c, L.F, vec_d, u[i]);
+        }
     }
 }
 

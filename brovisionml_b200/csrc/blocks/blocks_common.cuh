@@ -56,8 +56,13 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     }
 }
 
-// sigmoid: exp overflows to infinity for z below -88, where 1 / inf = 0 is the value
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.0f / (1.0f + expf(-z)); }
+// sigmoid: exp overflows to infinity for z below -88, where 1 / inf = 0 is the
+// value. The fast exponential and division: a relative error of a few 2^-24 and
+// |z| 2^-24 (on what is rounded to 16 bits as a rule), in a third of the
+// instructions, which bound the elementwise kernels.
+__device__ __forceinline__ float sigmoid_f(float z) {
+    return __fdividef(1.0f, 1.0f + __expf(-z));
+}
 
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
@@ -101,7 +106,7 @@ __device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d)
         case BVML_ACT_GELU: {
             const float phi = 0.5f * (1.0f + erff(z * kSqrtHalf));
             f = z * phi;
-            d = phi + z * kInvSqrt2Pi * expf(-0.5f * z * z);
+            d = phi + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
             break;
         }
         default: f = z; d = 1.0f;

@@ -92,8 +92,9 @@ Plan plan_of(const GemmLaunch& L) {
         p.skinny = true;
         p.tok = L.M <= 16 ? 16 : L.M <= 32 ? 32 : L.M <= 64 ? 64 : 128;
         const int tiles = cdiv(L.N, L.gated ? 64 : 128);
-        while (p.splits < 8 && (long long)tiles * p.splits * 2 <= 4 * kPairs &&
-               steps >= 4 * p.splits)
+        // up to what the SMs hold at once, and at least two K steps a CTA
+        const int slots = 2 * kPairs * (p.tok <= 64 ? 3 : 2);
+        while (p.splits < 8 && (long long)tiles * p.splits * 2 <= slots && steps >= 4 * p.splits)
             p.splits *= 2;
         p.bytes = off;
         return p;

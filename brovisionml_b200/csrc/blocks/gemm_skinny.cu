@@ -20,8 +20,8 @@ constexpr int kSkinnyPitch = 132;  // floats between two tokens' partial sums
 
 template <int TOK> constexpr int skinny_stage_bytes() { return (128 + TOK) * 128; }
 template <int TOK> constexpr int skinny_stages() {
-    // three CTAs an SM with few tokens, two with more: 72 and 96 KB
-    return (TOK <= 16 ? 73728 : 98304) / skinny_stage_bytes<TOK>();
+    // three CTAs an SM with up to 64 tokens, two with more: 72 and 96 KB
+    return (TOK <= 64 ? 73728 : 98304) / skinny_stage_bytes<TOK>();
 }
 template <int TOK> constexpr int skinny_smem_bytes() {
     // 1024-aligned ring (the partial sums take its place), barriers
@@ -37,6 +37,61 @@ __device__ __forceinline__ float get1(const void* p, long long i, int type) {
     if (type == BVML_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
     if (type == BVML_F16) return to_f(static_cast<const __half*>(p)[i]);
     return static_cast<const float*>(p)[i];
+}
+
+// This CTA's share of the features, summed over the cluster's SPLIT CTAs and
+// finished: four neighbouring features of a token a thread and turn, all the
+// shares' loads in flight at once.
+template <int SPLIT, bool GATED>
+__device__ __forceinline__ void add_up(const TileArgs& a, uint32_t sbase, int rank, int f0, int t0,
+                                       int tok) {
+    constexpr int kShare = (GATED ? 64 : 128) / SPLIT;
+    constexpr int kQuads = kShare / 4;
+    const int toks = a.M - t0 < tok ? a.M - t0 : tok;
+    uint32_t base[SPLIT];
+#pragma unroll
+    for (int r = 0; r < SPLIT; ++r) base[r] = tc::map_to(sbase, r);
+    for (int i = threadIdx.x; i < kQuads * toks; i += kSkinnyThreads) {
+        const int f = rank * kShare + i % kQuads * 4, t = i / kQuads;
+        const uint32_t at = 4 * (t * kSkinnyPitch + f);
+        float4 p[SPLIT], q[SPLIT];
+#pragma unroll
+        for (int r = 0; r < SPLIT; ++r) {
+            p[r] = tc::ld_cluster4(base[r] + at);
+            if constexpr (GATED) q[r] = tc::ld_cluster4(base[r] + at + 4 * 64);
+        }
+        float v[4] = {p[0].x, p[0].y, p[0].z, p[0].w}, u[4];
+        if constexpr (GATED) u[0] = q[0].x, u[1] = q[0].y, u[2] = q[0].z, u[3] = q[0].w;
+#pragma unroll
+        for (int r = 1; r < SPLIT; ++r) {
+            v[0] += p[r].x, v[1] += p[r].y, v[2] += p[r].z, v[3] += p[r].w;
+            if constexpr (GATED) u[0] += q[r].x, u[1] += q[r].y, u[2] += q[r].z, u[3] += q[r].w;
+        }
+        const long long m = t0 + t;
+        const float rs = a.row_scale ? a.row_scale[m] : 1.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int n = f0 + f + e;
+            if (n >= a.N) break;
+            if (a.col_scale[0]) {
+                v[e] *= rs * a.col_scale[0][n];
+                if constexpr (GATED) u[e] *= rs * a.col_scale[1][n];
+            }
+            if constexpr (GATED) {
+                if (a.save[0]) {
+                    put1(a.save[0], m * a.lds[0] + n, a.out_type, v[e]);
+                    put1(a.save[1], m * a.lds[1] + n, a.out_type, u[e]);
+                }
+                v[e] = act_f(v[e], a.act) * u[e];
+            } else {
+                if (a.bias) v[e] += a.bias[n];
+                if (a.save[0]) put1(a.save[0], m * a.lds[0] + n, a.out_type, v[e]);
+                v[e] = act_f(v[e], a.act);
+                if (a.residual) v[e] += get1(a.residual, m * a.ldr + n, a.out_type);
+            }
+            put1(a.out, m * a.ldo + n, a.out_type, v[e]);
+        }
+    }
 }
 
 template <int TOK, bool F8, bool GATED>
@@ -158,37 +213,11 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     if (warp == 1) tc::tmem_dealloc(tmem, kCols);
     __syncwarp();
     tc::cluster_sync();
-    const int share = kFeatures / split;  // features this CTA adds up
-    const int toks = a.M - t0 < TOK ? a.M - t0 : TOK;
-    for (int i = threadIdx.x; i < share * toks; i += kSkinnyThreads) {
-        const int f = rank * share + i % share, t = i / share;
-        const uint32_t at = sbase + 4 * (t * kSkinnyPitch + f);
-        float v = 0.0f, u = 0.0f;
-        for (int r = 0; r < split; ++r) {
-            v += tc::ld_cluster(tc::map_to(at, r));
-            if constexpr (GATED) u += tc::ld_cluster(tc::map_to(at + 4 * 64, r));
-        }
-        const int n = f0 + f;
-        const long long m = t0 + t;
-        if (n >= a.N) continue;
-        if (a.col_scale[0]) {
-            const float rs = a.row_scale[m];
-            v *= rs * a.col_scale[0][n];
-            if constexpr (GATED) u *= rs * a.col_scale[1][n];
-        }
-        if constexpr (GATED) {
-            if (a.save[0]) {
-                put1(a.save[0], m * a.lds[0] + n, a.out_type, v);
-                put1(a.save[1], m * a.lds[1] + n, a.out_type, u);
-            }
-            v = act_f(v, a.act) * u;
-        } else {
-            if (a.bias) v += a.bias[n];
-            if (a.save[0]) put1(a.save[0], m * a.lds[0] + n, a.out_type, v);
-            v = act_f(v, a.act);
-            if (a.residual) v += get1(a.residual, m * a.ldr + n, a.out_type);
-        }
-        put1(a.out, m * a.ldo + n, a.out_type, v);
+    switch (split) {
+        case 1: add_up<1, GATED>(a, sbase, rank, f0, t0, TOK); break;
+        case 2: add_up<2, GATED>(a, sbase, rank, f0, t0, TOK); break;
+        case 4: add_up<4, GATED>(a, sbase, rank, f0, t0, TOK); break;
+        default: add_up<8, GATED>(a, sbase, rank, f0, t0, TOK); break;
     }
     tc::cluster_sync();  // no CTA leaves while another still reads its sums
 }

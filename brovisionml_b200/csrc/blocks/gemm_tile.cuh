@@ -62,97 +62,159 @@ template <int BN, bool GATED> constexpr int tile_smem_bytes() {
            tile_stages<BN, GATED>() * tile_stage_bytes<BN>();
 }
 
-// Eight consecutive columns of one output row, n of them inside; 16-byte
-// stores where `vec` says that the row's groups of eight start on 16 bytes.
-template <typename T>
-__device__ __forceinline__ void put8(T* p, const float (&v)[8], int n, bool vec) {
-    if (vec && n >= 8) {
-        store8(p, v);
-    } else {
+// The rows of a group that a lane finishes at once: R rows m0, m0 + step, ...
+// of eight consecutive columns n .., `left` of them inside the matrix.
+template <int R>
+struct Group {
+    int m0, step, n, left;
+};
+
+// Rows past the last are skipped.
+template <typename T, int R>
+__device__ __forceinline__ void put_rows(T* base, long long ld, const Group<R>& g, int M,
+                                         const float (&v)[R][8], bool vec) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < n) p[e] = from_f<T>(v[e]);
+    for (int i = 0; i < R; ++i) {
+        const int m = g.m0 + i * g.step;
+        if (m >= M) continue;
+        T* p = base + m * ld + g.n;
+        if (vec && g.left >= 8) {
+            store8(p, v[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < g.left) p[e] = from_f<T>(v[i][e]);
+        }
     }
 }
-__device__ __forceinline__ void put8(void* base, long long at, int type, const float (&v)[8], int n,
-                                     bool vec) {
-    if (type == BVML_BF16) put8(static_cast<__nv_bfloat16*>(base) + at, v, n, vec);
-    else if (type == BVML_F16) put8(static_cast<__half*>(base) + at, v, n, vec);
-    else put8(static_cast<float*>(base) + at, v, n, vec);
+template <int R>
+__device__ __forceinline__ void put_rows(void* base, long long ld, int type, const Group<R>& g,
+                                         int M, const float (&v)[R][8], bool vec) {
+    if (type == BVML_BF16) put_rows(static_cast<__nv_bfloat16*>(base), ld, g, M, v, vec);
+    else if (type == BVML_F16) put_rows(static_cast<__half*>(base), ld, g, M, v, vec);
+    else put_rows(static_cast<float*>(base), ld, g, M, v, vec);
 }
-template <typename T>
-__device__ __forceinline__ void add8(const T* p, float (&v)[8], int n, bool vec) {
-    if (vec && n >= 8) {
-        float r[8];
-        load8(p, r);
+template <typename T, int R>
+__device__ __forceinline__ void add_rows(const T* base, long long ld, const Group<R>& g, int M,
+                                         float (&v)[R][8], bool vec) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += r[e];
-    } else {
+    for (int i = 0; i < R; ++i) {
+        const int m = g.m0 + i * g.step;
+        if (m >= M) continue;
+        const T* p = base + m * ld + g.n;
+        if (vec && g.left >= 8) {
+            float r[8];
+            load8(p, r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < n) v[e] += to_f(p[e]);
+            for (int e = 0; e < 8; ++e) v[i][e] += r[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < g.left) v[i][e] += to_f(p[e]);
+        }
     }
 }
 
-__device__ __forceinline__ void act8(float (&v)[8], int act) {
-    // the switch outside the loop: the activation is the same for the whole launch
+template <int R>
+__device__ __forceinline__ void act_rows(float (&v)[R][8], int act) {
+    // the switch outside the loops: the activation is the same for the whole launch
     switch (act) {
-#define BVML_ACT8(code)                                    \
-    case code:                                             \
-        _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] = act_f(v[e], code); \
+#define BVML_ACT_ROWS(code)                                                          \
+    case code:                                                                       \
+        _Pragma("unroll") for (int i = 0; i < R; ++i)                                \
+            _Pragma("unroll") for (int e = 0; e < 8; ++e) v[i][e] = act_f(v[i][e], code); \
         break;
-        BVML_ACT8(BVML_ACT_RELU)
-        BVML_ACT8(BVML_ACT_SIGMOID)
-        BVML_ACT8(BVML_ACT_TANH)
-        BVML_ACT8(BVML_ACT_SILU)
-        BVML_ACT8(BVML_ACT_GELU)
-#undef BVML_ACT8
+        BVML_ACT_ROWS(BVML_ACT_RELU)
+        BVML_ACT_ROWS(BVML_ACT_SIGMOID)
+        BVML_ACT_ROWS(BVML_ACT_TANH)
+        BVML_ACT_ROWS(BVML_ACT_SILU)
+        BVML_ACT_ROWS(BVML_ACT_GELU)
+#undef BVML_ACT_ROWS
         default: break;
     }
 }
 
-// Epilogue of eight consecutive columns n0 .. of row m (in bounds; `left`
-// columns of the group are).
-template <bool GATED>
-__device__ __forceinline__ void finish8(const TileArgs& a, int m, int n0, int left, float (&v)[8],
-                                        float (&u)[8]) {
-    const float rs = a.row_scale ? __ldg(a.row_scale + m) : 1.0f;
+// Epilogue of a lane's group. Every choice that is the same for the launch is
+// made once for all R rows, so that their loads and stores are in flight together.
+template <int R, bool GATED>
+__device__ __forceinline__ void finish_rows(const TileArgs& a, const Group<R>& g, float (&v)[R][8],
+                                            float (&u)[GATED ? R : 1][8]) {
+    float c[8];
     if (a.col_scale[0]) {
+        float rs[R];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] *= rs * (e < left ? __ldg(a.col_scale[0] + n0 + e) : 0.0f);
-            if constexpr (GATED) u[e] *= rs * (e < left ? __ldg(a.col_scale[1] + n0 + e) : 0.0f);
+        for (int i = 0; i < R; ++i) {
+            const int m = g.m0 + i * g.step;
+            rs[i] = m < a.M ? __ldg(a.row_scale + m) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = e < g.left ? __ldg(a.col_scale[0] + g.n + e) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] *= rs[i] * c[e];
+        if constexpr (GATED) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c[e] = e < g.left ? __ldg(a.col_scale[1] + g.n + e) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[i][e] *= rs[i] * c[e];
         }
     }
     if constexpr (GATED) {
         if (a.save[0]) {
-            put8(a.save[0], m * a.lds[0] + n0, a.out_type, v, left, a.vec & kVecSave);
-            put8(a.save[1], m * a.lds[1] + n0, a.out_type, u, left, a.vec & kVecSave);
+            put_rows(a.save[0], a.lds[0], a.out_type, g, a.M, v, a.vec & kVecSave);
+            put_rows(a.save[1], a.lds[1], a.out_type, g, a.M, u, a.vec & kVecSave);
         }
-        act8(v, a.act);
+        act_rows(v, a.act);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= u[e];
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] *= u[i][e];
     } else {
         if (a.bias) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += e < left ? __ldg(a.bias + n0 + e) : 0.0f;
+            for (int e = 0; e < 8; ++e) c[e] = e < g.left ? __ldg(a.bias + g.n + e) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] += c[e];
         }
-        if (a.save[0]) put8(a.save[0], m * a.lds[0] + n0, a.out_type, v, left, a.vec & kVecSave);
-        act8(v, a.act);
+        if (a.save[0]) put_rows(a.save[0], a.lds[0], a.out_type, g, a.M, v, a.vec & kVecSave);
+        act_rows(v, a.act);
         if (a.residual) {
-            const long long at = m * a.ldr + n0;
+            const bool vec = a.vec & kVecRes;
             if (a.out_type == BVML_BF16)
-                add8(static_cast<const __nv_bfloat16*>(a.residual) + at, v, left, a.vec & kVecRes);
+                add_rows(static_cast<const __nv_bfloat16*>(a.residual), a.ldr, g, a.M, v, vec);
             else if (a.out_type == BVML_F16)
-                add8(static_cast<const __half*>(a.residual) + at, v, left, a.vec & kVecRes);
+                add_rows(static_cast<const __half*>(a.residual), a.ldr, g, a.M, v, vec);
             else
-                add8(static_cast<const float*>(a.residual) + at, v, left, a.vec & kVecRes);
+                add_rows(static_cast<const float*>(a.residual), a.ldr, g, a.M, v, vec);
         }
     }
-    if (!a.out2 || m < a.rows0)
-        put8(a.out, m * a.ldo + n0, a.out_type, v, left, a.vec & kVecOut);
-    else if (m >= a.rows1)
-        put8(a.out2, (m - a.rows1) * a.ldo2 + n0, a.out_type, v, left, a.vec & kVecOut2);
+    if (!a.out2 || g.m0 + (R - 1) * g.step < a.rows0) {
+        put_rows(a.out, a.ldo, a.out_type, g, a.M, v, a.vec & kVecOut);
+    } else if (g.m0 >= a.rows1) {
+        Group<R> h = g;
+        h.m0 -= a.rows1;
+        put_rows(a.out2, a.ldo2, a.out_type, h, a.M - a.rows1, v, a.vec & kVecOut2);
+    } else {  // the few groups that span the border, row by row
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int m = g.m0 + i * g.step;
+            Group<1> h{m, 0, g.n, g.left};
+            float one[1][8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) one[0][e] = v[i][e];
+            if (m < a.rows0) {
+                put_rows(a.out, a.ldo, a.out_type, h, a.M, one, a.vec & kVecOut);
+            } else if (m >= a.rows1) {
+                h.m0 -= a.rows1;
+                put_rows(a.out2, a.ldo2, a.out_type, h, a.M - a.rows1, one, a.vec & kVecOut2);
+            }
+        }
+    }
 }
 
 template <int BN, bool AT, bool BT, bool F8, bool GATED>
@@ -392,15 +454,16 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                     if (lane == 0) tc::mbar_arrive_cluster(acc_empty0 + 8 * buf);
                 }
                 __syncwarp();
-                // phase 2: a lane holds eight consecutive columns of a row
-                constexpr int kGroups = kW / 8;        // lanes of a row
-                constexpr int kRows = 32 / kGroups;    // rows at a time
-                const int q = lane % kGroups;
+                // phase 2: a lane finishes eight consecutive columns of R rows
+                constexpr int kGroups = kW / 8;  // lanes of a row, and R
+                constexpr int kRows = 32 / kGroups;
+                const int q = lane % kGroups, r0 = lane / kGroups;
+                const Group<kGroups> grp{m0 + quarter * 32 + r0, kRows, n0 + col + q * 8,
+                                         a.N - (n0 + col + q * 8)};
+                float v[kGroups][8], g[GATED ? kGroups : 1][8];
 #pragma unroll
-                for (int it = 0; it < 32 / kRows; ++it) {
-                    const int r = it * kRows + lane / kGroups;
-                    const int m = m0 + quarter * 32 + r, n = n0 + col + q * 8;
-                    float v[8], g[8];
+                for (int i = 0; i < kGroups; ++i) {
+                    const int r = i * kRows + r0;
 #pragma unroll
                     for (int p = 0; p < (GATED ? 2 : 1); ++p) {
                         const float* d = stg + p * 1024 + r * 32;
@@ -408,18 +471,17 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                             d + (((2 * q) ^ (r & 7)) << 2));
                         const float4 y = *reinterpret_cast<const float4*>(
                             d + (((2 * q + 1) ^ (r & 7)) << 2));
-                        float* o = p == 0 ? v : g;
+                        float* o = p == 0 ? v[i] : g[GATED ? i : 0];
                         o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
                         o[4] = y.x, o[5] = y.y, o[6] = y.z, o[7] = y.w;
                     }
-                    if (m < a.M && n < a.N) {
-                        if (a.slab) {  // one of several shares of K: joined by a second kernel
-                            float* o = a.slab + ((long long)split * a.M + m) * a.ldslab + n;
-                            put8(o, v, a.N - n, true);
-                        } else {
-                            finish8<GATED>(a, m, n, a.N - n, v, g);
-                        }
-                    }
+                }
+                if (grp.left > 0) {
+                    if (a.slab)  // one of several shares of K: joined by a second kernel
+                        put_rows(a.slab + (long long)split * a.M * a.ldslab, a.ldslab, grp, a.M,
+                                 v, true);
+                    else
+                        finish_rows<kGroups, GATED>(a, grp, v, g);
                 }
                 __syncwarp();
             }

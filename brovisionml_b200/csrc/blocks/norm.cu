@@ -77,6 +77,39 @@ __device__ __forceinline__ void load_row(const T* p, int K, int vec, int l, floa
     }
 }
 
+// Eight elements as stored: what a thread keeps of a row that it has asked for
+// and not used yet.
+template <typename T>
+struct alignas(16) Raw {
+    T e[8];
+};
+template <typename T, int G, int VPT>
+__device__ __forceinline__ void fetch_row(const T* p, int K, int vec, int l, Raw<T> (&o)[VPT]) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        if (vec) {
+            const int k = (v * G + l) * 8;
+            uint4* d = reinterpret_cast<uint4*>(&o[v]);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                d[i] = k < K ? reinterpret_cast<const uint4*>(p + k)[i] : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = (v * 8 + e) * G + l;
+                o[v].e[e] = k < K ? p[k] : from_f<T>(0.0f);
+            }
+        }
+    }
+}
+template <typename T, int VPT>
+__device__ __forceinline__ void widen(const Raw<T> (&r)[VPT], float (&o)[VPT][8]) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[v][e] = to_f(r[v].e[e]);
+}
+
 template <typename T, int G, int VPT>
 __device__ __forceinline__ void store_row(T* p, int K, int vec, int l, const float (&o)[VPT][8]) {
 #pragma unroll
@@ -166,22 +199,33 @@ rms_norm_kernel(const NormArgs a) {
     else load_row<T, G, VPT>(static_cast<const T*>(a.w), a.K, a.vec, l, w);
     const float inv_k = 1.0f / (float)a.K;
     int slot = 0;
-    // every thread of the block makes the same number of turns (barriers, shuffles)
-    for (long long t0 = (long long)blockIdx.x * kRows; t0 < a.T;
-         t0 += (long long)gridDim.x * kRows, slot ^= 1) {
+    // The next turn's rows are asked for before this turn's reduction, so that a
+    // block has loads in flight all the time. Every thread of the block makes the
+    // same number of turns (barriers, shuffles).
+    const long long stride = (long long)gridDim.x * kRows;
+    Raw<T> xn[VPT], rn[VPT];
+    auto ask = [&](long long t) {
+        if (t >= a.T) return;
+        fetch_row<T, G, VPT>(static_cast<const T*>(a.x) + t * a.ldx, a.K, a.vec, l, xn);
+        if (a.r)
+            fetch_row<T, G, VPT>(static_cast<const T*>(a.r) + t * a.ldr, a.K, a.vec, l, rn);
+    };
+    ask((long long)blockIdx.x * kRows + g);
+    for (long long t0 = (long long)blockIdx.x * kRows; t0 < a.T; t0 += stride, slot ^= 1) {
         const long long t = t0 + g;
         const bool in = t < a.T;
         float s[VPT][8];
         if (in) {
-            load_row<T, G, VPT>(static_cast<const T*>(a.x) + t * a.ldx, a.K, a.vec, l, s);
+            widen(xn, s);
             if (a.r) {
                 float r[VPT][8];
-                load_row<T, G, VPT>(static_cast<const T*>(a.r) + t * a.ldr, a.K, a.vec, l, r);
+                widen(rn, r);
 #pragma unroll
                 for (int v = 0; v < VPT; ++v)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) s[v][e] += r[v][e];
             }
+            ask(t + stride);
             if (a.sum) store_row<T, G, VPT>(static_cast<T*>(a.sum) + t * a.lds, a.K, a.vec, l, s);
         } else {
 #pragma unroll
@@ -275,14 +319,24 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
         for (int e = 0; e < 8; ++e) dw[v][e] = 0.0f;
     const float inv_k = 1.0f / (float)a.K;
     int slot = 0;
-    for (long long t0 = (long long)blockIdx.x * kRows; t0 < a.T;
-         t0 += (long long)gridDim.x * kRows, slot ^= 1) {
+    const long long stride = (long long)gridDim.x * kRows;
+    Raw<T> sn[VPT], dn[VPT], en[VPT];  // the next turn's rows, as in the forward pass
+    auto ask = [&](long long t) {
+        if (t >= a.T) return;
+        fetch_row<T, G, VPT>(static_cast<const T*>(a.s) + t * a.lds, a.K, a.vec, l, sn);
+        fetch_row<T, G, VPT>(static_cast<const T*>(a.dy) + t * a.lddy, a.K, a.vec, l, dn);
+    };
+    ask((long long)blockIdx.x * kRows + g);
+    for (long long t0 = (long long)blockIdx.x * kRows; t0 < a.T; t0 += stride, slot ^= 1) {
         const long long t = t0 + g;
         const bool in = t < a.T;
         float s[VPT][8], dy[VPT][8];
         if (in) {
-            load_row<T, G, VPT>(static_cast<const T*>(a.s) + t * a.lds, a.K, a.vec, l, s);
-            load_row<T, G, VPT>(static_cast<const T*>(a.dy) + t * a.lddy, a.K, a.vec, l, dy);
+            widen(sn, s);
+            widen(dn, dy);
+            if (a.ds)  // used after the reduction
+                fetch_row<T, G, VPT>(static_cast<const T*>(a.ds) + t * a.ldds, a.K, a.vec, l, en);
+            ask(t + stride);
         } else {
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
@@ -311,7 +365,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
             }
         }
         if (a.ds) {
-            load_row<T, G, VPT>(static_cast<const T*>(a.ds) + t * a.ldds, a.K, a.vec, l, dy);
+            widen(en, dy);
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
@@ -380,8 +434,10 @@ column_sum_kernel(const float* __restrict__ part, int rows, int cols, T* __restr
     __shared__ float sh[16][33];
     const int c = blockIdx.x * 32 + threadIdx.x % 32, r0 = threadIdx.x / 32;
     float v = 0.0f;
-    if (c < cols)
+    if (c < cols) {
+#pragma unroll 8
         for (int r = r0; r < rows; r += 16) v += part[(long long)r * cols + c];
+    }
     sh[r0][threadIdx.x % 32] = v;
     __syncthreads();
     if (r0 == 0 && c < cols) {
@@ -483,7 +539,8 @@ cudaError_t launch_rms_norm(const NormLaunch& L, cudaStream_t s) {
     const Shape h = shape_of(L.K);
     const int rows = block_rows(h);
     const long long want = ((long long)L.T + rows - 1) / rows;
-    const long long most = (long long)sms * (2048 / block_threads(h));
+    // 1024 threads an SM with rows of a block's length, 2048 with shorter ones
+    const long long most = (long long)sms * ((rows > 1 ? 2048 : 1024) / block_threads(h));
     const int grid = (int)(want < most ? want : most);
     const bool q = L.scale != nullptr;
     if (L.type == BVML_F32) {
