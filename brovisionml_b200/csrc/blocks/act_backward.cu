@@ -3,8 +3,8 @@
 //   gated   dg = dh u act'(g), du = dh act(g)
 //
 // Bound by HBM: each input is read once, 16 bytes a thread and access; a block
-// covers 256 columns and walks rows, a thread keeps eight columns' sums in
-// registers. The sums over a block's warps and over blocks run in a fixed
+// covers up to 2048 columns and walks rows two at a time, a thread keeps eight
+// columns' sums in registers. The sums over a block's rows and over blocks run in a fixed
 // order. What the matrix products read back (dz, dg, du) is rounded to 16 bits,
 // the type the tensor cores take; the bias gradient sums the 32-bit values.
 #include "blocks_common.cuh"
@@ -14,8 +14,7 @@ namespace bvml {
 namespace blocks {
 namespace {
 
-constexpr int kCols = 256;  // columns of a block: 32 lanes of eight
-constexpr int kRowThreads = 8;
+constexpr int kThreads = 256;
 
 // Up to eight columns c .. of row pointer p as floats, zeros past n.
 template <typename T>
@@ -38,102 +37,162 @@ __device__ __forceinline__ void store_cols(T* p, int c, int n, bool vec, const f
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kCols)
-act_backward_kernel(const ActBackwardLaunch L, bool vec_dy, bool vec_z, bool vec_dz) {
-    __shared__ float sh[kRowThreads][kCols];
-    const int lane = threadIdx.x % 32, ry = threadIdx.x / 32;
-    const int c = blockIdx.x * kCols + lane * 8;
-    float sum[8] = {};
-    for (long long t = (long long)blockIdx.y * kRowThreads + ry; t < L.T;
-         t += (long long)gridDim.y * kRowThreads) {
-        if (c >= L.N) break;
-        float d[8];
-        load_cols(static_cast<const T*>(L.dy) + t * L.lddy, c, L.N, vec_dy, d);
-        if (L.z) {
-            float z[8];
-            load_cols(static_cast<const T*>(L.z) + t * L.ldz, c, L.N, vec_z, z);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float f, g;
-                act_grad_f(z[e], L.act, f, g);
-                d[e] *= g;
-            }
-        }
-        if (L.dz) store_cols(static_cast<T*>(L.dz) + t * L.lddz, c, L.N, vec_dz, d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += c + e < L.N ? d[e] : 0.0f;
-    }
-    if (!L.partial) return;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sh[ry][lane * 8 + e] = sum[e];
-    __syncthreads();
-    const int n = blockIdx.x * kCols + threadIdx.x;
-    if (n < L.N) {
-        float v = sh[0][threadIdx.x];
-#pragma unroll
-        for (int i = 1; i < kRowThreads; ++i) v += sh[i][threadIdx.x];
-        L.partial[(long long)blockIdx.y * L.N + n] = v;
-    }
-}
-
-// g, u <- dh u act'(g), dh act(g); the activation is chosen outside the loops
-__device__ __forceinline__ void grad_rows(int act, const float (&dh)[2][8], float (&g)[2][8],
-                                          float (&u)[2][8]) {
+// Activation derivatives of two rows' groups of eight, the choice of the
+// activation outside the loops: v <- v act'(z).
+__device__ __forceinline__ void times_grad(int act, const float (&z)[2][8], float (&v)[2][8]) {
     switch (act) {
-#define BVML_GRAD_ROWS(code)                                  \
+#define BVML_TIMES_GRAD(code)                                 \
     case code:                                                \
         _Pragma("unroll") for (int i = 0; i < 2; ++i)         \
             _Pragma("unroll") for (int e = 0; e < 8; ++e) {   \
                 float f, d;                                   \
-                act_grad_f(g[i][e], code, f, d);              \
-                g[i][e] = dh[i][e] * u[i][e] * d;             \
-                u[i][e] = dh[i][e] * f;                       \
+                act_grad_f(z[i][e], code, f, d);              \
+                v[i][e] *= d;                                 \
             }                                                 \
         break;
-        BVML_GRAD_ROWS(BVML_ACT_RELU)
-        BVML_GRAD_ROWS(BVML_ACT_SIGMOID)
-        BVML_GRAD_ROWS(BVML_ACT_TANH)
-        BVML_GRAD_ROWS(BVML_ACT_SILU)
-        BVML_GRAD_ROWS(BVML_ACT_GELU)
-#undef BVML_GRAD_ROWS
+        BVML_TIMES_GRAD(BVML_ACT_RELU)
+        BVML_TIMES_GRAD(BVML_ACT_SIGMOID)
+        BVML_TIMES_GRAD(BVML_ACT_TANH)
+        BVML_TIMES_GRAD(BVML_ACT_SILU)
+        BVML_TIMES_GRAD(BVML_ACT_GELU)
+#undef BVML_TIMES_GRAD
+        default: break;
+    }
+}
+
+// A block covers `span` threads of eight columns by kThreads / span rows at a time.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+act_backward_kernel(const ActBackwardLaunch L, int span, bool vec_dy, bool vec_z, bool vec_dz) {
+    __shared__ float sh[kThreads * 8];
+    const int x = threadIdx.x % span, ry = threadIdx.x / span, rows = blockDim.x / span;
+    const int c = (blockIdx.x * span + x) * 8;
+    float sum[8] = {};
+    const long long stride = (long long)gridDim.y * rows;
+    if (c < L.N) {
+        for (long long t0 = (long long)blockIdx.y * rows + ry; t0 < L.T; t0 += 2 * stride) {
+            float d[2][8], z[2][8];
+            const bool two = t0 + stride < L.T;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const long long t = i && two ? t0 + stride : t0;
+                load_cols(static_cast<const T*>(L.dy) + t * L.lddy, c, L.N, vec_dy, d[i]);
+                if (L.z) load_cols(static_cast<const T*>(L.z) + t * L.ldz, c, L.N, vec_z, z[i]);
+            }
+            if (L.z) times_grad(L.act, z, d);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i && !two) continue;
+                const long long t = t0 + i * stride;
+                if (L.dz) store_cols(static_cast<T*>(L.dz) + t * L.lddz, c, L.N, vec_dz, d[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += d[i][e];
+            }
+        }
+    }
+    if (!L.partial) return;
+    // the block's rows side by side, added in their order
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sh[threadIdx.x * 8 + e] = sum[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < span * 8; i += blockDim.x) {
+        const int n = blockIdx.x * span * 8 + i;
+        if (n >= L.N) break;
+        float v = sh[i];
+        for (int r = 1; r < rows; ++r) v += sh[r * span * 8 + i];
+        L.partial[(long long)blockIdx.y * L.N + n] = v;
+    }
+}
+
+// Eight columns as stored, asked for ahead of use.
+template <typename T>
+struct alignas(16) Raw {
+    T e[8];
+};
+template <typename T>
+__device__ __forceinline__ void ask_cols(const T* p, int c, int n, bool vec, Raw<T>& r) {
+    if (vec && c + 8 <= n) {
+        *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p + c);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.e[e] = c + e < n ? p[c + e] : from_f<T>(0.0f);
+    }
+}
+
+// g, u <- dh u act'(g), dh act(g); the activation is chosen outside the loop
+__device__ __forceinline__ void grad_cols(int act, const float (&dh)[8], float (&g)[8],
+                                          float (&u)[8]) {
+    switch (act) {
+#define BVML_GRAD_COLS(code)                              \
+    case code:                                            \
+        _Pragma("unroll") for (int e = 0; e < 8; ++e) {   \
+            float f, d;                                   \
+            act_grad_f(g[e], code, f, d);                 \
+            g[e] = dh[e] * u[e] * d;                      \
+            u[e] = dh[e] * f;                             \
+        }                                                 \
+        break;
+        BVML_GRAD_COLS(BVML_ACT_RELU)
+        BVML_GRAD_COLS(BVML_ACT_SIGMOID)
+        BVML_GRAD_COLS(BVML_ACT_TANH)
+        BVML_GRAD_COLS(BVML_ACT_SILU)
+        BVML_GRAD_COLS(BVML_ACT_GELU)
+#undef BVML_GRAD_COLS
         default: break;
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kCols)
-gated_backward_kernel(const GatedBackwardLaunch L, bool vec_h, bool vec_g, bool vec_u, bool vec_d) {
-    const int lane = threadIdx.x % 32, ry = threadIdx.x / 32;
-    const int c = blockIdx.x * kCols + lane * 8;
+__global__ void __launch_bounds__(kThreads, 4)
+gated_backward_kernel(const GatedBackwardLaunch L, int span, bool vec_h, bool vec_g, bool vec_u,
+                      bool vec_d) {
+    const int x = threadIdx.x % span, ry = threadIdx.x / span, rows = blockDim.x / span;
+    const int c = (blockIdx.x * span + x) * 8;
     if (c >= L.F) return;
-    // two rows at a time: six loads in flight a thread
-    const long long stride = (long long)gridDim.y * kRowThreads;
-    for (long long t0 = (long long)blockIdx.y * kRowThreads + ry; t0 < L.T; t0 += 2 * stride) {
-        float dh[2][8], g[2][8], u[2][8];
+    const long long stride = (long long)gridDim.y * rows;
+    // the next row's loads are in flight while this one is computed
+    Raw<T> rh, rg, ru;
+    auto ask = [&](long long t) {
+        if (t >= L.T) return;
+        ask_cols(static_cast<const T*>(L.dh) + t * L.lddh, c, L.F, vec_h, rh);
+        ask_cols(static_cast<const T*>(L.g) + t * L.ldg, c, L.F, vec_g, rg);
+        ask_cols(static_cast<const T*>(L.u) + t * L.ldu, c, L.F, vec_u, ru);
+    };
+    ask((long long)blockIdx.y * rows + ry);
+    for (long long t = (long long)blockIdx.y * rows + ry; t < L.T; t += stride) {
+        float dh[8], g[8], u[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const long long t = t0 + i * stride < L.T ? t0 + i * stride : t0;
-            load_cols(static_cast<const T*>(L.dh) + t * L.lddh, c, L.F, vec_h, dh[i]);
-            load_cols(static_cast<const T*>(L.g) + t * L.ldg, c, L.F, vec_g, g[i]);
-            load_cols(static_cast<const T*>(L.u) + t * L.ldu, c, L.F, vec_u, u[i]);
+        for (int e = 0; e < 8; ++e) {
+            dh[e] = to_f(rh.e[e]);
+            g[e] = to_f(rg.e[e]);
+            u[e] = to_f(ru.e[e]);
         }
-        grad_rows(L.act, dh, g, u);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const long long t = t0 + i * stride;
-            if (t >= L.T) continue;
-            store_cols(static_cast<T*>(L.dg) + t * L.ldd, c, L.F, vec_d, g[i]);
-            store_cols(static_cast<T*>(L.du) + t * L.ldd, c, L.F, vec_d, u[i]);
-        }
+        ask(t + stride);
+        grad_cols(L.act, dh, g, u);
+        store_cols(static_cast<T*>(L.dg) + t * L.ldd, c, L.F, vec_d, g);
+        store_cols(static_cast<T*>(L.du) + t * L.ldd, c, L.F, vec_d, u);
     }
 }
 
+// How a row of N is covered: `blocks` blocks of `span` threads, eight columns each,
+// evenly (a row of 2056 is 2 x 129 threads and not 256 and one), `rows` rows a block.
+struct Cover {
+    int span, rows, blocks;
+};
+Cover cover(int N) {
+    const int units = (int)(((long long)N + 7) / 8);
+    Cover c;
+    c.blocks = (units + kThreads - 1) / kThreads;
+    c.span = (units + c.blocks - 1) / c.blocks;
+    c.rows = kThreads / c.span;
+    return c;
+}
+// Blocks along the rows: about eight an SM (148) in all, so that there are
+// bytes enough in flight and few partial sums.
 int row_blocks(int T, int N) {
-    const long long cols = ((long long)N + kCols - 1) / kCols;
-    const long long rows = ((long long)T + kRowThreads - 1) / kRowThreads;
-    // about eight blocks an SM (148) in all: enough bytes in flight, few partial sums
-    long long want = (148 * 8 + cols - 1) / cols;
+    const Cover c = cover(N);
+    const long long rows = ((long long)T + c.rows - 1) / c.rows;
+    const long long want = (148 * 8 + c.blocks - 1) / c.blocks;
     return (int)(want < rows ? want : rows);
 }
 
@@ -143,21 +202,29 @@ int act_backward_parts(int T, int N) { return row_blocks(T, N); }
 
 cudaError_t launch_act_backward(const ActBackwardLaunch& L, cudaStream_t s) {
     if (L.T == 0) return cudaSuccess;
-    const dim3 grid((L.N + kCols - 1) / kCols, row_blocks(L.T, L.N));
+    const Cover v = cover(L.N);
+    const dim3 grid(v.blocks, row_blocks(L.T, L.N));
+    const int span = v.span, threads = v.span * v.rows;
     const bool a = on16(L.dy, L.lddy, 2), b = L.z && on16(L.z, L.ldz, 2),
                c = L.dz && on16(L.dz, L.lddz, 2);
-    if (L.type == BVML_F16) act_backward_kernel<__half><<<grid, kCols, 0, s>>>(L, a, b, c);
-    else act_backward_kernel<__nv_bfloat16><<<grid, kCols, 0, s>>>(L, a, b, c);
+    if (L.type == BVML_F16)
+        act_backward_kernel<__half><<<grid, threads, 0, s>>>(L, span, a, b, c);
+    else
+        act_backward_kernel<__nv_bfloat16><<<grid, threads, 0, s>>>(L, span, a, b, c);
     return cudaGetLastError();
 }
 
 cudaError_t launch_gated_backward(const GatedBackwardLaunch& L, cudaStream_t s) {
     if (L.T == 0) return cudaSuccess;
-    const dim3 grid((L.F + kCols - 1) / kCols, row_blocks(L.T, L.F));
+    const Cover v = cover(L.F);
+    const dim3 grid(v.blocks, row_blocks(L.T, L.F));
+    const int span = v.span, threads = v.span * v.rows;
     const bool a = on16(L.dh, L.lddh, 2), b = on16(L.g, L.ldg, 2), c = on16(L.u, L.ldu, 2),
                d = on16(L.dg, L.ldd, 2) && on16(L.du, L.ldd, 2);
-    if (L.type == BVML_F16) gated_backward_kernel<__half><<<grid, kCols, 0, s>>>(L, a, b, c, d);
-    else gated_backward_kernel<__nv_bfloat16><<<grid, kCols, 0, s>>>(L, a, b, c, d);
+    if (L.type == BVML_F16)
+        gated_backward_kernel<__half><<<grid, threads, 0, s>>>(L, span, a, b, c, d);
+    else
+        gated_backward_kernel<__nv_bfloat16><<<grid, threads, 0, s>>>(L, span, a, b, c, d);
     return cudaGetLastError();
 }
 

@@ -27,6 +27,18 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
     return __float2bfloat16_rn(v);
 }
 
+// Two values as a pair of 16-bit elements, in one (packed) conversion: single ones
+// run at a quarter of the rate.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(h);
+}
+
 // Eight consecutive elements as floats; p on 16 bytes.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -48,11 +60,8 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        uint4 u;
-        T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
-        *reinterpret_cast<uint4*>(p) = u;
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                                  pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     }
 }
 
@@ -67,6 +76,28 @@ __device__ __forceinline__ float sigmoid_f(float z) {
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
+// The normal distribution function, and e = exp(-z^2 / 2) on the way, without a
+// branch (erff takes two paths, which lanes and unrolled elements walk one
+// after the other: 50 us on an 8192 x 8192 epilogue). With x = |z| / sqrt 2 and
+// t = 1 / (1 + 0.3 x), Phi(-|z|) = exp(-x^2) erfc(x) exp(x^2) / 2, and erfc(x) exp(x^2) / t
+// is smooth in t on (0, 1]: a polynomial of degree 8, fitted here for the least relative
+// error (2e-8 in exact arithmetic; in fp32 6e-7 of Phi for |z| < 4).
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float t = __fdividef(1.0f, fmaf(0.3f * kSqrtHalf, fabsf(z), 1.0f));
+    e = __expf(-0.5f * z * z);
+    float q = -0.12952278554439545f;
+    q = fmaf(q, t, 0.48556262254714966f);
+    q = fmaf(q, t, -0.5122768878936768f);
+    q = fmaf(q, t, 0.5477187037467957f);
+    q = fmaf(q, t, -0.09464981406927109f);
+    q = fmaf(q, t, 0.21492567658424377f);
+    q = fmaf(q, t, 0.14833925664424896f);
+    q = fmaf(q, t, 0.17071521282196045f);
+    q = fmaf(q, t, 0.1691880077123642f);
+    q *= 0.5f * e * t;
+    return z < 0.0f ? q : 1.0f - q;
+}
+
 // The activations of bvml_blocks.h. NaN stays NaN (relu compares, it does not
 // take a maximum, which would drop it).
 __device__ __forceinline__ float act_f(float z, int act) {
@@ -75,7 +106,7 @@ __device__ __forceinline__ float act_f(float z, int act) {
         case BVML_ACT_SIGMOID: return sigmoid_f(z);
         case BVML_ACT_TANH: return tanhf(z);
         case BVML_ACT_SILU: return z * sigmoid_f(z);
-        case BVML_ACT_GELU: return 0.5f * z * (1.0f + erff(z * kSqrtHalf));
+        case BVML_ACT_GELU: { float e; return z * normal_cdf(z, e); }
         default: return z;
     }
 }
@@ -104,9 +135,10 @@ __device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d)
             break;
         }
         case BVML_ACT_GELU: {
-            const float phi = 0.5f * (1.0f + erff(z * kSqrtHalf));
+            float e;
+            const float phi = normal_cdf(z, e);
             f = z * phi;
-            d = phi + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+            d = fmaf(z * kInvSqrt2Pi, e, phi);
             break;
         }
         default: f = z; d = 1.0f;

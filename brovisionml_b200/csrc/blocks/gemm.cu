@@ -47,8 +47,8 @@ int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 // run at about 0.9, 64 at about 0.7 of the rate of 256); `tail` is what a turn costs
 // beside its K steps (filling the ring, draining the last accumulator).
 double tile_cost(int tiles, int steps, int splits, int bn) {
-    const double rate = bn == 256 ? 1.0 : bn == 128 ? 0.56 : 0.36;
-    const double tail = bn == 256 ? 5.0 : bn == 128 ? 3.5 : 2.5;
+    const double rate = bn == 256 ? 1.0 : bn == 192 ? 0.79 : bn == 128 ? 0.56 : 0.36;
+    const double tail = bn == 256 ? 5.0 : bn == 192 ? 4.2 : bn == 128 ? 3.5 : 2.5;
     const long long works = (long long)tiles * splits;
     const long long turns = (works + kPairs - 1) / kPairs;
     // joining the shares reads and writes the output once more for each
@@ -105,7 +105,8 @@ Plan plan_of(const GemmLaunch& L) {
     const bool plain = !L.gated && !L.bias && !L.residual && !L.save[0] && !L.row_scale &&
                        L.act == BVML_ACT_NONE;
     double best = 1e300;
-    for (int bn = 256; bn >= (L.b_t ? 128 : 64); bn /= 2) {
+    for (int bn = 256; bn >= (L.b_t ? 128 : 64); bn -= 64) {
+        if (bn == 192 && L.b_t) continue;
         const int tn = cdiv(L.N, L.gated ? bn / 2 : bn);
         for (int sp = 1; sp <= (plain ? 32 : 1) && (sp == 1 || steps / sp >= 8); sp *= 2) {
             const double c = tile_cost(p.tiles_m * tn, steps, sp, bn);
@@ -119,7 +120,7 @@ Plan plan_of(const GemmLaunch& L) {
     }
     p.slab = off;
     if (p.splits > 1) {
-        p.ldslab = ((long long)L.N + 7) / 8 * 8;
+        p.ldslab = ((long long)L.N + 31) / 32 * 32;
         off += round256((size_t)p.splits * L.M * p.ldslab * 4);
     }
     p.bytes = off;
@@ -300,18 +301,26 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
         a.idesc = idesc_of(L.in_type, false, false, 128, p.tok);
         return launch_skinny(p.tok, L.in_type == BVML_E4M3, L.gated, maps, k, s);
     }
-    const bool out_ok = on16(L.out, L.ldo, eo), out2_ok = !L.out2 || on16(L.out2, L.ldo2, eo);
-    if (out_ok) a.vec |= kVecOut;
-    if (out2_ok) a.vec |= kVecOut2;
-    if (L.residual && on16(L.residual, L.ldr, eo)) a.vec |= kVecRes;
-    if (L.save[0] && on16(L.save[0], L.lds[0], eo) &&
-        (!L.save[1] || on16(L.save[1], L.lds[1], eo)))
-        a.vec |= kVecSave;
+    // what the addresses and pitches that the epilogue touches have in common
+    auto bits = [&](const void* ptr, long long ld) {
+        return ptr ? reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)ld * eo : (uintptr_t)0;
+    };
+    const uintptr_t out = bits(L.out, L.ldo) | bits(L.out2, L.ldo2);
+    const uintptr_t save = bits(L.save[0], L.lds[0]) | bits(L.save[1], L.lds[1]);
+    const uintptr_t all = out | save | bits(L.residual, L.ldr) |
+                          reinterpret_cast<uintptr_t>(L.bias) |
+                          reinterpret_cast<uintptr_t>(L.col_scale[0]) |
+                          reinterpret_cast<uintptr_t>(L.col_scale[1]);
+    a.vec = ((all & 15) == 0 ? kOn16 : 0) | ((out & 31) == 0 ? kWideOut : 0) |
+            ((save & 31) == 0 ? kWideSave : 0);
+    const bool vec = (out & 15) == 0;
     a.idesc = idesc_of(L.in_type, L.a_t, L.b_t, 256, p.bn);
     if (p.splits > 1) {
         a.slab = reinterpret_cast<float*>(static_cast<char*>(ws) + p.slab);
         a.ldslab = p.ldslab;
     }
+    a.by_tiles = divide_by((uint32_t)(p.tiles_m * p.tiles_n));
+    a.by_group = divide_by((uint32_t)(kTileGroup * p.tiles_n));
     int sms = 0;
     if ((e = sm_count(&sms)) != cudaSuccess) return e;
     const long long works = (long long)p.tiles_m * p.tiles_n * p.splits;
@@ -320,7 +329,6 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     else if (L.in_type == BVML_E4M3) e = launch_tile_nt_f8(p.bn, L.gated, maps, a, pairs, s);
     else e = launch_tile_nt(p.bn, L.gated, maps, a, pairs, s);
     if (e != cudaSuccess || p.splits == 1) return e;
-    const bool vec = out_ok && out2_ok;
     if (L.out_type == BVML_F16) return join<__half>(L, p, a.slab, vec, s);
     if (L.out_type == BVML_BF16) return join<__nv_bfloat16>(L, p, a.slab, vec, s);
     return join<float>(L, p, a.slab, vec, s);

@@ -13,8 +13,29 @@ struct TileMaps {
     CUtensorMap b[2];  // one a segment, or gate and up
 };
 
-// groups of eight columns start on 16 bytes in ...
-enum : int { kVecOut = 1, kVecOut2 = 2, kVecRes = 4, kVecSave = 8 };
+// Division of n < 2^31 by d >= 2: n / d = (n mul >> 32) >> shift with 2^shift < d <=
+// 2^(shift + 1) and mul = ceil(2^(32 + shift) / d). mul d exceeds 2^(32 + shift) by
+// less than d, so n times the excess stays below 2^(32 + shift): the quotient is exact.
+struct Division {
+    uint32_t mul, shift;
+};
+
+inline Division divide_by(uint32_t d) {
+    Division v{0, 0};
+    if (d < 2) return v;  // not used: see work_of
+    while ((uint64_t)2 << v.shift < d) ++v.shift;
+    v.mul = (uint32_t)((((uint64_t)1 << (32 + v.shift)) + d - 1) / d);
+    return v;
+}
+
+constexpr int kTileGroup = 8;  // tile rows that are walked together
+
+// TileArgs::vec
+enum : int {
+    kOn16 = 1,     // every row of 32 columns and every vector over columns starts on 16 bytes
+    kWideOut = 2,  // the outputs' (out and out2) on 32
+    kWideSave = 4  // save's on 32
+};
 
 struct TileArgs {
     int M, N;              // output rows and columns (features when gated)
@@ -22,6 +43,7 @@ struct TileArgs {
     int tiles_m, tiles_n;
     int splits;            // shares of K, each a work item of its own
     uint32_t idesc;
+    Division by_tiles, by_group;  // tiles_m * tiles_n, kTileGroup * tiles_n
     const float* row_scale;
     const float* col_scale[2];
     const float* bias;
@@ -36,7 +58,7 @@ struct TileArgs {
     long long ldslab;
 };
 
-// bn: the pair's columns (256, 128 or 64; transposed B: at least 128)
+// bn: the pair's columns (256, 128, 64, 192; transposed B: 256 or 128)
 cudaError_t launch_tile_nt(int bn, bool gated, const TileMaps& m, const TileArgs& a, int pairs,
                            cudaStream_t s);
 cudaError_t launch_tile_nt_f8(int bn, bool gated, const TileMaps& m, const TileArgs& a, int pairs,

@@ -28,17 +28,6 @@ template <int TOK> constexpr int skinny_smem_bytes() {
     return 1024 + skinny_stages<TOK>() * skinny_stage_bytes<TOK>() + 256;
 }
 
-__device__ __forceinline__ void put1(void* p, long long i, int type, float v) {
-    if (type == BVML_BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
-    else if (type == BVML_F16) static_cast<__half*>(p)[i] = from_f<__half>(v);
-    else static_cast<float*>(p)[i] = v;
-}
-__device__ __forceinline__ float get1(const void* p, long long i, int type) {
-    if (type == BVML_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
-    if (type == BVML_F16) return to_f(static_cast<const __half*>(p)[i]);
-    return static_cast<const float*>(p)[i];
-}
-
 // This CTA's share of the features, summed over the cluster's SPLIT CTAs and
 // finished: four neighbouring features of a token a thread and turn, all the
 // shares' loads in flight at once.
@@ -67,30 +56,10 @@ __device__ __forceinline__ void add_up(const TileArgs& a, uint32_t sbase, int ra
             v[0] += p[r].x, v[1] += p[r].y, v[2] += p[r].z, v[3] += p[r].w;
             if constexpr (GATED) u[0] += q[r].x, u[1] += q[r].y, u[2] += q[r].z, u[3] += q[r].w;
         }
-        const long long m = t0 + t;
-        const float rs = a.row_scale ? a.row_scale[m] : 1.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int n = f0 + f + e;
-            if (n >= a.N) break;
-            if (a.col_scale[0]) {
-                v[e] *= rs * a.col_scale[0][n];
-                if constexpr (GATED) u[e] *= rs * a.col_scale[1][n];
-            }
-            if constexpr (GATED) {
-                if (a.save[0]) {
-                    put1(a.save[0], m * a.lds[0] + n, a.out_type, v[e]);
-                    put1(a.save[1], m * a.lds[1] + n, a.out_type, u[e]);
-                }
-                v[e] = act_f(v[e], a.act) * u[e];
-            } else {
-                if (a.bias) v[e] += a.bias[n];
-                if (a.save[0]) put1(a.save[0], m * a.lds[0] + n, a.out_type, v[e]);
-                v[e] = act_f(v[e], a.act);
-                if (a.residual) v[e] += get1(a.residual, m * a.ldr + n, a.out_type);
-            }
-            put1(a.out, m * a.ldo + n, a.out_type, v[e]);
-        }
+        for (int e = 0; e < 4; ++e)
+            if (f0 + f + e < a.N)
+                finish_one<GATED>(a, t0 + t, f0 + f + e, v[e], GATED ? u[e] : 0.0f);
     }
 }
 

@@ -16,10 +16,8 @@
 //    of both CTAs are counted on the first CTA's barrier;
 //  * warp 1 of the first CTA issues the MMAs of the pair, and hands ring entries
 //    back to both producers by multicast commits;
-//  * warps 2-9 drain one of two accumulators in TMEM while the other fills: 32
-//    columns at a time through a swizzled staging buffer in shared memory, so that a
-//    thread finishes eight consecutive columns of a row and loads and stores
-//    16 bytes (the residual, the outputs) where the rows allow it.
+//  * warps 2-9 drain one of two accumulators in TMEM while the other fills, 32
+//    columns of a row a lane.
 //
 // Operands come in row-major order for the forward pass; the backward pass reads
 // the same tensors with the contracted axis outermost (AT, BT) without a
@@ -37,8 +35,8 @@
 namespace bvml {
 namespace blocks {
 
-constexpr int kTileThreads = 320;
-constexpr int kTileEpiWarps = 8;
+constexpr int kTileEpiWarps = 8;  // two for each quarter of the TMEM lanes
+constexpr int kTileThreads = 64 + 32 * kTileEpiWarps;
 constexpr int kTileMaxStages = 8;
 constexpr uint32_t kTileWaitLimit = 1u << 22;
 constexpr int kTileSmem = 227 * 1024;
@@ -46,193 +44,206 @@ constexpr int kTileBarBytes = 256;
 
 static __device__ int g_tile_error;
 
+// n / d for n < 2^31 by what Division (gemm_internal.h) holds of d
+__device__ __forceinline__ uint32_t divide(uint32_t n, Division d) {
+    return (uint32_t)(((uint64_t)n * d.mul) >> 32) >> d.shift;
+}
+
 // bytes of one ring entry: 128 rows of A, BN / 2 of B, 128 bytes each
 template <int BN> constexpr int tile_stage_bytes() { return (128 + BN / 2) * 128; }
-// staging: 32 rows x 32 fp32 columns a warp, one for each projection
-template <bool GATED> constexpr int tile_staging_bytes() {
-    return kTileEpiWarps * 4096 * (GATED ? 2 : 1);
-}
-template <int BN, bool GATED> constexpr int tile_stages() {
-    constexpr int n = (kTileSmem - 1024 - kTileBarBytes - tile_staging_bytes<GATED>()) /
-                      tile_stage_bytes<BN>();
+template <int BN> constexpr int tile_stages() {
+    constexpr int n = (kTileSmem - 1024 - kTileBarBytes) / tile_stage_bytes<BN>();
     return n < kTileMaxStages ? n : kTileMaxStages;
 }
-template <int BN, bool GATED> constexpr int tile_smem_bytes() {
-    return 1024 + kTileBarBytes + tile_staging_bytes<GATED>() +
-           tile_stages<BN, GATED>() * tile_stage_bytes<BN>();
+template <int BN> constexpr int tile_smem_bytes() {
+    return 1024 + kTileBarBytes + tile_stages<BN>() * tile_stage_bytes<BN>();
 }
 
-// The rows of a group that a lane finishes at once: R rows m0, m0 + step, ...
-// of eight consecutive columns n .., `left` of them inside the matrix.
-template <int R>
-struct Group {
-    int m0, step, n, left;
-};
-
-// Rows past the last are skipped.
-template <typename T, int R>
-__device__ __forceinline__ void put_rows(T* base, long long ld, const Group<R>& g, int M,
-                                         const float (&v)[R][8], bool vec) {
+// A lane finishes 32 consecutive columns of one row, as they lie in TMEM: 64
+// or 128 bytes, in 32-byte stores where the rows start on 32 bytes, so that every
+// sector is touched once. No staging through shared memory.
+__device__ __forceinline__ void st32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+template <int WORDS>
+__device__ __forceinline__ void st_words(void* p, const uint32_t (&w)[WORDS], bool wide) {
+    if (wide) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int m = g.m0 + i * g.step;
-        if (m >= M) continue;
-        T* p = base + m * ld + g.n;
-        if (vec && g.left >= 8) {
-            store8(p, v[i]);
-        } else {
+        for (int i = 0; i < WORDS / 8; ++i) st32(static_cast<uint32_t*>(p) + 8 * i, w + 8 * i);
+    } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < g.left) p[e] = from_f<T>(v[i][e]);
-        }
+        for (int i = 0; i < WORDS / 4; ++i)
+            static_cast<uint4*>(p)[i] =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
 }
-template <int R>
-__device__ __forceinline__ void put_rows(void* base, long long ld, int type, const Group<R>& g,
-                                         int M, const float (&v)[R][8], bool vec) {
-    if (type == BVML_BF16) put_rows(static_cast<__nv_bfloat16*>(base), ld, g, M, v, vec);
-    else if (type == BVML_F16) put_rows(static_cast<__half*>(base), ld, g, M, v, vec);
-    else put_rows(static_cast<float*>(base), ld, g, M, v, vec);
-}
-template <typename T, int R>
-__device__ __forceinline__ void add_rows(const T* base, long long ld, const Group<R>& g, int M,
-                                         float (&v)[R][8], bool vec) {
+// 32 columns to rows that start on 16 bytes (wide: on 32).
+__device__ __forceinline__ void put_row(void* base, long long at, int type, const float (&v)[32],
+                                        bool wide) {
+    if (type == BVML_F32) {
+        uint32_t w[32];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int m = g.m0 + i * g.step;
-        if (m >= M) continue;
-        const T* p = base + m * ld + g.n;
-        if (vec && g.left >= 8) {
-            float r[8];
-            load8(p, r);
+        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+        st_words(static_cast<float*>(base) + at, w, wide);
+    } else {
+        uint32_t w[16];
+        if (type == BVML_BF16) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] += r[e];
+            for (int i = 0; i < 16; ++i) w[i] = pack2<__nv_bfloat16>(v[2 * i], v[2 * i + 1]);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < g.left) v[i][e] += to_f(p[e]);
+            for (int i = 0; i < 16; ++i) w[i] = pack2<__half>(v[2 * i], v[2 * i + 1]);
         }
+        st_words(static_cast<uint16_t*>(base) + at, w, wide);
     }
 }
 
-template <int R>
-__device__ __forceinline__ void act_rows(float (&v)[R][8], int act) {
-    // the switch outside the loops: the activation is the same for the whole launch
+__device__ __forceinline__ void act_row(float (&v)[32], int act) {
+    if (act == BVML_ACT_NONE) return;
+    // the switch outside the loop: the activation is the same for the whole launch
     switch (act) {
-#define BVML_ACT_ROWS(code)                                                          \
-    case code:                                                                       \
-        _Pragma("unroll") for (int i = 0; i < R; ++i)                                \
-            _Pragma("unroll") for (int e = 0; e < 8; ++e) v[i][e] = act_f(v[i][e], code); \
+#define BVML_ACT_ROW(code)                                                  \
+    case code:                                                              \
+        _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = act_f(v[i], code); \
         break;
-        BVML_ACT_ROWS(BVML_ACT_RELU)
-        BVML_ACT_ROWS(BVML_ACT_SIGMOID)
-        BVML_ACT_ROWS(BVML_ACT_TANH)
-        BVML_ACT_ROWS(BVML_ACT_SILU)
-        BVML_ACT_ROWS(BVML_ACT_GELU)
-#undef BVML_ACT_ROWS
+        BVML_ACT_ROW(BVML_ACT_RELU)
+        BVML_ACT_ROW(BVML_ACT_SIGMOID)
+        BVML_ACT_ROW(BVML_ACT_TANH)
+        BVML_ACT_ROW(BVML_ACT_SILU)
+        BVML_ACT_ROW(BVML_ACT_GELU)
+#undef BVML_ACT_ROW
         default: break;
     }
 }
 
-// Epilogue of a lane's group. Every choice that is the same for the launch is
-// made once for all R rows, so that their loads and stores are in flight together.
-template <int R, bool GATED>
-__device__ __forceinline__ void finish_rows(const TileArgs& a, const Group<R>& g, float (&v)[R][8],
-                                            float (&u)[GATED ? R : 1][8]) {
-    float c[8];
+// v[i] = v[i] * s * p[i], or v[i] + p[i], for a vector over columns on 16 bytes
+__device__ __forceinline__ void scale_cols(float (&v)[32], float s, const float* p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
+        v[4 * i] *= s * f.x, v[4 * i + 1] *= s * f.y;
+        v[4 * i + 2] *= s * f.z, v[4 * i + 3] *= s * f.w;
+    }
+}
+__device__ __forceinline__ void add_cols(float (&v)[32], const float* p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
+        v[4 * i] += f.x, v[4 * i + 1] += f.y, v[4 * i + 2] += f.z, v[4 * i + 3] += f.w;
+    }
+}
+
+__device__ __forceinline__ void put_one(void* p, long long i, int type, float v) {
+    if (type == BVML_BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
+    else if (type == BVML_F16) static_cast<__half*>(p)[i] = from_f<__half>(v);
+    else static_cast<float*>(p)[i] = v;
+}
+__device__ __forceinline__ float get_one(const void* p, long long i, int type) {
+    if (type == BVML_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
+    if (type == BVML_F16) return to_f(static_cast<const __half*>(p)[i]);
+    return static_cast<const float*>(p)[i];
+}
+
+// One output element of row m, column n from its accumulators.
+template <bool GATED>
+__device__ __forceinline__ void finish_one(const TileArgs& a, long long m, int n, float v,
+                                           float u) {
     if (a.col_scale[0]) {
-        float rs[R];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int m = g.m0 + i * g.step;
-            rs[i] = m < a.M ? __ldg(a.row_scale + m) : 0.0f;
+        const float rs = a.row_scale[m];
+        v *= rs * a.col_scale[0][n];
+        if (GATED) u *= rs * a.col_scale[1][n];
+    }
+    if (GATED) {
+        if (a.save[0]) {
+            put_one(a.save[0], m * a.lds[0] + n, a.out_type, v);
+            put_one(a.save[1], m * a.lds[1] + n, a.out_type, u);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = e < g.left ? __ldg(a.col_scale[0] + g.n + e) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] *= rs[i] * c[e];
-        if constexpr (GATED) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = e < g.left ? __ldg(a.col_scale[1] + g.n + e) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) u[i][e] *= rs[i] * c[e];
-        }
+        v = act_f(v, a.act) * u;
+    } else {
+        if (a.bias) v += a.bias[n];
+        if (a.save[0]) put_one(a.save[0], m * a.lds[0] + n, a.out_type, v);
+        v = act_f(v, a.act);
+        if (a.residual) v += get_one(a.residual, m * a.ldr + n, a.out_type);
+    }
+    if (!a.out2 || m < a.rows0) put_one(a.out, m * a.ldo + n, a.out_type, v);
+    else if (m >= a.rows1) put_one(a.out2, (m - a.rows1) * a.ldo2 + n, a.out_type, v);
+}
+
+// Chunks at the right edge, and rows that start on no 16 bytes: one element after
+// the other, out of line, so that the path that every chunk takes stays short.
+template <bool GATED>
+__device__ __noinline__ void finish_slowly(const TileArgs& a, int m, int n, const float* v,
+                                           const float* u) {
+    const int left = a.N - n < 32 ? a.N - n : 32;
+    for (int i = 0; i < left; ++i) finish_one<GATED>(a, m, n + i, v[i], GATED ? u[i] : 0.0f);
+}
+
+// Epilogue of columns n .. n + 31 of row m, all inside and on 16 bytes; raw: the
+// 16-bit residual's.
+template <bool GATED>
+__device__ __forceinline__ void finish_row(const TileArgs& a, int m, int n, float (&v)[32],
+                                           float (&u)[GATED ? 32 : 1], float row_scale,
+                                           const uint4 (&raw)[4]) {
+    if (a.col_scale[0]) {
+        scale_cols(v, row_scale, a.col_scale[0] + n);
+        if constexpr (GATED) scale_cols(u, row_scale, a.col_scale[1] + n);
     }
     if constexpr (GATED) {
         if (a.save[0]) {
-            put_rows(a.save[0], a.lds[0], a.out_type, g, a.M, v, a.vec & kVecSave);
-            put_rows(a.save[1], a.lds[1], a.out_type, g, a.M, u, a.vec & kVecSave);
+            put_row(a.save[0], m * a.lds[0] + n, a.out_type, v, a.vec & kWideSave);
+            put_row(a.save[1], m * a.lds[1] + n, a.out_type, u, a.vec & kWideSave);
         }
-        act_rows(v, a.act);
+        act_row(v, a.act);
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] *= u[i][e];
+        for (int i = 0; i < 32; ++i) v[i] *= u[i];
     } else {
-        if (a.bias) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = e < g.left ? __ldg(a.bias + g.n + e) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[i][e] += c[e];
-        }
-        if (a.save[0]) put_rows(a.save[0], a.lds[0], a.out_type, g, a.M, v, a.vec & kVecSave);
-        act_rows(v, a.act);
+        if (a.bias) add_cols(v, a.bias + n);
+        if (a.save[0])
+            put_row(a.save[0], m * a.lds[0] + n, a.out_type, v, a.vec & kWideSave);
+        act_row(v, a.act);
         if (a.residual) {
-            const bool vec = a.vec & kVecRes;
-            if (a.out_type == BVML_BF16)
-                add_rows(static_cast<const __nv_bfloat16*>(a.residual), a.ldr, g, a.M, v, vec);
-            else if (a.out_type == BVML_F16)
-                add_rows(static_cast<const __half*>(a.residual), a.ldr, g, a.M, v, vec);
-            else
-                add_rows(static_cast<const float*>(a.residual), a.ldr, g, a.M, v, vec);
-        }
-    }
-    if (!a.out2 || g.m0 + (R - 1) * g.step < a.rows0) {
-        put_rows(a.out, a.ldo, a.out_type, g, a.M, v, a.vec & kVecOut);
-    } else if (g.m0 >= a.rows1) {
-        Group<R> h = g;
-        h.m0 -= a.rows1;
-        put_rows(a.out2, a.ldo2, a.out_type, h, a.M - a.rows1, v, a.vec & kVecOut2);
-    } else {  // the few groups that span the border, row by row
+            if (a.out_type == BVML_F32) {
+                add_cols(v, static_cast<const float*>(a.residual) + m * a.ldr + n);
+            } else {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int m = g.m0 + i * g.step;
-            Group<1> h{m, 0, g.n, g.left};
-            float one[1][8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) one[0][e] = v[i][e];
-            if (m < a.rows0) {
-                put_rows(a.out, a.ldo, a.out_type, h, a.M, one, a.vec & kVecOut);
-            } else if (m >= a.rows1) {
-                h.m0 -= a.rows1;
-                put_rows(a.out2, a.ldo2, a.out_type, h, a.M - a.rows1, one, a.vec & kVecOut2);
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t w = (&raw[i / 4].x)[i % 4];
+                    if (a.out_type == BVML_BF16) {
+                        v[2 * i] += __uint_as_float(w << 16);
+                        v[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
+                    } else {
+                        const float2 f = __half22float2(reinterpret_cast<const __half2&>(w));
+                        v[2 * i] += f.x;
+                        v[2 * i + 1] += f.y;
+                    }
+                }
             }
         }
     }
+    if (!a.out2 || m < a.rows0)
+        put_row(a.out, m * a.ldo + n, a.out_type, v, a.vec & kWideOut);
+    else if (m >= a.rows1)
+        put_row(a.out2, (m - a.rows1) * a.ldo2 + n, a.out_type, v, a.vec & kWideOut);
 }
 
 template <int BN, bool AT, bool BT, bool F8, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
 gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
-    static_assert(!BT || BN >= 128, "a box of B's rows is 64 wide");
+    static_assert(!BT || BN % 128 == 0, "a box of B's rows is 64 wide");
+    static_assert(BN % 64 == 0, "chunks of 32 columns, half of them of each projection");
     static_assert(!F8 || (!AT && !BT), "8-bit operands are row-major");
     constexpr int kStage = tile_stage_bytes<BN>();
-    constexpr int kStages = tile_stages<BN, GATED>();
-    constexpr int kStaging = tile_staging_bytes<GATED>();
+    constexpr int kStages = tile_stages<BN>();
     constexpr int kStep = F8 ? 128 : 64;  // elements of a K step
-    constexpr uint32_t kCols = 2 * BN;    // two accumulators
+    constexpr uint32_t kCols = BN > 128 ? 512 : 2 * BN;  // two accumulators, a power of two
     constexpr int kCN = GATED ? BN / 2 : BN;  // output columns of a tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t sbase = tc::smem_u32(smem);
-    uint8_t* bar_mem = smem + kStages * kStage + kStaging;
+    uint8_t* bar_mem = smem + kStages * kStage;
     const uint32_t bars = tc::smem_u32(bar_mem);
     const uint32_t bar_full = bars;               // kTileMaxStages, counted on the first CTA's
     const uint32_t bar_empty = bars + 64;         // kTileMaxStages, in each CTA
@@ -249,18 +260,24 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     const int works = tiles * a.splits;
     const int steps = a.steps[0] + a.steps[1];
     // work w -> tile row, tile column, K steps [k0, k1); tiles in groups of
-    // kGroup tile rows, so that the pairs at work share operands in L2
+    // kTileGroup tile rows, so that the pairs at work share operands in L2. The
+    // divisions are by numbers known to the host (a 64-bit division here cost
+    // each role 900 cycles a tile).
     auto work_of = [&](int w, int& m0, int& n0, int& k0, int& k1, int& split) {
-        split = w / tiles;
-        const int t = w - split * tiles;
-        constexpr int kGroup = 8;
-        const int per = kGroup * a.tiles_n;
-        const int g = t / per, r = t - g * per;
-        const int gm = a.tiles_m - g * kGroup < kGroup ? a.tiles_m - g * kGroup : kGroup;
-        m0 = (g * kGroup + r % gm) * 256 + (int)rank * 128;
-        n0 = (r / gm) * kCN;
-        k0 = (int)((long long)steps * split / a.splits);
-        k1 = (int)((long long)steps * (split + 1) / a.splits);
+        int t = w;
+        split = 0, k0 = 0, k1 = steps;
+        if (a.splits > 1) {
+            split = tiles > 1 ? (int)divide((uint32_t)w, a.by_tiles) : w;
+            t = w - split * tiles;
+            k0 = (int)((uint32_t)(steps * split) / (uint32_t)a.splits);
+            k1 = (int)((uint32_t)(steps * (split + 1)) / (uint32_t)a.splits);
+        }
+        const int g = (int)divide((uint32_t)t, a.by_group), r = t - g * kTileGroup * a.tiles_n;
+        const int gm = a.tiles_m - g * kTileGroup;  // rows of tiles in the last group
+        const int rn = gm >= kTileGroup ? r / kTileGroup : (int)((uint32_t)r / (uint32_t)gm);
+        const int rm = r - rn * (gm >= kTileGroup ? kTileGroup : gm);
+        m0 = (g * kTileGroup + rm) * 256 + (int)rank * 128;
+        n0 = rn * kCN;
     };
 
     if (threadIdx.x == 0) {
@@ -298,25 +315,23 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
         if (lane == 0) {
             // ------------------------------------------------------ producer
             int i = 0;  // ring entries issued
+            int slot = 0;
+            uint32_t parity = 1;  // of the wait for the slot's hand-back: passes at once at first
             bool ok = true;
+            const uint32_t full0 = tc::map_to(bar_full, 0);
             for (int w = pair; ok && w < works; w += pairs) {
                 int m0, n0, k0, k1, split;
                 work_of(w, m0, n0, k0, k1, split);
+                if (aborted()) break;
                 for (int k = k0; k < k1; ++k, ++i) {
-                    const int s = i % kStages, j = i / kStages;
-                    if (j > 0 && !tc::mbar_wait_pipe(bar_empty + 8 * s, (j - 1) & 1,
-                                                     kTileWaitLimit)) {
+                    if (!tc::mbar_wait_pipe(bar_empty + 8 * slot, parity, kTileWaitLimit)) {
                         fail(1);
                         ok = false;
                         break;
                     }
-                    if (aborted()) {
-                        ok = false;
-                        break;
-                    }
-                    if (rank == 0) tc::mbar_expect_tx(bar_full + 8 * s, 2 * kStage);
-                    const uint32_t full = tc::map_to(bar_full + 8 * s, 0);
-                    const uint32_t sa = sbase + s * kStage, sb = sa + 128 * 128;
+                    if (rank == 0) tc::mbar_expect_tx(bar_full + 8 * slot, 2 * kStage);
+                    const uint32_t full = full0 + 8 * slot;
+                    const uint32_t sa = sbase + slot * kStage, sb = sa + 128 * 128;
                     const int seg = k >= a.steps[0];
                     const int x = (k - (seg ? a.steps[0] : 0)) * kStep;
                     if constexpr (AT) {
@@ -338,6 +353,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                             tc::tma_load_2d_pair(sb, &maps.b[seg], full, x, nb);
                         }
                     }
+                    if (++slot == kStages) slot = 0, parity ^= 1;
                 }
             }
             // nothing may still arrive in shared memory when the pair leaves: the last
@@ -361,12 +377,18 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ----------------------------------------------------------- MMA
-            int i = 0, tl = 0;
+            int slot = 0, tl = 0;
+            uint32_t parity = 0;
             bool ok = true;
+            const uint64_t da0 = AT ? tc::umma_desc_mn_sw128(sbase, 8192)
+                                    : tc::umma_desc_k_sw128(sbase);
+            const uint64_t db0 = BT ? tc::umma_desc_mn_sw128(sbase + 128 * 128, 8192)
+                                    : tc::umma_desc_k_sw128(sbase + 128 * 128);
             for (int w = pair; ok && w < works; w += pairs, ++tl) {
                 int m0, n0, k0, k1, split;
                 work_of(w, m0, n0, k0, k1, split);
                 const int buf = tl & 1, u = tl >> 1;
+                if (aborted()) break;
                 if (u > 0 && !tc::mbar_wait_pipe(bar_acc_empty + 8 * buf, (u - 1) & 1,
                                                  kTileWaitLimit)) {
                     fail(3);
@@ -374,25 +396,22 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                 }
                 tc::tc_fence_after();
                 const uint32_t acc = tmem + buf * BN;
-                for (int k = k0; k < k1; ++k, ++i) {
-                    const int s = i % kStages;
-                    if (!tc::mbar_wait_pipe(bar_full + 8 * s, (i / kStages) & 1, kTileWaitLimit) ||
-                        aborted()) {
+                for (int k = k0; k < k1; ++k) {
+                    if (!tc::mbar_wait_pipe(bar_full + 8 * slot, parity, kTileWaitLimit)) {
                         fail(4);
                         ok = false;
                         break;
                     }
                     tc::tc_fence_after();
-                    const uint32_t sa = sbase + s * kStage, sb = sa + 128 * 128;
-                    const uint64_t da = AT ? tc::umma_desc_mn_sw128(sa, 8192)
-                                           : tc::umma_desc_k_sw128(sa);
-                    const uint64_t db = BT ? tc::umma_desc_mn_sw128(sb, 8192)
-                                           : tc::umma_desc_k_sw128(sb);
+                    // addresses in a descriptor count 16-byte units
+                    const uint64_t da = da0 + (uint32_t)(slot * (kStage >> 4));
+                    const uint64_t db = db0 + (uint32_t)(slot * (kStage >> 4));
 #pragma unroll
                     for (int q = 0; q < 4; ++q)  // 32 bytes of K, or 16 rows of k
                         tc::umma_pair<F8>(acc, da + q * (AT ? 128 : 2), db + q * (BT ? 128 : 2),
                                           a.idesc, k > k0 || q > 0);
-                    tc::umma_commit_pair(bar_empty + 8 * s);
+                    tc::umma_commit_pair(bar_empty + 8 * slot);
+                    if (++slot == kStages) slot = 0, parity ^= 1;
                 }
                 if (ok) tc::umma_commit_pair(bar_acc_full + 8 * buf);
             }
@@ -403,14 +422,32 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     } else {
         // ------------------------------------------------------------ epilogue
         const int quarter = warp & 3;            // the TMEM lanes this warp may read
-        const int part = (warp - 2) >> 2;        // which half of the columns
-        float* stg = reinterpret_cast<float*>(smem + kStages * kStage +
-                                              (warp - 2) * 4096 * (GATED ? 2 : 1));
+        const int part = (warp - 2) >> 2;        // even or odd chunks of 32 columns
+        constexpr int kChunks = kCN / 32;
         const uint32_t acc_empty0 = tc::map_to(bar_acc_empty, 0);
+        // whole chunks of rows on 16 bytes take the short path
+        const bool fast = (a.vec & kOn16) != 0;
+        const bool halves = !GATED && fast && a.residual && a.out_type != BVML_F32;
         int tl = 0;
         for (int w = pair; w < works; w += pairs, ++tl) {
             int m0, n0, k0, k1, split;
             work_of(w, m0, n0, k0, k1, split);
+            const int m = m0 + quarter * 32 + lane;
+            const bool in = m < a.M;
+            // an odd number of chunks falls to either warp in turn
+            const int first = kChunks % 2 ? (part + tl) & 1 : part;
+            uint4 raw[4] = {};
+            auto ask = [&](int chunk) {  // the residual's
+                const int n = n0 + chunk * 32;
+                if (halves && in && chunk < kChunks && n + 32 <= a.N) {
+                    const uint4* p = reinterpret_cast<const uint4*>(
+                        static_cast<const uint16_t*>(a.residual) + m * a.ldr + n);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) raw[i] = p[i];
+                }
+            };
+            ask(first);
+            const float row_scale = a.row_scale && in ? __ldg(a.row_scale + m) : 0.0f;
             const int buf = tl & 1, u = tl >> 1;
             const bool full = tc::mbar_wait_pipe(bar_acc_full + 8 * buf, u & 1, kTileWaitLimit);
             if (!__all_sync(0xffffffffu, full && !aborted())) {  // the whole warp gives up
@@ -419,71 +456,44 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
             }
             tc::tc_fence_after();
             const uint32_t acc = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
-            constexpr int kHalf = kCN / 2;               // columns of this warp
-            constexpr int kW = kHalf < 32 ? kHalf : 32;  // ... at a time
+            auto hand_back = [&]() {  // this warp is done with the accumulator
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive_cluster_relaxed(acc_empty0 + 8 * buf);
+            };
+            if (first >= kChunks) hand_back();
 #pragma unroll 1
-            for (int c = 0; c < kHalf; c += kW) {
-                const int col = part * kHalf + c;
-                // phase 1: a lane holds kW columns of one row; staged as 16-byte units,
-                // unit q of row r at q ^ (r & 7): no bank is hit twice
+            for (int c = first; c < kChunks; c += 2) {
+                const int n = n0 + c * 32;
+                if (c != first) ask(c);
+                float v[32], g[GATED ? 32 : 1];
+                {
+                    uint32_t x[32], y[GATED ? 32 : 1];
+                    tc::tmem_ld_32cols(acc + c * 32, x);
+                    if constexpr (GATED) tc::tmem_ld_32cols(acc + BN / 2 + c * 32, y);
+                    tc::tmem_ld_wait();
 #pragma unroll
-                for (int p = 0; p < (GATED ? 2 : 1); ++p) {
-                    float* d = stg + p * 1024;
-                    if constexpr (kW == 32) {
-                        uint32_t v[32];
-                        tc::tmem_ld_32cols(acc + col + p * (BN / 2), v);
-                        tc::tmem_ld_wait();
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(x[i]);
+                    if constexpr (GATED) {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            *reinterpret_cast<uint4*>(d + lane * 32 + ((q ^ (lane & 7)) << 2)) =
-                                make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                    } else {
-                        static_assert(kW == 32 || kW == 16, "columns a warp takes at a time");
-                        uint32_t v[16];
-                        tc::tmem_ld_16cols(acc + col + p * (BN / 2), v);
-                        tc::tmem_ld_wait();
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            *reinterpret_cast<uint4*>(d + lane * 32 + ((q ^ (lane & 7)) << 2)) =
-                                make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(y[i]);
                     }
                 }
-                if (c + kW == kHalf) {  // this warp is done with the accumulator
-                    tc::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive_cluster(acc_empty0 + 8 * buf);
-                }
-                __syncwarp();
-                // phase 2: a lane finishes eight consecutive columns of R rows
-                constexpr int kGroups = kW / 8;  // lanes of a row, and R
-                constexpr int kRows = 32 / kGroups;
-                const int q = lane % kGroups, r0 = lane / kGroups;
-                const Group<kGroups> grp{m0 + quarter * 32 + r0, kRows, n0 + col + q * 8,
-                                         a.N - (n0 + col + q * 8)};
-                float v[kGroups][8], g[GATED ? kGroups : 1][8];
+                if (c + 2 >= kChunks) hand_back();
+                if (!in || n >= a.N) continue;
+                if (a.slab)  // one of several shares of K, its pitch a multiple of 32
+                    put_row(a.slab, ((long long)split * a.M + m) * a.ldslab + n, BVML_F32, v, true);
+                else if (fast && n + 32 <= a.N)
+                    finish_row<GATED>(a, m, n, v, g, row_scale, raw);
+                else {
+                    // copies: an array whose address leaves lives in memory everywhere
+                    float tv[32], tg[GATED ? 32 : 1];
 #pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    const int r = i * kRows + r0;
+                    for (int i = 0; i < 32; ++i) tv[i] = v[i];
 #pragma unroll
-                    for (int p = 0; p < (GATED ? 2 : 1); ++p) {
-                        const float* d = stg + p * 1024 + r * 32;
-                        const float4 x = *reinterpret_cast<const float4*>(
-                            d + (((2 * q) ^ (r & 7)) << 2));
-                        const float4 y = *reinterpret_cast<const float4*>(
-                            d + (((2 * q + 1) ^ (r & 7)) << 2));
-                        float* o = p == 0 ? v[i] : g[GATED ? i : 0];
-                        o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
-                        o[4] = y.x, o[5] = y.y, o[6] = y.z, o[7] = y.w;
-                    }
+                    for (int i = 0; i < (GATED ? 32 : 1); ++i) tg[i] = g[i];
+                    finish_slowly<GATED>(a, m, n, tv, tg);
                 }
-                if (grp.left > 0) {
-                    if (a.slab)  // one of several shares of K: joined by a second kernel
-                        put_rows(a.slab + (long long)split * a.M * a.ldslab, a.ldslab, grp, a.M,
-                                 v, true);
-                    else
-                        finish_rows<kGroups, GATED>(a, grp, v, g);
-                }
-                __syncwarp();
             }
         }
     }
@@ -497,7 +507,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
 template <int BN, bool AT, bool BT, bool F8, bool GATED>
 cudaError_t launch_tile(const TileMaps& maps, const TileArgs& a, int pairs, cudaStream_t s) {
     auto kern = gemm_tile_kernel<BN, AT, BT, F8, GATED>;
-    constexpr int smem = tile_smem_bytes<BN, GATED>();
+    constexpr int smem = tile_smem_bytes<BN>();
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     kern<<<2 * pairs, kTileThreads, smem, s>>>(maps, a);

@@ -302,8 +302,16 @@ rms_norm_long_kernel(const NormArgs a) {
     }
 }
 
+// Blocks an SM that the backward pass is built for: 64 registers a thread with
+// one group of eight, twice that with two.
+constexpr int backward_blocks(int G, int VPT) {
+    const int threads = G > 32 ? G : kNormThreads;
+    const int n = (VPT == 1 ? 1024 : 512) / threads;
+    return n > 0 ? n : 1;
+}
+
 template <typename T, int G, int VPT>
-__global__ void __launch_bounds__(G > 32 ? G : kNormThreads)
+__global__ void __launch_bounds__(G > 32 ? G : kNormThreads, backward_blocks(G, VPT))
 rms_norm_backward_kernel(const NormBwdArgs a) {
     constexpr int kThreads = G > 32 ? G : kNormThreads;
     constexpr int kRows = kThreads / G;
@@ -427,34 +435,35 @@ rms_norm_backward_long_kernel(const NormBwdArgs a) {
     }
 }
 
-// 32 columns a block, 16 rows side by side
+// 16 columns a block, 32 rows side by side
 template <typename T>
 __global__ void __launch_bounds__(512)
 column_sum_kernel(const float* __restrict__ part, int rows, int cols, T* __restrict__ out) {
-    __shared__ float sh[16][33];
-    const int c = blockIdx.x * 32 + threadIdx.x % 32, r0 = threadIdx.x / 32;
+    __shared__ float sh[32][17];
+    const int x = threadIdx.x % 16, c = blockIdx.x * 16 + x, r0 = threadIdx.x / 16;
     float v = 0.0f;
     if (c < cols) {
 #pragma unroll 8
-        for (int r = r0; r < rows; r += 16) v += part[(long long)r * cols + c];
+        for (int r = r0; r < rows; r += 32) v += part[(long long)r * cols + c];
     }
-    sh[r0][threadIdx.x % 32] = v;
+    sh[r0][x] = v;
     __syncthreads();
     if (r0 == 0 && c < cols) {
-        for (int i = 1; i < 16; ++i) v += sh[i][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) v += sh[i][x];
         out[c] = from_f<T>(v);
     }
 }
 
 // Threads a row and groups of eight a thread, by the row's length: the fewest
 // registers that hold it.
-enum class Shape { G8, G16, G32x1, G32x2, G32x4, G256x1, G256x2, G512x2, G512x4, Long };
+enum class Shape { G8, G16, G32x1, G32x2, G128x1, G256x1, G256x2, G512x2, G512x4, Long };
 Shape shape_of(int K) {
     if (K <= 64) return Shape::G8;
     if (K <= 128) return Shape::G16;
     if (K <= 256) return Shape::G32x1;
     if (K <= 512) return Shape::G32x2;
-    if (K <= 1024) return Shape::G32x4;
+    if (K <= 1024) return Shape::G128x1;
     if (K <= 2048) return Shape::G256x1;
     if (K <= 4096) return Shape::G256x2;
     if (K <= 8192) return Shape::G512x2;
@@ -463,6 +472,7 @@ Shape shape_of(int K) {
 }
 int block_threads(Shape h) {
     switch (h) {
+        case Shape::G128x1: return 128;
         case Shape::G512x2:
         case Shape::G512x4:
         case Shape::Long: return 512;
@@ -474,8 +484,7 @@ int block_rows(Shape h) {
         case Shape::G8: return 32;
         case Shape::G16: return 16;
         case Shape::G32x1:
-        case Shape::G32x2:
-        case Shape::G32x4: return 8;
+        case Shape::G32x2: return 8;
         default: return 1;
     }
 }
@@ -487,7 +496,7 @@ void norm_by_shape(Shape h, int grid, const NormArgs& a, cudaStream_t s) {
         case Shape::G16: rms_norm_kernel<T, 16, 1, Q><<<grid, 256, 0, s>>>(a); break;
         case Shape::G32x1: rms_norm_kernel<T, 32, 1, Q><<<grid, 256, 0, s>>>(a); break;
         case Shape::G32x2: rms_norm_kernel<T, 32, 2, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G32x4: rms_norm_kernel<T, 32, 4, Q><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G128x1: rms_norm_kernel<T, 128, 1, Q><<<grid, 128, 0, s>>>(a); break;
         case Shape::G256x1: rms_norm_kernel<T, 256, 1, Q><<<grid, 256, 0, s>>>(a); break;
         case Shape::G256x2: rms_norm_kernel<T, 256, 2, Q><<<grid, 256, 0, s>>>(a); break;
         case Shape::G512x2: rms_norm_kernel<T, 512, 2, Q><<<grid, 512, 0, s>>>(a); break;
@@ -503,7 +512,7 @@ void norm_backward_by_shape(Shape h, int grid, const NormBwdArgs& a, cudaStream_
         case Shape::G16: rms_norm_backward_kernel<T, 16, 1><<<grid, 256, 0, s>>>(a); break;
         case Shape::G32x1: rms_norm_backward_kernel<T, 32, 1><<<grid, 256, 0, s>>>(a); break;
         case Shape::G32x2: rms_norm_backward_kernel<T, 32, 2><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G32x4: rms_norm_backward_kernel<T, 32, 4><<<grid, 256, 0, s>>>(a); break;
+        case Shape::G128x1: rms_norm_backward_kernel<T, 128, 1><<<grid, 128, 0, s>>>(a); break;
         case Shape::G256x1: rms_norm_backward_kernel<T, 256, 1><<<grid, 256, 0, s>>>(a); break;
         case Shape::G256x2: rms_norm_backward_kernel<T, 256, 2><<<grid, 256, 0, s>>>(a); break;
         case Shape::G512x2: rms_norm_backward_kernel<T, 512, 2><<<grid, 512, 0, s>>>(a); break;
@@ -556,15 +565,27 @@ cudaError_t launch_rms_norm(const NormLaunch& L, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// Blocks of the backward pass, each with a row of partial sums: four blocks of
-// 256 threads an SM (half its threads) on 148 SMs at most. A constant and not
-// the device's count, so that the workspace's size needs no device.
+// Blocks of the backward pass, each with a row of partial sums: what 148 SMs hold
+// at once. A constant and not the device's count, so that the workspace's size
+// needs no device.
 int norm_backward_parts(int T, int K) {
     const Shape h = shape_of(K);
+    int blocks = 1;  // an SM
+    switch (h) {
+        case Shape::G8:
+        case Shape::G16:
+        case Shape::G32x1: blocks = backward_blocks(32, 1); break;
+        case Shape::G32x2: blocks = backward_blocks(32, 2); break;
+        case Shape::G128x1: blocks = backward_blocks(128, 1); break;
+        case Shape::G256x1: blocks = backward_blocks(256, 1); break;
+        case Shape::G256x2: blocks = backward_blocks(256, 2); break;
+        case Shape::G512x2: blocks = backward_blocks(512, 2); break;
+        case Shape::G512x4: blocks = backward_blocks(512, 4); break;
+        case Shape::Long: blocks = 2; break;
+    }
     const long long rows = block_rows(h);
     const long long want = ((long long)T + rows - 1) / rows;
-    const long long most = 148LL * (1024 / block_threads(h));
-    return (int)(want < most ? want : most);
+    return (int)(want < 148LL * blocks ? want : 148LL * blocks);
 }
 
 cudaError_t launch_rms_norm_backward(const NormBackwardLaunch& L, cudaStream_t s) {
@@ -589,7 +610,7 @@ cudaError_t launch_rms_norm_backward(const NormBackwardLaunch& L, cudaStream_t s
 
 cudaError_t launch_column_sum(const float* part, int rows, int cols, void* out, int type,
                               cudaStream_t s) {
-    const int grid = (cols + 31) / 32;
+    const int grid = (cols + 15) / 16;
     if (type == BVML_F32)
         column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols, static_cast<float*>(out));
     else if (type == BVML_F16)

@@ -38,8 +38,11 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
                  : "memory");
     return v;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t remote) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote)
+// Arrive on a barrier of another CTA of the cluster, relaxed: for hand-backs of
+// tensor memory, whose loads have completed (tcgen05.wait::ld). A release would wait
+// until this thread's earlier global stores are visible to the whole cluster.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote)
                  : "memory");
 }
 
