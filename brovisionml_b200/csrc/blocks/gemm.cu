@@ -320,7 +320,12 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
         a.ldslab = p.ldslab;
     }
     a.by_tiles = divide_by((uint32_t)(p.tiles_m * p.tiles_n));
-    a.by_group = divide_by((uint32_t)(kTileGroup * p.tiles_n));
+    // as many tile rows together as keep their rows of A at home in L2 (40 MB of 126:
+    // the rest is for B passing through and the outputs), 4 to 64
+    const long long row = 256LL * (p.steps[0] + p.steps[1]) * 128;
+    a.group = 2;
+    while (a.group < 6 && (row << (a.group + 1)) <= (40LL << 20)) ++a.group;
+    a.by_group = divide_by((uint32_t)(p.tiles_n << a.group));
     int sms = 0;
     if ((e = sm_count(&sms)) != cudaSuccess) return e;
     const long long works = (long long)p.tiles_m * p.tiles_n * p.splits;

@@ -28,8 +28,6 @@ inline Division divide_by(uint32_t d) {
     return v;
 }
 
-constexpr int kTileGroup = 8;  // tile rows that are walked together
-
 // TileArgs::vec
 enum : int {
     kOn16 = 1,     // every row of 32 columns and every vector over columns starts on 16 bytes
@@ -43,7 +41,8 @@ struct TileArgs {
     int tiles_m, tiles_n;
     int splits;            // shares of K, each a work item of its own
     uint32_t idesc;
-    Division by_tiles, by_group;  // tiles_m * tiles_n, kTileGroup * tiles_n
+    int group;                    // 2^group tile rows are walked together
+    Division by_tiles, by_group;  // tiles_m * tiles_n, 2^group * tiles_n
     const float* row_scale;
     const float* col_scale[2];
     const float* bias;

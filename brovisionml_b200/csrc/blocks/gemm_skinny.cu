@@ -81,9 +81,9 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     const uint32_t bar_full = tc::smem_u32(bar_mem), bar_empty = bar_full + 64,
                    bar_acc = bar_full + 128;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 136);
-    int* abort_flag = reinterpret_cast<int*>(bar_mem + 140);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
     const int split = sa.split;
     const int rank = blockIdx.x % split;  // the cluster's CTAs are neighbours in x
     const int f0 = (blockIdx.x / split) * kFeatures, t0 = blockIdx.y * TOK;
@@ -96,7 +96,6 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
             tc::mbar_init(bar_empty + 8 * s, 1);
         }
         tc::mbar_init(bar_acc, 1);
-        *abort_flag = 0;
         tc::mbar_fence_init();
     }
     if (warp == 1) {
@@ -106,53 +105,50 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-    auto fail = [&](int code) {
-        atomicExch(&g_tile_error, code);
-        *reinterpret_cast<volatile int*>(abort_flag) = 1;
+    auto fail = [&](int code) { atomicExch(&g_tile_error, code); };
+    auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {  // a whole warp's wait
+        const bool done = tc::mbar_wait_pipe(bar, parity, kTileWaitLimit);
+        if (__all_sync(0xffffffffu, done)) return true;
+        if (lane == 0) fail(code);
+        return false;
     };
-    if (warp == 0 && lane == 0) {
-        int i = 0;
+    if (warp == 0) {
+        const uint32_t on = tc::elect_one();
+        int i = 0, slot = 0;
+        uint32_t phase = 1;
         for (int k = k0; k < k1; ++k, ++i) {
-            const int s = i % kStages, j = i / kStages;
-            if (j > 0 &&
-                !tc::mbar_wait_pipe(bar_empty + 8 * s, (j - 1) & 1, kTileWaitLimit)) {
-                fail(11);
-                break;
-            }
-            if (*reinterpret_cast<volatile int*>(abort_flag)) break;
-            tc::mbar_expect_tx(bar_full + 8 * s, kStage);
-            const uint32_t d = sbase + s * kStage;
-            tc::tma_load_2d(d, &maps.b[0], bar_full + 8 * s, k * kStep, f0);
+            if (!wait_all(bar_empty + 8 * slot, phase, 11)) break;
+            tc::mbar_expect_tx_on(on, bar_full + 8 * slot, kStage);
+            const uint32_t d = sbase + slot * kStage;
+            tc::tma_load_2d(on, d, &maps.b[0], bar_full + 8 * slot, k * kStep, f0);
             if constexpr (GATED)
-                tc::tma_load_2d(d + 8192, &maps.b[1], bar_full + 8 * s, k * kStep, f0);
-            tc::tma_load_2d(d + 128 * 128, &maps.a[0], bar_full + 8 * s, k * kStep, t0);
+                tc::tma_load_2d(on, d + 8192, &maps.b[1], bar_full + 8 * slot, k * kStep, f0);
+            tc::tma_load_2d(on, d + 128 * 128, &maps.a[0], bar_full + 8 * slot, k * kStep, t0);
+            if (++slot == kStages) slot = 0, phase ^= 1;
         }
         // no copy may still be landing when the ring is used anew
         for (int q = i > kStages ? i - kStages : 0; q < i; ++q)
-            if (!tc::mbar_wait(bar_full + 8 * (q % kStages), (q / kStages) & 1, kTileWaitLimit)) {
-                fail(12);
-                break;
-            }
-    } else if (warp == 1 && lane == 0) {
-        int i = 0;
-        for (int k = k0; k < k1; ++k, ++i) {
-            const int s = i % kStages;
-            if (!tc::mbar_wait_pipe(bar_full + 8 * s, (i / kStages) & 1, kTileWaitLimit) ||
-                *reinterpret_cast<volatile int*>(abort_flag)) {
-                fail(13);
-                break;
-            }
+            if (!wait_all(bar_full + 8 * (q % kStages), (q / kStages) & 1, 12)) break;
+    } else if (warp == 1) {
+        const uint32_t on = tc::elect_one();
+        int slot = 0;
+        uint32_t phase = 0;
+        const uint64_t dw0 = tc::umma_desc_k_sw128(sbase);
+        const uint64_t dx0 = tc::umma_desc_k_sw128(sbase + 128 * 128);
+        for (int k = k0; k < k1; ++k) {
+            if (!wait_all(bar_full + 8 * slot, phase, 13)) break;
             tc::tc_fence_after();
-            const uint64_t dw = tc::umma_desc_k_sw128(sbase + s * kStage);
-            const uint64_t dx = tc::umma_desc_k_sw128(sbase + s * kStage + 128 * 128);
+            const uint64_t dw = dw0 + (uint32_t)(slot * (kStage >> 4));
+            const uint64_t dx = dx0 + (uint32_t)(slot * (kStage >> 4));
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                tc::umma_single<F8>(tmem, dw + 2 * q, dx + 2 * q, a.idesc, i > 0 || q > 0);
-            tc::umma_commit(bar_empty + 8 * s);
+                tc::umma_single<F8>(on, tmem, dw + 2 * q, dx + 2 * q, a.idesc, k > k0 || q > 0);
+            tc::umma_commit_on(on, bar_empty + 8 * slot);
+            if (++slot == kStages) slot = 0, phase ^= 1;
         }
-        tc::umma_commit(bar_acc);
+        tc::umma_commit_on(on, bar_acc);
     }
     __syncwarp();
     // the accumulator, and with it every copy and MMA, is complete

@@ -11,7 +11,7 @@
 // accumulator holds both projections of BN / 2 features side by side.
 //
 // Persistent, one pair on two SMs:
-//  * warp 0 (one lane, in both CTAs) streams operands by TMA in 128-byte swizzled
+//  * warp 0 (in both CTAs) streams operands by TMA in 128-byte swizzled
 //    rows of one K step (64 16-bit or 128 8-bit elements) through a ring; the bytes
 //    of both CTAs are counted on the first CTA's barrier;
 //  * warp 1 of the first CTA issues the MMAs of the pair, and hands ring entries
@@ -253,14 +253,15 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 168);
     int* abort_flag = reinterpret_cast<int*>(bar_mem + 172);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int tiles = a.tiles_m * a.tiles_n;
     const int works = tiles * a.splits;
     const int steps = a.steps[0] + a.steps[1];
     // work w -> tile row, tile column, K steps [k0, k1); tiles in groups of
-    // kTileGroup tile rows, so that the pairs at work share operands in L2. The
+    // 2^group tile rows, so that the pairs at work share operands in L2. The
     // divisions are by numbers known to the host (a 64-bit division here cost
     // each role 900 cycles a tile).
     auto work_of = [&](int w, int& m0, int& n0, int& k0, int& k1, int& split) {
@@ -272,11 +273,12 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
             k0 = (int)((uint32_t)(steps * split) / (uint32_t)a.splits);
             k1 = (int)((uint32_t)(steps * (split + 1)) / (uint32_t)a.splits);
         }
-        const int g = (int)divide((uint32_t)t, a.by_group), r = t - g * kTileGroup * a.tiles_n;
-        const int gm = a.tiles_m - g * kTileGroup;  // rows of tiles in the last group
-        const int rn = gm >= kTileGroup ? r / kTileGroup : (int)((uint32_t)r / (uint32_t)gm);
-        const int rm = r - rn * (gm >= kTileGroup ? kTileGroup : gm);
-        m0 = (g * kTileGroup + rm) * 256 + (int)rank * 128;
+        const int g = (int)divide((uint32_t)t, a.by_group), r = t - (g << a.group) * a.tiles_n;
+        const int gm = a.tiles_m - (g << a.group);  // rows of tiles in the last group
+        const bool whole = gm >= 1 << a.group;
+        const int rn = whole ? r >> a.group : (int)((uint32_t)r / (uint32_t)gm);
+        const int rm = r - (whole ? rn << a.group : rn * gm);
+        m0 = ((g << a.group) + rm) * 256 + (int)rank * 128;
         n0 = rn * kCN;
     };
 
@@ -303,7 +305,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     __syncthreads();
     tc::cluster_sync();  // the peer's barriers exist before anything arrives on them
     tc::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     auto fail = [&](int code) {
         atomicExch(&g_tile_error, code);
@@ -311,72 +313,74 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     };
     auto aborted = [&]() { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
 
+    // A wait of a whole warp: every lane polls, and they agree.
+    auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
+        const bool done = tc::mbar_wait_pipe(bar, parity, kTileWaitLimit);
+        if (__all_sync(0xffffffffu, done)) return true;
+        if (lane == 0) fail(code);
+        return false;
+    };
+    auto gone = [&]() { return __any_sync(0xffffffffu, aborted()) != 0; };
+
     if (warp == 0) {
-        if (lane == 0) {
-            // ------------------------------------------------------ producer
-            int i = 0;  // ring entries issued
-            int slot = 0;
-            uint32_t parity = 1;  // of the wait for the slot's hand-back: passes at once at first
-            bool ok = true;
-            const uint32_t full0 = tc::map_to(bar_full, 0);
-            for (int w = pair; ok && w < works; w += pairs) {
-                int m0, n0, k0, k1, split;
-                work_of(w, m0, n0, k0, k1, split);
-                if (aborted()) break;
-                for (int k = k0; k < k1; ++k, ++i) {
-                    if (!tc::mbar_wait_pipe(bar_empty + 8 * slot, parity, kTileWaitLimit)) {
-                        fail(1);
-                        ok = false;
-                        break;
-                    }
-                    if (rank == 0) tc::mbar_expect_tx(bar_full + 8 * slot, 2 * kStage);
-                    const uint32_t full = full0 + 8 * slot;
-                    const uint32_t sa = sbase + slot * kStage, sb = sa + 128 * 128;
-                    const int seg = k >= a.steps[0];
-                    const int x = (k - (seg ? a.steps[0] : 0)) * kStep;
-                    if constexpr (AT) {
-                        tc::tma_load_2d_pair(sa, &maps.a[seg], full, m0, x);
-                        tc::tma_load_2d_pair(sa + 8192, &maps.a[seg], full, m0 + 64, x);
-                    } else {
-                        tc::tma_load_2d_pair(sa, &maps.a[seg], full, x, m0);
-                    }
-                    if constexpr (GATED) {
-                        tc::tma_load_2d_pair(sb, &maps.b[rank], full, x, n0);
-                    } else {
-                        const int nb = n0 + (int)rank * (BN / 2);
-                        if constexpr (BT) {
-#pragma unroll
-                            for (int c = 0; c < BN / 128; ++c)
-                                tc::tma_load_2d_pair(sb + c * 8192, &maps.b[seg], full,
-                                                     nb + 64 * c, x);
-                        } else {
-                            tc::tma_load_2d_pair(sb, &maps.b[seg], full, x, nb);
-                        }
-                    }
-                    if (++slot == kStages) slot = 0, parity ^= 1;
-                }
-            }
-            // nothing may still arrive in shared memory when the pair leaves: the last
-            // round's entries have been consumed and handed back (to both CTAs);
-            // after an abort the copies at least have landed (the first CTA's
-            // barriers count both CTAs' bytes)
-            const int q0 = i > kStages ? i - kStages : 0;
-            for (int q = q0; ok && q < i; ++q) {
-                if (!tc::mbar_wait(bar_empty + 8 * (q % kStages), (q / kStages) & 1,
-                                   kTileWaitLimit)) {
-                    fail(2);
+        // ---------------------------------------------------------- producer
+        const uint32_t on = tc::elect_one();
+        const uint32_t first_on = rank == 0 ? on : 0;
+        int i = 0;  // ring entries issued
+        int slot = 0;
+        uint32_t parity = 1;  // of the wait for the slot's hand-back: passes at once at first
+        bool ok = true;
+        const uint32_t full0 = tc::map_to(bar_full, 0);
+        for (int w = pair; ok && w < works; w += pairs) {
+            int m0, n0, k0, k1, split;
+            work_of(w, m0, n0, k0, k1, split);
+            if (gone()) break;
+            for (int k = k0; k < k1; ++k, ++i) {
+                if (!wait_all(bar_empty + 8 * slot, parity, 1)) {
                     ok = false;
+                    break;
                 }
+                tc::mbar_expect_tx_on(first_on, bar_full + 8 * slot, 2 * kStage);
+                const uint32_t full = full0 + 8 * slot;
+                const uint32_t sa = sbase + slot * kStage, sb = sa + 128 * 128;
+                const int seg = k >= a.steps[0];
+                const int x = (k - (seg ? a.steps[0] : 0)) * kStep;
+                if constexpr (AT) {
+                    tc::tma_load_2d_pair(on, sa, &maps.a[seg], full, m0, x);
+                    tc::tma_load_2d_pair(on, sa + 8192, &maps.a[seg], full, m0 + 64, x);
+                } else {
+                    tc::tma_load_2d_pair(on, sa, &maps.a[seg], full, x, m0);
+                }
+                if constexpr (GATED) {
+                    tc::tma_load_2d_pair(on, sb, &maps.b[rank], full, x, n0);
+                } else {
+                    const int nb = n0 + (int)rank * (BN / 2);
+                    if constexpr (BT) {
+#pragma unroll
+                        for (int c = 0; c < BN / 128; ++c)
+                            tc::tma_load_2d_pair(on, sb + c * 8192, &maps.b[seg], full,
+                                                 nb + 64 * c, x);
+                    } else {
+                        tc::tma_load_2d_pair(on, sb, &maps.b[seg], full, x, nb);
+                    }
+                }
+                if (++slot == kStages) slot = 0, parity ^= 1;
             }
-            if (!ok && rank == 0)
-                for (int q = q0; q < i; ++q)
-                    if (!tc::mbar_wait(bar_full + 8 * (q % kStages), (q / kStages) & 1,
-                                       kTileWaitLimit))
-                        break;
         }
+        // nothing may still arrive in shared memory when the pair leaves: the last
+        // round's entries have been consumed and handed back (to both CTAs);
+        // after an abort the copies at least have landed (the first CTA's
+        // barriers count both CTAs' bytes)
+        const int q0 = i > kStages ? i - kStages : 0;
+        for (int q = q0; ok && q < i; ++q)
+            ok = wait_all(bar_empty + 8 * (q % kStages), (q / kStages) & 1, 2);
+        if (!ok && rank == 0)
+            for (int q = q0; q < i; ++q)
+                if (!wait_all(bar_full + 8 * (q % kStages), (q / kStages) & 1, 2)) break;
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             // ----------------------------------------------------------- MMA
+            const uint32_t on = tc::elect_one();
             int slot = 0, tl = 0;
             uint32_t parity = 0;
             bool ok = true;
@@ -388,17 +392,12 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                 int m0, n0, k0, k1, split;
                 work_of(w, m0, n0, k0, k1, split);
                 const int buf = tl & 1, u = tl >> 1;
-                if (aborted()) break;
-                if (u > 0 && !tc::mbar_wait_pipe(bar_acc_empty + 8 * buf, (u - 1) & 1,
-                                                 kTileWaitLimit)) {
-                    fail(3);
-                    break;
-                }
+                if (gone()) break;
+                if (u > 0 && !wait_all(bar_acc_empty + 8 * buf, (u - 1) & 1, 3)) break;
                 tc::tc_fence_after();
                 const uint32_t acc = tmem + buf * BN;
                 for (int k = k0; k < k1; ++k) {
-                    if (!tc::mbar_wait_pipe(bar_full + 8 * slot, parity, kTileWaitLimit)) {
-                        fail(4);
+                    if (!wait_all(bar_full + 8 * slot, parity, 4)) {
                         ok = false;
                         break;
                     }
@@ -408,21 +407,22 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                     const uint64_t db = db0 + (uint32_t)(slot * (kStage >> 4));
 #pragma unroll
                     for (int q = 0; q < 4; ++q)  // 32 bytes of K, or 16 rows of k
-                        tc::umma_pair<F8>(acc, da + q * (AT ? 128 : 2), db + q * (BT ? 128 : 2),
-                                          a.idesc, k > k0 || q > 0);
-                    tc::umma_commit_pair(bar_empty + 8 * slot);
+                        tc::umma_pair<F8>(on, acc, da + q * (AT ? 128 : 2),
+                                          db + q * (BT ? 128 : 2), a.idesc, k > k0 || q > 0);
+                    tc::umma_commit_pair(on, bar_empty + 8 * slot);
                     if (++slot == kStages) slot = 0, parity ^= 1;
                 }
-                if (ok) tc::umma_commit_pair(bar_acc_full + 8 * buf);
+                if (ok) tc::umma_commit_pair(on, bar_acc_full + 8 * buf);
             }
             // every issued MMA has completed, after an abort too
-            tc::umma_commit_pair_local(bar_end);
-            if (!tc::mbar_wait(bar_end, 0, kTileWaitLimit)) fail(5);
+            tc::umma_commit_pair_local(on, bar_end);
+            wait_all(bar_end, 0, 5);
         }
     } else {
         // ------------------------------------------------------------ epilogue
         const int quarter = warp & 3;            // the TMEM lanes this warp may read
-        const int part = (warp - 2) >> 2;        // even or odd chunks of 32 columns
+        constexpr int kParts = kTileEpiWarps / 4;
+        const int part = (warp - 2) >> 2;        // every kParts-th chunk of 32 columns
         constexpr int kChunks = kCN / 32;
         const uint32_t acc_empty0 = tc::map_to(bar_acc_empty, 0);
         // whole chunks of rows on 16 bytes take the short path
@@ -434,8 +434,8 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
             work_of(w, m0, n0, k0, k1, split);
             const int m = m0 + quarter * 32 + lane;
             const bool in = m < a.M;
-            // an odd number of chunks falls to either warp in turn
-            const int first = kChunks % 2 ? (part + tl) & 1 : part;
+            // chunks that do not go round fall to one warp after the other
+            const int first = kChunks % kParts ? (part + tl) % kParts : part;
             uint4 raw[4] = {};
             auto ask = [&](int chunk) {  // the residual's
                 const int n = n0 + chunk * 32;
@@ -449,11 +449,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
             ask(first);
             const float row_scale = a.row_scale && in ? __ldg(a.row_scale + m) : 0.0f;
             const int buf = tl & 1, u = tl >> 1;
-            const bool full = tc::mbar_wait_pipe(bar_acc_full + 8 * buf, u & 1, kTileWaitLimit);
-            if (!__all_sync(0xffffffffu, full && !aborted())) {  // the whole warp gives up
-                if (lane == 0) fail(6);
-                break;
-            }
+            if (!wait_all(bar_acc_full + 8 * buf, u & 1, 6) || gone()) break;
             tc::tc_fence_after();
             const uint32_t acc = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
             auto hand_back = [&]() {  // this warp is done with the accumulator
@@ -463,7 +459,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
             };
             if (first >= kChunks) hand_back();
 #pragma unroll 1
-            for (int c = first; c < kChunks; c += 2) {
+            for (int c = first; c < kChunks; c += kParts) {
                 const int n = n0 + c * 32;
                 if (c != first) ask(c);
                 float v[32], g[GATED ? 32 : 1];
@@ -479,7 +475,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                         for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(y[i]);
                     }
                 }
-                if (c + 2 >= kChunks) hand_back();
+                if (c + kParts >= kChunks) hand_back();
                 if (!in || n >= a.N) continue;
                 if (a.slab)  // one of several shares of K, its pitch a multiple of 32
                     put_row(a.slab, ((long long)split * a.M + m) * a.ldslab + n, BVML_F32, v, true);

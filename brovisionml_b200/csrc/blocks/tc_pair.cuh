@@ -46,22 +46,49 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote) {
                  : "memory");
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int c0, int c1) {
+// One lane of the warp, chosen by the hardware. The loops that feed the tensor
+// cores are walked by the whole warp, and only the instructions below are
+// carried out by this lane (`on`): in a branch that one lane takes, every
+// descriptor and address goes through vector registers first (130 cycles for an
+// MMA, 580 a K step of which the tensor cores need 512 or fewer).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t on;
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(on));
+    return on;
+}
+__device__ __forceinline__ void mbar_expect_tx_on(uint32_t on, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.u32 q, %2, 0;\n\t"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+        "r"(bytes), "r"(on)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t on, uint32_t dst, const CUtensorMap* map,
+                                            uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.u32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(on)
         : "memory");
 }
 // The same, its bytes counted on a barrier of either CTA of the pair (`bar` a
 // shared::cluster address).
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map,
-                                                 uint32_t bar, int c0, int c1) {
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t on, uint32_t dst,
+                                                 const CUtensorMap* map, uint32_t bar, int c0,
+                                                 int c1) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.u32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(on)
         : "memory");
 }
 
@@ -91,55 +118,59 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
 }
 // D (256 rows, 128 in each CTA) (+)= A B^T: each CTA holds its 128 rows of A and
 // half of B's rows; K = 32 bytes of each row. F8: e4m3 operands.
+#define BVML_UMMA(group, kind)                                                                \
+    asm volatile(                                                                             \
+        "{\n\t.reg .pred p, q;\n\t"                                                           \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                           \
+        "setp.ne.b32 q, %5, 0;\n\t"                                                           \
+        "@q tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(   \
+            tmem_d),                                                                          \
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate), "r"(on)              \
+        : "memory")
 template <bool F8>
-__device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, bool accumulate) {
-    if constexpr (F8) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
-            : "memory");
-    } else {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
-            : "memory");
-    }
+__device__ __forceinline__ void umma_pair(uint32_t on, uint32_t tmem_d, uint64_t a_desc,
+                                          uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    if constexpr (F8) BVML_UMMA("2", "f8f6f4");
+    else BVML_UMMA("2", "f16");
 }
 // ... and one CTA's: D (128 rows), K = 32 bytes.
 template <bool F8>
-__device__ __forceinline__ void umma_single(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc,
-                                            uint32_t idesc, bool accumulate) {
-    if constexpr (F8) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
-            : "memory");
-    } else {
-        umma_f16(tmem_d, a_desc, b_desc, idesc, accumulate);
-    }
+__device__ __forceinline__ void umma_single(uint32_t on, uint32_t tmem_d, uint64_t a_desc,
+                                            uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    if constexpr (F8) BVML_UMMA("1", "f8f6f4");
+    else BVML_UMMA("1", "f16");
 }
+#undef BVML_UMMA
 // Arrive on the barrier at this offset in both CTAs of the pair once every MMA
 // issued before by this thread has completed.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+__device__ __forceinline__ void umma_commit_pair(uint32_t on, uint32_t bar) {
     asm volatile(
-        "{\n\t.reg .b16 m;\n\t"
+        "{\n\t.reg .b16 m;\n\t.reg .pred q;\n\t"
         "mov.b16 m, 3;\n\t"
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-        " [%0], m;\n\t}" ::"r"(bar)
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], m;\n\t}" ::"r"(bar), "r"(on)
         : "memory");
 }
 // ... on this CTA's barrier alone.
-__device__ __forceinline__ void umma_commit_pair_local(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     bar)
-                 : "memory");
+__device__ __forceinline__ void umma_commit_pair_local(uint32_t on, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            bar),
+        "r"(on)
+        : "memory");
+}
+// ... and one CTA's MMAs.
+__device__ __forceinline__ void umma_commit_on(uint32_t on, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            bar),
+        "r"(on)
+        : "memory");
 }
 // 16 consecutive fp32 columns of this warp's 32 TMEM lanes, one lane per thread.
 __device__ __forceinline__ void tmem_ld_16cols(uint32_t taddr, uint32_t (&v)[16]) {
