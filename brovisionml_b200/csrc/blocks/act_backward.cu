@@ -3,8 +3,8 @@
 //   gated   dg = dh u act'(g), du = dh act(g)
 //
 // Bound by HBM: each input is read once, 16 bytes a thread and access; a block
-// covers up to 2048 columns and walks rows two at a time, a thread keeps eight
-// columns' sums in registers. The sums over a block's rows and over blocks run in a fixed
+// covers up to 2048 columns and walks rows, the next rows' loads in flight; a
+// thread keeps eight columns' sums in registers. The sums over a block's rows and over blocks run in a fixed
 // order. What the matrix products read back (dz, dg, du) is rounded to 16 bits,
 // the type the tensor cores take; the bias gradient sums the 32-bit values.
 #include "blocks_common.cuh"
@@ -16,16 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Up to eight columns c .. of row pointer p as floats, zeros past n.
-template <typename T>
-__device__ __forceinline__ void load_cols(const T* p, int c, int n, bool vec, float (&v)[8]) {
-    if (vec && c + 8 <= n) {
-        load8(p + c, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < n ? to_f(p[c + e]) : 0.0f;
-    }
-}
+// Up to eight columns c .. of row pointer p; what lies past n is left.
 template <typename T>
 __device__ __forceinline__ void store_cols(T* p, int c, int n, bool vec, const float (&v)[8]) {
     if (vec && c + 8 <= n) {
@@ -34,73 +25,6 @@ __device__ __forceinline__ void store_cols(T* p, int c, int n, bool vec, const f
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (c + e < n) p[c + e] = from_f<T>(v[e]);
-    }
-}
-
-// Activation derivatives of two rows' groups of eight, the choice of the
-// activation outside the loops: v <- v act'(z).
-__device__ __forceinline__ void times_grad(int act, const float (&z)[2][8], float (&v)[2][8]) {
-    switch (act) {
-#define BVML_TIMES_GRAD(code)                                 \
-    case code:                                                \
-        _Pragma("unroll") for (int i = 0; i < 2; ++i)         \
-            _Pragma("unroll") for (int e = 0; e < 8; ++e) {   \
-                float f, d;                                   \
-                act_grad_f(z[i][e], code, f, d);              \
-                v[i][e] *= d;                                 \
-            }                                                 \
-        break;
-        BVML_TIMES_GRAD(BVML_ACT_RELU)
-        BVML_TIMES_GRAD(BVML_ACT_SIGMOID)
-        BVML_TIMES_GRAD(BVML_ACT_TANH)
-        BVML_TIMES_GRAD(BVML_ACT_SILU)
-        BVML_TIMES_GRAD(BVML_ACT_GELU)
-#undef BVML_TIMES_GRAD
-        default: break;
-    }
-}
-
-// A block covers `span` threads of eight columns by kThreads / span rows at a time.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-act_backward_kernel(const ActBackwardLaunch L, int span, bool vec_dy, bool vec_z, bool vec_dz) {
-    __shared__ float sh[kThreads * 8];
-    const int x = threadIdx.x % span, ry = threadIdx.x / span, rows = blockDim.x / span;
-    const int c = (blockIdx.x * span + x) * 8;
-    float sum[8] = {};
-    const long long stride = (long long)gridDim.y * rows;
-    if (c < L.N) {
-        for (long long t0 = (long long)blockIdx.y * rows + ry; t0 < L.T; t0 += 2 * stride) {
-            float d[2][8], z[2][8];
-            const bool two = t0 + stride < L.T;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const long long t = i && two ? t0 + stride : t0;
-                load_cols(static_cast<const T*>(L.dy) + t * L.lddy, c, L.N, vec_dy, d[i]);
-                if (L.z) load_cols(static_cast<const T*>(L.z) + t * L.ldz, c, L.N, vec_z, z[i]);
-            }
-            if (L.z) times_grad(L.act, z, d);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (i && !two) continue;
-                const long long t = t0 + i * stride;
-                if (L.dz) store_cols(static_cast<T*>(L.dz) + t * L.lddz, c, L.N, vec_dz, d[i]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] += d[i][e];
-            }
-        }
-    }
-    if (!L.partial) return;
-    // the block's rows side by side, added in their order
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sh[threadIdx.x * 8 + e] = sum[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < span * 8; i += blockDim.x) {
-        const int n = blockIdx.x * span * 8 + i;
-        if (n >= L.N) break;
-        float v = sh[i];
-        for (int r = 1; r < rows; ++r) v += sh[r * span * 8 + i];
-        L.partial[(long long)blockIdx.y * L.N + n] = v;
     }
 }
 
@@ -116,6 +40,79 @@ __device__ __forceinline__ void ask_cols(const T* p, int c, int n, bool vec, Raw
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) r.e[e] = c + e < n ? p[c + e] : from_f<T>(0.0f);
+    }
+}
+
+// v <- v act'(z); the activation is chosen outside the loop
+__device__ __forceinline__ void times_grad(int act, const float (&z)[8], float (&v)[8]) {
+    switch (act) {
+#define BVML_TIMES_GRAD(code)                             \
+    case code:                                            \
+        _Pragma("unroll") for (int e = 0; e < 8; ++e) {   \
+            float f, d;                                   \
+            act_grad_f(z[e], code, f, d);                 \
+            v[e] *= d;                                    \
+        }                                                 \
+        break;
+        BVML_TIMES_GRAD(BVML_ACT_RELU)
+        BVML_TIMES_GRAD(BVML_ACT_SIGMOID)
+        BVML_TIMES_GRAD(BVML_ACT_TANH)
+        BVML_TIMES_GRAD(BVML_ACT_SILU)
+        BVML_TIMES_GRAD(BVML_ACT_GELU)
+#undef BVML_TIMES_GRAD
+        default: break;
+    }
+}
+
+// A block covers `span` threads of eight columns by blockDim.x / span rows at a time.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4)
+act_backward_kernel(const ActBackwardLaunch L, int span, bool vec_dy, bool vec_z, bool vec_dz) {
+    __shared__ float sh[kThreads * 8];
+    const int x = threadIdx.x % span, ry = threadIdx.x / span, rows = blockDim.x / span;
+    const int c = (blockIdx.x * span + x) * 8;
+    float sum[8] = {};
+    const long long stride = (long long)gridDim.y * rows;
+    if (c < L.N) {
+        // the next two rows' loads are in flight while a row is computed
+        Raw<T> rd[2], rz[2];
+        auto ask = [&](long long t, int i) {
+            if (t >= L.T) return;
+            ask_cols(static_cast<const T*>(L.dy) + t * L.lddy, c, L.N, vec_dy, rd[i]);
+            if (L.z) ask_cols(static_cast<const T*>(L.z) + t * L.ldz, c, L.N, vec_z, rz[i]);
+        };
+        const long long t0 = (long long)blockIdx.y * rows + ry;
+        ask(t0, 0);
+        ask(t0 + stride, 1);
+        for (long long t = t0; t < L.T;) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i, t += stride) {
+                if (t >= L.T) break;
+                float d[8], z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    d[e] = to_f(rd[i].e[e]);
+                    z[e] = to_f(rz[i].e[e]);
+                }
+                ask(t + 2 * stride, i);
+                if (L.z) times_grad(L.act, z, d);
+                if (L.dz) store_cols(static_cast<T*>(L.dz) + t * L.lddz, c, L.N, vec_dz, d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += d[e];
+            }
+        }
+    }
+    if (!L.partial) return;
+    // the block's rows side by side, added in their order
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sh[threadIdx.x * 8 + e] = sum[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < span * 8; i += blockDim.x) {
+        const int n = blockIdx.x * span * 8 + i;
+        if (n >= L.N) break;
+        float v = sh[i];
+        for (int r = 1; r < rows; ++r) v += sh[r * span * 8 + i];
+        L.partial[(long long)blockIdx.y * L.N + n] = v;
     }
 }
 
@@ -187,23 +184,26 @@ Cover cover(int N) {
     c.rows = kThreads / c.span;
     return c;
 }
-// Blocks along the rows: about eight an SM (148) in all, so that there are
-// bytes enough in flight and few partial sums.
-int row_blocks(int T, int N) {
+// Blocks along the rows: 1024 threads an SM (148) in all, what is resident at
+// once, so that there are bytes enough in flight and few partial sums.
+// `turns` times as many where nothing is summed: blocks that start as others end
+// keep the loads coming (gated, 8191 x 5632: 80 us with two turns, 92 with one).
+int row_blocks(int T, int N, int turns) {
     const Cover c = cover(N);
     const long long rows = ((long long)T + c.rows - 1) / c.rows;
-    const long long want = (148 * 8 + c.blocks - 1) / c.blocks;
+    const int per_sm = 1024 / ((c.span * c.rows + 31) / 32 * 32);
+    const long long want = (148LL * per_sm * turns + c.blocks - 1) / c.blocks;
     return (int)(want < rows ? want : rows);
 }
 
 }  // namespace
 
-int act_backward_parts(int T, int N) { return row_blocks(T, N); }
+int act_backward_parts(int T, int N) { return row_blocks(T, N, 1); }
 
 cudaError_t launch_act_backward(const ActBackwardLaunch& L, cudaStream_t s) {
     if (L.T == 0) return cudaSuccess;
     const Cover v = cover(L.N);
-    const dim3 grid(v.blocks, row_blocks(L.T, L.N));
+    const dim3 grid(v.blocks, row_blocks(L.T, L.N, 1));
     const int span = v.span, threads = v.span * v.rows;
     const bool a = on16(L.dy, L.lddy, 2), b = L.z && on16(L.z, L.ldz, 2),
                c = L.dz && on16(L.dz, L.lddz, 2);
@@ -217,7 +217,7 @@ cudaError_t launch_act_backward(const ActBackwardLaunch& L, cudaStream_t s) {
 cudaError_t launch_gated_backward(const GatedBackwardLaunch& L, cudaStream_t s) {
     if (L.T == 0) return cudaSuccess;
     const Cover v = cover(L.F);
-    const dim3 grid(v.blocks, row_blocks(L.T, L.F));
+    const dim3 grid(v.blocks, row_blocks(L.T, L.F, 2));
     const int span = v.span, threads = v.span * v.rows;
     const bool a = on16(L.dh, L.lddh, 2), b = on16(L.g, L.ldg, 2), c = on16(L.u, L.ldu, 2),
                d = on16(L.dg, L.ldd, 2) && on16(L.du, L.ldd, 2);

@@ -41,19 +41,19 @@ struct Plan {
 
 int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 
-// A product's cost in K steps of a 256-column tile, by the number of turns that the
-// pairs take. A narrower tile loads more bytes a flop and keeps the tensor cores
-// less busy, which the weights carry (measured on square products: 128 columns
-// run at about 0.9, 64 at about 0.7 of the rate of 256); `tail` is what a turn costs
-// beside its K steps (filling the ring, draining the last accumulator).
-double tile_cost(int tiles, int steps, int splits, int bn) {
-    const double rate = bn == 256 ? 1.0 : bn == 192 ? 0.79 : bn == 128 ? 0.56 : 0.36;
-    const double tail = bn == 256 ? 5.0 : bn == 192 ? 4.2 : bn == 128 ? 3.5 : 2.5;
-    const long long works = (long long)tiles * splits;
-    const long long turns = (works + kPairs - 1) / kPairs;
-    // joining the shares reads and writes the output once more for each
-    const double join = splits > 1 ? 4.0 + 0.5 * splits * tiles * bn / (256.0 * kPairs) : 0.0;
-    return turns * (rate * steps / splits + tail) + join;
+// A product's cost in K steps of a 256-column tile (512 cycles, 0.3 us): the turns
+// that the pairs take, times the longer of a tile's K steps and its epilogue. Both were
+// measured: a step takes as long as its operands take to arrive, (128 + bn / 2) rows a
+// CTA, whatever the tensor cores need for a narrower tile (8192 x 4096 x 8192: 310 us
+// with 256 columns); an epilogue 0.054 steps a column and one more a tile (57600 x 128
+// -> 576: 36 us with 192 columns, 44 with 256). Shares of K are written and read once
+// more (6.5 TB/s), which fewer idle pairs have to earn back.
+double tile_cost(int tiles, int steps, int splits, int bn, double outputs) {
+    const double rate = (128 + bn / 2) / 256.0;
+    const long long turns = ((long long)tiles * splits + kPairs - 1) / kPairs;
+    const double main = rate * steps / splits, epilogue = 0.054 * bn + 1.0;
+    const double join = splits > 1 ? 7.0 + outputs * (6.0 * splits + 2.0) / 6.5e6 / 0.3 : 0.0;
+    return turns * (main > epilogue ? main : epilogue) + epilogue + join;
 }
 
 Plan plan_of(const GemmLaunch& L) {
@@ -109,7 +109,7 @@ Plan plan_of(const GemmLaunch& L) {
         if (bn == 192 && L.b_t) continue;
         const int tn = cdiv(L.N, L.gated ? bn / 2 : bn);
         for (int sp = 1; sp <= (plain ? 32 : 1) && (sp == 1 || steps / sp >= 8); sp *= 2) {
-            const double c = tile_cost(p.tiles_m * tn, steps, sp, bn);
+            const double c = tile_cost(p.tiles_m * tn, steps, sp, bn, (double)L.M * L.N);
             if (c < best * 0.999) {
                 best = c;
                 p.bn = bn;
@@ -296,11 +296,6 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     a.ldr = L.ldr, a.ldo = L.ldo, a.ldo2 = L.ldo2;
     a.rows0 = L.rows0, a.rows1 = L.rows1;
     a.out_type = L.out_type, a.act = L.act;
-    if (p.skinny) {
-        k.split = p.splits;
-        a.idesc = idesc_of(L.in_type, false, false, 128, p.tok);
-        return launch_skinny(p.tok, L.in_type == BVML_E4M3, L.gated, maps, k, s);
-    }
     // what the addresses and pitches that the epilogue touches have in common
     auto bits = [&](const void* ptr, long long ld) {
         return ptr ? reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)ld * eo : (uintptr_t)0;
@@ -314,6 +309,11 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     a.vec = ((all & 15) == 0 ? kOn16 : 0) | ((out & 31) == 0 ? kWideOut : 0) |
             ((save & 31) == 0 ? kWideSave : 0);
     const bool vec = (out & 15) == 0;
+    if (p.skinny) {
+        k.split = p.splits;
+        a.idesc = idesc_of(L.in_type, false, false, 128, p.tok);
+        return launch_skinny(p.tok, L.in_type == BVML_E4M3, L.gated, maps, k, s);
+    }
     a.idesc = idesc_of(L.in_type, L.a_t, L.b_t, 256, p.bn);
     if (p.splits > 1) {
         a.slab = reinterpret_cast<float*>(static_cast<char*>(ws) + p.slab);

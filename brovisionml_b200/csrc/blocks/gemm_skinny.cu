@@ -28,43 +28,130 @@ template <int TOK> constexpr int skinny_smem_bytes() {
     return 1024 + skinny_stages<TOK>() * skinny_stage_bytes<TOK>() + 256;
 }
 
+// What the epilogue of four neighbouring features of a token reads beside their
+// sums; asked for before the cluster meets, so that its latency passes meanwhile.
+struct Beside {
+    float rs, cs[4], cu[4], add[4], res[4];
+};
+template <bool GATED>
+__device__ __forceinline__ void ask_beside(const TileArgs& a, long long m, int n, Beside& o) {
+    if (a.col_scale[0]) o.rs = __ldg(a.row_scale + m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (n + e >= a.N) break;
+        if (a.col_scale[0]) {
+            o.cs[e] = __ldg(a.col_scale[0] + n + e);
+            if (GATED) o.cu[e] = __ldg(a.col_scale[1] + n + e);
+        }
+        if (!GATED && a.bias) o.add[e] = __ldg(a.bias + n + e);
+        if (!GATED && a.residual) o.res[e] = get_one(a.residual, m * a.ldr + n + e, a.out_type);
+    }
+}
+__device__ __forceinline__ void put_four(void* p, long long at, int type, const float (&v)[4],
+                                         int left, bool vec) {
+    if (vec && left >= 4) {
+        if (type == BVML_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p) + at) =
+                make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) =
+                type == BVML_BF16 ? make_uint2(pack2<__nv_bfloat16>(v[0], v[1]),
+                                               pack2<__nv_bfloat16>(v[2], v[3]))
+                                  : make_uint2(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) put_one(p, at + e, type, v[e]);
+    }
+}
+
 // This CTA's share of the features, summed over the cluster's SPLIT CTAs and
-// finished: four neighbouring features of a token a thread and turn, all the
-// shares' loads in flight at once.
+// finished: four neighbouring features of a token a thread, P tokens at a time, all
+// the shares' loads in flight at once. The cluster meets between asking for what
+// lies beside the first sums and reading them.
 template <int SPLIT, bool GATED>
 __device__ __forceinline__ void add_up(const TileArgs& a, uint32_t sbase, int rank, int f0, int t0,
                                        int tok) {
     constexpr int kShare = (GATED ? 64 : 128) / SPLIT;
     constexpr int kQuads = kShare / 4;
+    constexpr int P = SPLIT * (GATED ? 2 : 1) <= 4 ? 2 : 1;
     const int toks = a.M - t0 < tok ? a.M - t0 : tok;
+    const int items = kQuads * toks;
+    const bool vec = a.vec & kOn16;
+    Beside b[P];
+    auto ask = [&](int i0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int i = i0 + p * kSkinnyThreads;
+            if (i < items)
+                ask_beside<GATED>(a, t0 + i / kQuads, f0 + rank * kShare + i % kQuads * 4, b[p]);
+        }
+    };
+    ask(threadIdx.x);
+    tc::cluster_sync();
     uint32_t base[SPLIT];
 #pragma unroll
     for (int r = 0; r < SPLIT; ++r) base[r] = tc::map_to(sbase, r);
-    for (int i = threadIdx.x; i < kQuads * toks; i += kSkinnyThreads) {
-        const int f = rank * kShare + i % kQuads * 4, t = i / kQuads;
-        const uint32_t at = 4 * (t * kSkinnyPitch + f);
-        float4 p[SPLIT], q[SPLIT];
+    for (int i0 = threadIdx.x; i0 < items; i0 += P * kSkinnyThreads) {
+        if (i0 != (int)threadIdx.x) ask(i0);
+        float4 x[P][SPLIT], y[P][GATED ? SPLIT : 1];
 #pragma unroll
-        for (int r = 0; r < SPLIT; ++r) {
-            p[r] = tc::ld_cluster4(base[r] + at);
-            if constexpr (GATED) q[r] = tc::ld_cluster4(base[r] + at + 4 * 64);
+        for (int p = 0; p < P; ++p) {
+            // past the end: the first item's place again, not used
+            const int i = i0 + p * kSkinnyThreads < items ? i0 + p * kSkinnyThreads : i0;
+            const uint32_t at =
+                4 * (i / kQuads * kSkinnyPitch + rank * kShare + i % kQuads * 4);
+#pragma unroll
+            for (int r = 0; r < SPLIT; ++r) {
+                x[p][r] = tc::ld_cluster4(base[r] + at);
+                if constexpr (GATED) y[p][r] = tc::ld_cluster4(base[r] + at + 4 * 64);
+            }
         }
-        float v[4] = {p[0].x, p[0].y, p[0].z, p[0].w}, u[4];
-        if constexpr (GATED) u[0] = q[0].x, u[1] = q[0].y, u[2] = q[0].z, u[3] = q[0].w;
 #pragma unroll
-        for (int r = 1; r < SPLIT; ++r) {
-            v[0] += p[r].x, v[1] += p[r].y, v[2] += p[r].z, v[3] += p[r].w;
-            if constexpr (GATED) u[0] += q[r].x, u[1] += q[r].y, u[2] += q[r].z, u[3] += q[r].w;
+        for (int p = 0; p < P; ++p) {
+            const int i = i0 + p * kSkinnyThreads;
+            if (i >= items) break;
+            float v[4] = {x[p][0].x, x[p][0].y, x[p][0].z, x[p][0].w}, u[4] = {};
+#pragma unroll
+            for (int r = 1; r < SPLIT; ++r)
+                v[0] += x[p][r].x, v[1] += x[p][r].y, v[2] += x[p][r].z, v[3] += x[p][r].w;
+            if constexpr (GATED) {
+                u[0] = y[p][0].x, u[1] = y[p][0].y, u[2] = y[p][0].z, u[3] = y[p][0].w;
+#pragma unroll
+                for (int r = 1; r < SPLIT; ++r)
+                    u[0] += y[p][r].x, u[1] += y[p][r].y, u[2] += y[p][r].z, u[3] += y[p][r].w;
+            }
+            const long long m = t0 + i / kQuads;
+            const int n = f0 + rank * kShare + i % kQuads * 4, left = a.N - n;
+            if (left <= 0) continue;
+            if (a.col_scale[0]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] *= b[p].rs * b[p].cs[e];
+                    if (GATED) u[e] *= b[p].rs * b[p].cu[e];
+                }
+            }
+            if (!GATED && a.bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += b[p].add[e];
+            }
+            if (a.save[0]) {
+                put_four(a.save[0], m * a.lds[0] + n, a.out_type, v, left, vec);
+                if (GATED) put_four(a.save[1], m * a.lds[1] + n, a.out_type, u, left, vec);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = act_f(v[e], a.act);
+                if (GATED) v[e] *= u[e];
+                if (!GATED && a.residual) v[e] += b[p].res[e];
+            }
+            put_four(a.out, m * a.ldo + n, a.out_type, v, left, vec);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (f0 + f + e < a.N)
-                finish_one<GATED>(a, t0 + t, f0 + f + e, v[e], GATED ? u[e] : 0.0f);
     }
 }
 
 template <int TOK, bool F8, bool GATED>
-__global__ void __launch_bounds__(kSkinnyThreads)
+__global__ void __launch_bounds__(kSkinnyThreads, TOK <= 64 ? 3 : 2)  // what shared memory holds
 skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     constexpr int kStage = skinny_stage_bytes<TOK>();
     constexpr int kStages = skinny_stages<TOK>();
@@ -177,7 +264,6 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     __syncthreads();
     if (warp == 1) tc::tmem_dealloc(tmem, kCols);
     __syncwarp();
-    tc::cluster_sync();
     switch (split) {
         case 1: add_up<1, GATED>(a, sbase, rank, f0, t0, TOK); break;
         case 2: add_up<2, GATED>(a, sbase, rank, f0, t0, TOK); break;
