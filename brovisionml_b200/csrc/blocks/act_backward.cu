@@ -71,6 +71,7 @@ act_backward_kernel(const ActBackwardLaunch L, int span, bool vec_dy, bool vec_z
     __shared__ float sh[kThreads * 8];
     const int x = threadIdx.x % span, ry = threadIdx.x / span, rows = blockDim.x / span;
     const int c = (blockIdx.x * span + x) * 8;
+    begin();
     float sum[8] = {};
     const long long stride = (long long)gridDim.y * rows;
     if (c < L.N) {
@@ -145,6 +146,7 @@ gated_backward_kernel(const GatedBackwardLaunch L, int span, bool vec_h, bool ve
                       bool vec_d) {
     const int x = threadIdx.x % span, ry = threadIdx.x / span, rows = blockDim.x / span;
     const int c = (blockIdx.x * span + x) * 8;
+    begin();
     if (c >= L.F) return;
     const long long stride = (long long)gridDim.y * rows;
     // the next row's loads are in flight while this one is computed
@@ -208,10 +210,8 @@ cudaError_t launch_act_backward(const ActBackwardLaunch& L, cudaStream_t s) {
     const bool a = on16(L.dy, L.lddy, 2), b = L.z && on16(L.z, L.ldz, 2),
                c = L.dz && on16(L.dz, L.lddz, 2);
     if (L.type == BVML_F16)
-        act_backward_kernel<__half><<<grid, threads, 0, s>>>(L, span, a, b, c);
-    else
-        act_backward_kernel<__nv_bfloat16><<<grid, threads, 0, s>>>(L, span, a, b, c);
-    return cudaGetLastError();
+        return launch_pdl(act_backward_kernel<__half>, grid, threads, 0, s, true, L, span, a, b, c);
+    return launch_pdl(act_backward_kernel<__nv_bfloat16>, grid, threads, 0, s, true, L, span, a, b, c);
 }
 
 cudaError_t launch_gated_backward(const GatedBackwardLaunch& L, cudaStream_t s) {
@@ -222,10 +222,8 @@ cudaError_t launch_gated_backward(const GatedBackwardLaunch& L, cudaStream_t s) 
     const bool a = on16(L.dh, L.lddh, 2), b = on16(L.g, L.ldg, 2), c = on16(L.u, L.ldu, 2),
                d = on16(L.dg, L.ldd, 2) && on16(L.du, L.ldd, 2);
     if (L.type == BVML_F16)
-        gated_backward_kernel<__half><<<grid, threads, 0, s>>>(L, span, a, b, c, d);
-    else
-        gated_backward_kernel<__nv_bfloat16><<<grid, threads, 0, s>>>(L, span, a, b, c, d);
-    return cudaGetLastError();
+        return launch_pdl(gated_backward_kernel<__half>, grid, threads, 0, s, true, L, span, a, b, c, d);
+    return launch_pdl(gated_backward_kernel<__nv_bfloat16>, grid, threads, 0, s, true, L, span, a, b, c, d);
 }
 
 }  // namespace blocks

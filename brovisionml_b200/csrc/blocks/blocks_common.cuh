@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../bvml_common.cuh"
 #include "bvml_blocks.h"
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
@@ -16,6 +17,15 @@
 
 namespace bvml {
 namespace blocks {
+
+// Every kernel here is launched as a programmatic dependent of the one before it
+// in the stream (launch_pdl): it may be resident before that one has ended, so each
+// calls begin() before it touches global memory, once what its CTA holds on to
+// (TMEM) has been allocated; the next kernel may come then.
+__device__ __forceinline__ void begin() {
+    pdl_trigger();
+    pdl_wait();
+}
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }

@@ -137,6 +137,7 @@ pack_kernel(const T* __restrict__ src, long long ld, int rows, int cols, T* __re
             int units) {
     constexpr int kE = 16 / sizeof(T);
     const long long total = (long long)rows * units;
+    begin();
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
          i += (long long)gridDim.x * 256) {
         const long long r = i / units;
@@ -158,12 +159,12 @@ cudaError_t pack(const Stored& s, size_t es, void* ws, cudaStream_t st) {
     const int grid = (int)(want < 148 * 16 ? want : 148 * 16);
     void* d = static_cast<char*>(ws) + s.at;
     if (es == 1)
-        pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(s.p), s.ld, s.rows, s.cols,
-                                          static_cast<uint8_t*>(d), units);
-    else
-        pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(s.p), s.ld, s.rows, s.cols,
-                                          static_cast<uint16_t*>(d), units);
-    return cudaGetLastError();
+        return launch_pdl(pack_kernel<uint8_t>, grid, 256, 0, st, true,
+                          static_cast<const uint8_t*>(s.p), s.ld, s.rows, s.cols,
+                          static_cast<uint8_t*>(d), units);
+    return launch_pdl(pack_kernel<uint16_t>, grid, 256, 0, st, true,
+                      static_cast<const uint16_t*>(s.p), s.ld, s.rows, s.cols,
+                      static_cast<uint16_t*>(d), units);
 }
 
 // ------------------------------------------------------------ the shares' sum
@@ -174,6 +175,7 @@ join_kernel(const float* __restrict__ slab, long long stride, long long lds, int
             T* __restrict__ out, long long ldo, T* __restrict__ out2, long long ldo2, int rows0,
             int rows1, bool vec) {
     const long long m = blockIdx.x;
+    begin();
     T* o;
     if (!out2 || m < rows0) o = out + m * ldo;
     else if (m >= rows1) o = out2 + (m - rows1) * ldo2;
@@ -198,11 +200,10 @@ join_kernel(const float* __restrict__ slab, long long stride, long long lds, int
 
 template <typename T>
 cudaError_t join(const GemmLaunch& L, const Plan& p, const float* slab, bool vec, cudaStream_t s) {
-    const dim3 grid(L.M, cdiv(L.N, 256 * 8));
-    join_kernel<<<grid, 256, 0, s>>>(slab, (long long)L.M * p.ldslab, p.ldslab, p.splits, L.N,
-                                     static_cast<T*>(L.out), L.ldo, static_cast<T*>(L.out2),
-                                     L.ldo2, L.rows0, L.rows1, vec);
-    return cudaGetLastError();
+    const dim3 grid((unsigned)L.M, (unsigned)cdiv(L.N, 256 * 8));
+    return launch_pdl(join_kernel<T>, grid, 256, 0, s, true, slab, (long long)L.M * p.ldslab,
+                      p.ldslab, p.splits, L.N, static_cast<T*>(L.out), L.ldo,
+                      static_cast<T*>(L.out2), L.ldo2, L.rows0, L.rows1, vec);
 }
 
 // ------------------------------------------------------------------ tensor maps

@@ -192,6 +192,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
+    begin();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     auto fail = [&](int code) { atomicExch(&g_tile_error, code); };
@@ -286,13 +287,15 @@ cudaError_t launch_one(const TileMaps& m, const SkinnyArgs& a, cudaStream_t s) {
     cfg.blockDim = dim3(kSkinnyThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)a.split;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, m, a);
 }
 

@@ -304,6 +304,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     tc::tc_fence_before();
     __syncthreads();
     tc::cluster_sync();  // the peer's barriers exist before anything arrives on them
+    begin();
     tc::tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
@@ -506,8 +507,7 @@ cudaError_t launch_tile(const TileMaps& maps, const TileArgs& a, int pairs, cuda
     constexpr int smem = tile_smem_bytes<BN>();
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    kern<<<2 * pairs, kTileThreads, smem, s>>>(maps, a);
-    return cudaGetLastError();
+    return launch_pdl(kern, 2 * pairs, kTileThreads, smem, s, true, maps, a);
 }
 
 // Host reader of this translation unit's error word; resets it.

@@ -194,6 +194,7 @@ rms_norm_kernel(const NormArgs a) {
     constexpr int kRows = kThreads / G;
     __shared__ float slots[2][2][16];
     const int l = threadIdx.x % G, g = threadIdx.x / G;
+    begin();
     float w[VPT][8];
     if (a.w32) load_row<float, G, VPT>(static_cast<const float*>(a.w), a.K, a.vec, l, w);
     else load_row<T, G, VPT>(static_cast<const T*>(a.w), a.K, a.vec, l, w);
@@ -269,6 +270,7 @@ template <typename T, bool Q>
 __global__ void __launch_bounds__(kLongThreads)
 rms_norm_long_kernel(const NormArgs a) {
     __shared__ float slots[2][2][16];
+    begin();
     const float inv_k = 1.0f / (float)a.K;
     int slot = 0;
     auto wt = [&](int k) {
@@ -318,6 +320,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
     __shared__ float slots[2][2][16];
     __shared__ float part[kRows > 1 ? kThreads * VPT * 8 : 1];
     const int l = threadIdx.x % G, g = threadIdx.x / G;
+    begin();
     float w[VPT][8], dw[VPT][8];
     if (a.w32) load_row<float, G, VPT>(static_cast<const float*>(a.w), a.K, a.vec, l, w);
     else load_row<T, G, VPT>(static_cast<const T*>(a.w), a.K, a.vec, l, w);
@@ -405,6 +408,7 @@ template <typename T>
 __global__ void __launch_bounds__(kLongThreads)
 rms_norm_backward_long_kernel(const NormBwdArgs a) {
     __shared__ float slots[2][2][16];
+    begin();
     const float inv_k = 1.0f / (float)a.K;
     float* out = a.partial + (long long)blockIdx.x * a.K;
     auto wt = [&](int k) {
@@ -441,6 +445,7 @@ __global__ void __launch_bounds__(512)
 column_sum_kernel(const float* __restrict__ part, int rows, int cols, T* __restrict__ out) {
     __shared__ float sh[32][17];
     const int x = threadIdx.x % 16, c = blockIdx.x * 16 + x, r0 = threadIdx.x / 16;
+    begin();
     float v = 0.0f;
     if (c < cols) {
 #pragma unroll 8
@@ -490,37 +495,38 @@ int block_rows(Shape h) {
 }
 
 template <typename T, bool Q>
-void norm_by_shape(Shape h, int grid, const NormArgs& a, cudaStream_t s) {
+cudaError_t norm_by_shape(Shape h, int grid, const NormArgs& a, cudaStream_t s) {
     switch (h) {
-        case Shape::G8: rms_norm_kernel<T, 8, 1, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G16: rms_norm_kernel<T, 16, 1, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G32x1: rms_norm_kernel<T, 32, 1, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G32x2: rms_norm_kernel<T, 32, 2, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G128x1: rms_norm_kernel<T, 128, 1, Q><<<grid, 128, 0, s>>>(a); break;
-        case Shape::G256x1: rms_norm_kernel<T, 256, 1, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G256x2: rms_norm_kernel<T, 256, 2, Q><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G512x2: rms_norm_kernel<T, 512, 2, Q><<<grid, 512, 0, s>>>(a); break;
-        case Shape::G512x4: rms_norm_kernel<T, 512, 4, Q><<<grid, 512, 0, s>>>(a); break;
-        case Shape::Long: rms_norm_long_kernel<T, Q><<<grid, kLongThreads, 0, s>>>(a); break;
+        case Shape::G8: return launch_pdl(rms_norm_kernel<T, 8, 1, Q>, grid, 256, 0, s, true, a);
+        case Shape::G16: return launch_pdl(rms_norm_kernel<T, 16, 1, Q>, grid, 256, 0, s, true, a);
+        case Shape::G32x1: return launch_pdl(rms_norm_kernel<T, 32, 1, Q>, grid, 256, 0, s, true, a);
+        case Shape::G32x2: return launch_pdl(rms_norm_kernel<T, 32, 2, Q>, grid, 256, 0, s, true, a);
+        case Shape::G128x1: return launch_pdl(rms_norm_kernel<T, 128, 1, Q>, grid, 128, 0, s, true, a);
+        case Shape::G256x1: return launch_pdl(rms_norm_kernel<T, 256, 1, Q>, grid, 256, 0, s, true, a);
+        case Shape::G256x2: return launch_pdl(rms_norm_kernel<T, 256, 2, Q>, grid, 256, 0, s, true, a);
+        case Shape::G512x2: return launch_pdl(rms_norm_kernel<T, 512, 2, Q>, grid, 512, 0, s, true, a);
+        case Shape::G512x4: return launch_pdl(rms_norm_kernel<T, 512, 4, Q>, grid, 512, 0, s, true, a);
+        case Shape::Long: return launch_pdl(rms_norm_long_kernel<T, Q>, grid, kLongThreads, 0, s, true, a);
     }
+    return cudaErrorInvalidValue;
 }
 
 template <typename T>
-void norm_backward_by_shape(Shape h, int grid, const NormBwdArgs& a, cudaStream_t s) {
+cudaError_t norm_backward_by_shape(Shape h, int grid, const NormBwdArgs& a, cudaStream_t s) {
     switch (h) {
-        case Shape::G8: rms_norm_backward_kernel<T, 8, 1><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G16: rms_norm_backward_kernel<T, 16, 1><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G32x1: rms_norm_backward_kernel<T, 32, 1><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G32x2: rms_norm_backward_kernel<T, 32, 2><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G128x1: rms_norm_backward_kernel<T, 128, 1><<<grid, 128, 0, s>>>(a); break;
-        case Shape::G256x1: rms_norm_backward_kernel<T, 256, 1><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G256x2: rms_norm_backward_kernel<T, 256, 2><<<grid, 256, 0, s>>>(a); break;
-        case Shape::G512x2: rms_norm_backward_kernel<T, 512, 2><<<grid, 512, 0, s>>>(a); break;
-        case Shape::G512x4: rms_norm_backward_kernel<T, 512, 4><<<grid, 512, 0, s>>>(a); break;
+        case Shape::G8: return launch_pdl(rms_norm_backward_kernel<T, 8, 1>, grid, 256, 0, s, true, a);
+        case Shape::G16: return launch_pdl(rms_norm_backward_kernel<T, 16, 1>, grid, 256, 0, s, true, a);
+        case Shape::G32x1: return launch_pdl(rms_norm_backward_kernel<T, 32, 1>, grid, 256, 0, s, true, a);
+        case Shape::G32x2: return launch_pdl(rms_norm_backward_kernel<T, 32, 2>, grid, 256, 0, s, true, a);
+        case Shape::G128x1: return launch_pdl(rms_norm_backward_kernel<T, 128, 1>, grid, 128, 0, s, true, a);
+        case Shape::G256x1: return launch_pdl(rms_norm_backward_kernel<T, 256, 1>, grid, 256, 0, s, true, a);
+        case Shape::G256x2: return launch_pdl(rms_norm_backward_kernel<T, 256, 2>, grid, 256, 0, s, true, a);
+        case Shape::G512x2: return launch_pdl(rms_norm_backward_kernel<T, 512, 2>, grid, 512, 0, s, true, a);
+        case Shape::G512x4: return launch_pdl(rms_norm_backward_kernel<T, 512, 4>, grid, 512, 0, s, true, a);
         case Shape::Long:
-            rms_norm_backward_long_kernel<T><<<grid, kLongThreads, 0, s>>>(a);
-            break;
+            return launch_pdl(rms_norm_backward_long_kernel<T>, grid, kLongThreads, 0, s, true, a);
     }
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -553,16 +559,14 @@ cudaError_t launch_rms_norm(const NormLaunch& L, cudaStream_t s) {
     const int grid = (int)(want < most ? want : most);
     const bool q = L.scale != nullptr;
     if (L.type == BVML_F32) {
-        if (q) norm_by_shape<float, true>(h, grid, a, s);
-        else norm_by_shape<float, false>(h, grid, a, s);
+        return q ? norm_by_shape<float, true>(h, grid, a, s)
+                 : norm_by_shape<float, false>(h, grid, a, s);
     } else if (L.type == BVML_F16) {
-        if (q) norm_by_shape<__half, true>(h, grid, a, s);
-        else norm_by_shape<__half, false>(h, grid, a, s);
-    } else {
-        if (q) norm_by_shape<__nv_bfloat16, true>(h, grid, a, s);
-        else norm_by_shape<__nv_bfloat16, false>(h, grid, a, s);
+        return q ? norm_by_shape<__half, true>(h, grid, a, s)
+                 : norm_by_shape<__half, false>(h, grid, a, s);
     }
-    return cudaGetLastError();
+    return q ? norm_by_shape<__nv_bfloat16, true>(h, grid, a, s)
+             : norm_by_shape<__nv_bfloat16, false>(h, grid, a, s);
 }
 
 // Blocks of the backward pass, each with a row of partial sums: what 148 SMs hold
@@ -599,10 +603,10 @@ cudaError_t launch_rms_norm_backward(const NormBackwardLaunch& L, cudaStream_t s
         a.vec = L.K % 8 == 0 && on16(L.dy, L.lddy, es) && on16(L.s, L.lds, es) &&
                 (!L.ds || on16(L.ds, L.ldds, es)) && on16(L.w, 0, 1) && on16(L.dx, L.lddx, es);
         const Shape h = shape_of(L.K);
-        if (L.type == BVML_F32) norm_backward_by_shape<float>(h, parts, a, s);
-        else if (L.type == BVML_F16) norm_backward_by_shape<__half>(h, parts, a, s);
-        else norm_backward_by_shape<__nv_bfloat16>(h, parts, a, s);
-        cudaError_t e = cudaGetLastError();
+        const cudaError_t e = L.type == BVML_F32 ? norm_backward_by_shape<float>(h, parts, a, s)
+                              : L.type == BVML_F16
+                                  ? norm_backward_by_shape<__half>(h, parts, a, s)
+                                  : norm_backward_by_shape<__nv_bfloat16>(h, parts, a, s);
         if (e != cudaSuccess) return e;
     }
     return launch_column_sum(L.partial, parts, L.K, L.dw, L.wtype, s);
@@ -612,13 +616,13 @@ cudaError_t launch_column_sum(const float* part, int rows, int cols, void* out, 
                               cudaStream_t s) {
     const int grid = (cols + 15) / 16;
     if (type == BVML_F32)
-        column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols, static_cast<float*>(out));
-    else if (type == BVML_F16)
-        column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols, static_cast<__half*>(out));
-    else
-        column_sum_kernel<<<grid, 512, 0, s>>>(part, rows, cols,
-                                               static_cast<__nv_bfloat16*>(out));
-    return cudaGetLastError();
+        return launch_pdl(column_sum_kernel<float>, grid, 512, 0, s, true, part, rows, cols,
+                          static_cast<float*>(out));
+    if (type == BVML_F16)
+        return launch_pdl(column_sum_kernel<__half>, grid, 512, 0, s, true, part, rows, cols,
+                          static_cast<__half*>(out));
+    return launch_pdl(column_sum_kernel<__nv_bfloat16>, grid, 512, 0, s, true, part, rows, cols,
+                      static_cast<__nv_bfloat16*>(out));
 }
 
 }  // namespace blocks
