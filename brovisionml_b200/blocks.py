@@ -130,16 +130,21 @@ def _check(rc: int) -> None:
         raise RuntimeError(msg or f"dsine ops: failed with status {rc}")
 
 
-def _device(op: str, ts) -> torch.device:
-    dev = ts[0].device
+def _device(op: str, *ts) -> int:
+    """The index of the CUDA device that the tensors (or Nones) share."""
+    dev = ts[0].get_device()
     grad = torch.is_grad_enabled()
     for t in ts:
-        if t.device != dev:
+        if t is None:
+            continue
+        if t.get_device() != dev:
             raise _err(op, "all inputs must share a device")
         if grad and t.requires_grad:
             raise _err(op, "no autograd: pass detached tensors, or call under torch.no_grad() "
                            "(the gradients have functions of their own, *_backward)")
-    if dev.type != "cuda":
+    if dev < 0 or not ts[0].is_cuda:
+        if any(t is not None and t.device != ts[0].device for t in ts):
+            raise _err(op, "all inputs must share a device")
         raise _err(op, "tensors must be CUDA-resident (this library has no CPU path)")
     return dev
 
@@ -177,19 +182,21 @@ def _rows(op: str, t: torch.Tensor, name: str, cols: int | None = None, rows: in
                 raise _err(op, f"{name}'s leading axes must be evenly spaced rows") from None
         shape = t.shape
     T, K = shape
-    s0, s1 = t.stride()
-    if K > 1 and s1 != 1:
-        raise _err(op, f"{name}'s last axis must be contiguous")
     if cols is not None and K != cols:
         raise _err(op, f"{name} has {K} columns, expected {cols}")
     if rows is not None and T != rows:
         raise _err(op, f"{name} has {T} rows, expected {rows}")
     if dtype is not None and t.dtype != dtype:
         raise _err(op, f"{name} must be {dtype}, is {t.dtype}")
-    if T > 1 and s0 < K:
-        raise _err(op, f"{name}'s rows overlap")
     if T > 0x7fffffff or K > 0x7fffffff:
         raise _err(op, f"{name} is too large")
+    if t.is_contiguous():
+        return t.data_ptr(), K, T, K
+    s0, s1 = t.stride()
+    if K > 1 and s1 != 1:
+        raise _err(op, f"{name}'s last axis must be contiguous")
+    if T > 1 and s0 < K:
+        raise _err(op, f"{name}'s rows overlap")
     return t.data_ptr(), (s0 if T > 1 else K), T, K
 
 
@@ -199,7 +206,7 @@ def _vec(op: str, t: torch.Tensor | None, name: str, n: int, dtype: torch.dtype 
         return None
     if t.dtype != dtype:
         raise _err(op, f"{name} must be {dtype}, is {t.dtype}")
-    if t.dim() != 1 and t.numel() != n or t.numel() != n:
+    if t.numel() != n:
         raise _err(op, f"{name} has {t.numel()} values, expected {n}")
     if not t.is_contiguous():
         raise _err(op, f"{name} must be contiguous")
@@ -211,37 +218,28 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class _On:
-    """Makes `dev` the current device for a launch, when it is not."""
-    __slots__ = ("guard",)
-
-    def __init__(self, dev: torch.device):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_current_device = torch.cuda.current_device
 
 
-def _run(fn, ws_fn, args, dev: torch.device, need: int | None = None) -> None:
-    """fn(args) with a workspace where it wants one: `need` bytes, or, when
-    not known, asked for only if the call without one is turned down (the common
-    call needs none)."""
+def _call(dev: int, fn, *args) -> int:
+    """fn(*args, stream) with `dev` as the current device and its current stream."""
+    if _current_device() == dev:
+        return fn(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev))
+
+
+def _run(fn, ws_fn, args, dev: int) -> None:
+    """fn(args), with a workspace only where the call without one is turned
+    down (the common call needs none)."""
     p = ctypes.byref(args)
-    with _On(dev):
-        stream = _raw_stream(dev.index)
-        if need is None:
-            rc = fn(p, None, 0, stream)
-            if rc != BVML_EWORKSPACE:
-                _check(rc)
-                return
-            need = ws_fn(p)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _check(fn(p, None if ws is None else ws.data_ptr(), need, stream))
+    rc = _call(dev, fn, p, None, 0)
+    if rc == BVML_EWORKSPACE:
+        need = ws_fn(p)
+        ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
+        rc = _call(dev, fn, p, ws.data_ptr(), need)
+    if rc:
+        _check(rc)
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
@@ -250,26 +248,27 @@ def _like(t: torch.Tensor) -> torch.Tensor:
         torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _new(rows_of: torch.Tensor, cols: int, dtype: torch.dtype, dev: torch.device):
-    return torch.empty((*rows_of.shape[:-1], cols), dtype=dtype, device=dev)
+def _new(t: torch.Tensor, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised tensor of t's rows, `cols` columns."""
+    return torch.empty((*t.shape[:-1], cols), dtype=dtype, device=t.device)
 
 
 # ----------------------------------------------------------------------- norm
 
 
 def _norm_inputs(op, x, weight, residual):
-    dev = _device(op, (x, weight) if residual is None else (x, weight, residual))
+    dev = _device(op, x, weight, residual)
     px, ldx, T, K = _rows(op, x, "x")
-    ty = _type(op, x.dtype)
-    if weight.dtype not in (x.dtype, _F32):
-        raise _err(op, f"weight must be float32 or {x.dtype}, is {weight.dtype}")
-    pw = _vec(op, weight, "weight", K, weight.dtype)
+    dt, wt = x.dtype, weight.dtype
+    if wt != dt and wt != _F32:
+        raise _err(op, f"weight must be float32 or {dt}, is {wt}")
+    pw = _vec(op, weight, "weight", K, wt)
     pr, ldr = None, 0
     if residual is not None:
         if residual.shape != x.shape:
             raise _err(op, "residual must have x's shape")
-        pr, ldr, _, _ = _rows(op, residual, "residual", K, T, x.dtype)
-    return dev, px, ldx, T, K, ty, _TYPES[weight.dtype], pw, pr, ldr
+        pr, ldr, _, _ = _rows(op, residual, "residual", K, T, dt)
+    return dev, px, ldx, T, K, _type(op, dt), _TYPES[wt], pw, pr, ldr
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -278,15 +277,19 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     x and residual (..., K) fp32, fp16 or bf16; weight (K) of that type or
     fp32. Returns y, or with a residual (y, s), both of x's type; the norm
     is taken of the unrounded sum."""
-    op = "rms_norm"
-    dev, px, ldx, T, K, ty, wt, pw, pr, ldr = _norm_inputs(op, x, weight, residual)
+    dev, px, ldx, T, K, ty, wt, pw, pr, ldr = _norm_inputs("rms_norm", x, weight, residual)
     y = _like(x)
-    s = _like(x) if residual is not None else None
-    with _On(dev):
-        _check(_norm(px, ldx, pr, ldr, pw, T, K, ty, wt, eps, y.data_ptr(), K,
-                     None if s is None else s.data_ptr(), K,
-                     _raw_stream(dev.index)))
-    return y if s is None else (y, s)
+    if residual is None:
+        rc = _call(dev, _norm, px, ldx, None, 0, pw, T, K, ty, wt, eps, y.data_ptr(), K, None, K)
+        if rc:
+            _check(rc)
+        return y
+    s = _like(x)
+    rc = _call(dev, _norm, px, ldx, pr, ldr, pw, T, K, ty, wt, eps, y.data_ptr(), K, s.data_ptr(),
+               K)
+    if rc:
+        _check(rc)
+    return y, s
 
 
 def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
@@ -295,15 +298,14 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     (q, scale) or, with a residual, (q, scale, s); q (..., K) float8_e4m3fn, scale (...)
     fp32, y ~ q * scale[..., None]. The row's largest magnitude becomes 448
     (scale 1 for a row of zeros; a row with NaN or infinities has a NaN scale)."""
-    op = "rms_norm_e4m3"
-    dev, px, ldx, T, K, ty, wt, pw, pr, ldr = _norm_inputs(op, x, weight, residual)
-    q = torch.empty(x.shape, dtype=_E4M3, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=_F32, device=dev)
+    dev, px, ldx, T, K, ty, wt, pw, pr, ldr = _norm_inputs("rms_norm_e4m3", x, weight, residual)
+    q = torch.empty(x.shape, dtype=_E4M3, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=_F32, device=x.device)
     s = _like(x) if residual is not None else None
-    with _On(dev):
-        _check(_norm_e4m3(px, ldx, pr, ldr, pw, T, K, ty, wt, eps, q.data_ptr(), K,
-                          scale.data_ptr(), None if s is None else s.data_ptr(), K,
-                          _raw_stream(dev.index)))
+    rc = _call(dev, _norm_e4m3, px, ldx, pr, ldr, pw, T, K, ty, wt, eps, q.data_ptr(), K,
+               scale.data_ptr(), None if s is None else s.data_ptr(), K)
+    if rc:
+        _check(rc)
     return (q, scale) if s is None else (q, scale, s)
 
 
@@ -313,26 +315,25 @@ def rms_norm_backward(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor,
     without a residual), dsum the gradient of that sum where it went on as
     the residual stream. dx is the gradient of x and of the residual alike."""
     op = "rms_norm_backward"
-    dev = _device(op, (dy, s, weight) if dsum is None else (dy, s, weight, dsum))
+    dev = _device(op, dy, s, weight, dsum)
     if dy.shape != s.shape or dsum is not None and dsum.shape != s.shape:
         raise _err(op, "dy, s and dsum must have one shape")
     ps, lds, T, K = _rows(op, s, "s")
-    pd, ldd, _, _ = _rows(op, dy, "dy", K, T, s.dtype)
-    if weight.dtype not in (s.dtype, _F32):
-        raise _err(op, f"weight must be float32 or {s.dtype}, is {weight.dtype}")
-    pw = _vec(op, weight, "weight", K, weight.dtype)
+    dt, wt = s.dtype, weight.dtype
+    pd, ldd, _, _ = _rows(op, dy, "dy", K, T, dt)
+    if wt != dt and wt != _F32:
+        raise _err(op, f"weight must be float32 or {dt}, is {wt}")
+    pw = _vec(op, weight, "weight", K, wt)
     pr, ldr = None, 0
     if dsum is not None:
-        pr, ldr, _, _ = _rows(op, dsum, "dsum", K, T, s.dtype)
-    ty = _type(op, s.dtype)
+        pr, ldr, _, _ = _rows(op, dsum, "dsum", K, T, dt)
+    ty = _type(op, dt)
     dx = _like(s)
-    dw = torch.empty((K,), dtype=weight.dtype, device=dev)
+    dw = torch.empty((K,), dtype=wt, device=s.device)
     need = _norm_bwd_ws(T, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _On(dev):
-        _check(_norm_bwd(pd, ldd, ps, lds, pw, pr, ldr, T, K, ty, _TYPES[weight.dtype], eps,
-                         dx.data_ptr(), K, dw.data_ptr(), ws.data_ptr(), need,
-                         _raw_stream(dev.index)))
+    ws = torch.empty(need, dtype=torch.uint8, device=s.device)
+    _check(_call(dev, _norm_bwd, pd, ldd, ps, lds, pw, pr, ldr, T, K, ty, _TYPES[wt], eps,
+                 dx.data_ptr(), K, dw.data_ptr(), ws.data_ptr(), need))
     return dx, dw
 
 
@@ -369,8 +370,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     otherwise. act: none, relu, sigmoid, tanh, silu, gelu (erf form). Returns
     y (..., N), with save=True (y, z), z the pre-activation for linear_backward."""
     op = "linear"
-    ts = [t for t in (x, weight, bias, residual, x_scale, w_scale) if t is not None]
-    dev = _device(op, ts)
+    dev = _device(op, x, weight, bias, residual, x_scale, w_scale)
     px, ldx, T, K = _rows(op, x, "x")
     pw, ldw, N, _ = _rows(op, weight, "weight", K, None, x.dtype)
     od = _out_type(op, x.dtype, out_dtype, (x_scale, w_scale))
@@ -380,8 +380,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         if residual.shape[:-1] != x.shape[:-1]:
             raise _err(op, "residual must have the output's shape")
         pr, ldr, _, _ = _rows(op, residual, "residual", N, T, od)
-    y = _new(x, N, od, dev)
-    z = _new(x, N, od, dev) if save else None
+    y = _new(x, N, od)
+    z = _new(x, N, od) if save else None
     a = LinearArgs(px, pw, _vec(op, x_scale, "x_scale", T), _vec(op, w_scale, "w_scale", N),
                    _vec(op, bias, "bias", N), pr, y.data_ptr(), None if z is None else z.data_ptr(),
                    ldx, ldw, ldr, N, N, T, K, N, ty, to, _act(op, act))
@@ -397,7 +397,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     returned (None without an activation). dbias is fp32, None unless ``bias``; dx=False
     or dw=False leave that gradient out (None). The residual's gradient is dy."""
     op = "linear_backward"
-    dev = _device(op, (dy, x, weight) if z is None else (dy, x, weight, z))
+    dev = _device(op, dy, x, weight, z)
     px, ldx, T, K = _rows(op, x, "x")
     pw, ldw, N, _ = _rows(op, weight, "weight", K, None, x.dtype)
     if dy.shape[:-1] != x.shape[:-1]:
@@ -412,8 +412,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
             raise _err(op, "z must have dy's shape")
         pz, ldz, _, _ = _rows(op, z, "z", N, T, x.dtype)
     gx = _like(x) if dx else None
-    gw = torch.empty((N, K), dtype=x.dtype, device=dev) if dw else None
-    gb = torch.empty((N,), dtype=_F32, device=dev) if bias else None
+    gw = torch.empty((N, K), dtype=x.dtype, device=x.device) if dw else None
+    gb = torch.empty((N,), dtype=_F32, device=x.device) if bias else None
     a = LinearBackwardArgs(pd, pz, px, pw, None if gx is None else gx.data_ptr(),
                            None if gw is None else gw.data_ptr(),
                            None if gb is None else gb.data_ptr(), ldd, ldz, ldx, ldw, K, K,
@@ -430,15 +430,14 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *,
     (F, K); types and scales as ``linear``. Returns h (..., F), with save=True
     (h, g, u), g and u the two projections for gated_linear_backward."""
     op = "gated_linear"
-    ts = [t for t in (x, w_gate, w_up, x_scale, gate_scale, up_scale) if t is not None]
-    dev = _device(op, ts)
+    dev = _device(op, x, w_gate, w_up, x_scale, gate_scale, up_scale)
     px, ldx, T, K = _rows(op, x, "x")
     pg, ldg, F, _ = _rows(op, w_gate, "w_gate", K, None, x.dtype)
     pu, ldu, _, _ = _rows(op, w_up, "w_up", K, F, x.dtype)
     od = _out_type(op, x.dtype, out_dtype, (x_scale, gate_scale, up_scale))
     ty, to = _type(op, x.dtype), _type(op, od)
-    h = _new(x, F, od, dev)
-    g, u = (_new(x, F, od, dev), _new(x, F, od, dev)) if save else (None, None)
+    h = _new(x, F, od)
+    g, u = (_new(x, F, od), _new(x, F, od)) if save else (None, None)
     a = GatedArgs(px, pg, pu, _vec(op, x_scale, "x_scale", T),
                   _vec(op, gate_scale, "gate_scale", F), _vec(op, up_scale, "up_scale", F),
                   h.data_ptr(), None if g is None else g.data_ptr(),
@@ -455,7 +454,7 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
     (..., F) are what gated_linear(save=True) returned. dx=False or dw=False
     leave gradients out (None)."""
     op = "gated_linear_backward"
-    dev = _device(op, (dh, x, w_gate, w_up, g, u))
+    dev = _device(op, dh, x, w_gate, w_up, g, u)
     px, ldx, T, K = _rows(op, x, "x")
     pg, ldg, F, _ = _rows(op, w_gate, "w_gate", K, None, x.dtype)
     pu, ldu, _, _ = _rows(op, w_up, "w_up", K, F, x.dtype)
@@ -465,7 +464,7 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
     pgv, ldgv, _, _ = _rows(op, g, "g", F, T, x.dtype)
     puv, lduv, _, _ = _rows(op, u, "u", F, T, x.dtype)
     gx = _like(x) if dx else None
-    gg, gu = (torch.empty((F, K), dtype=x.dtype, device=dev) for _ in range(2)) if dw \
+    gg, gu = (torch.empty((F, K), dtype=x.dtype, device=x.device) for _ in range(2)) if dw \
         else (None, None)
     a = GatedBackwardArgs(pd, pgv, puv, px, pg, pu, None if gx is None else gx.data_ptr(),
                           None if gg is None else gg.data_ptr(),

@@ -213,6 +213,10 @@ const char* forward_types(int in_type, int out_type, const void* xs, const void*
     return nullptr;
 }
 
+// 16-bit columns in whole 128-byte lines: a copy of the products' operands then
+// touches one line a row and K step and not two.
+long long whole_lines(int cols) { return ((long long)cols + 63) / 64 * 64; }
+
 // linear_backward's workspace: dz (unless it is dy), the bias gradient's
 // partial sums, the products' scratch.
 struct LinearBackwardPlan {
@@ -224,7 +228,7 @@ LinearBackwardPlan plan_of(const bvml_linear_backward_args& a, GemmLaunch* gx, G
                            void* ws) {
     LinearBackwardPlan p;
     p.own_dz = a.act != BVML_ACT_NONE;
-    p.lddz = p.own_dz ? ((long long)a.N + 7) / 8 * 8 : a.lddy;
+    p.lddz = p.own_dz ? whole_lines(a.N) : a.lddy;
     const bool products = a.dx || a.dw;
     p.partial = p.own_dz && products ? round256((size_t)a.T * p.lddz * 2) : 0;
     p.gemm = p.partial + (a.dbias ? round256((size_t)act_backward_parts(a.T, a.N) * a.N * 4) : 0);
@@ -250,7 +254,7 @@ struct GatedBackwardPlan {
 GatedBackwardPlan plan_of(const bvml_gated_backward_args& a, GemmLaunch* gx, GemmLaunch* gw,
                           void* ws) {
     GatedBackwardPlan p;
-    p.fp = (a.F + 7) / 8 * 8;
+    p.fp = (int)whole_lines(a.F);
     p.gemm = round256((size_t)a.T * 2 * p.fp * 2);
     void* d = ws ? ws : reinterpret_cast<void*>(256);
     void* du = at(d, (size_t)p.fp * 2);
@@ -344,7 +348,7 @@ int check_linear_backward(const bvml_linear_backward_args* a) {
 int check_gated_backward(const bvml_gated_backward_args* a) {
     const char* op = "gated_linear_backward";
     if (!a) return einval(op, "no arguments");
-    if (a->T < 0 || a->K < 1 || a->F < 1 || a->F > (1 << 30) - 8) return einval(op, "bad shape");
+    if (a->T < 0 || a->K < 1 || a->F < 1 || a->F > (1 << 30) - 64) return einval(op, "bad shape");
     if (!type16(a->type)) return einval(op, "matrices must be fp16 or bf16");
     if (!act_ok(a->act) || a->act == BVML_ACT_NONE) return einval(op, "unknown activation");
     if (!a->dw_gate != !a->dw_up) return einval(op, "dw_gate and dw_up are computed together");

@@ -72,7 +72,8 @@ Plan plan_of(const GemmLaunch& L) {
         if (rows == 1) s.ld = cols;  // one row has no pitch
         // (one row's pitch is made up where the tensor map is)
         s.pack = rows == 1 ? (reinterpret_cast<uintptr_t>(ptr) & 15) != 0 : !on16(ptr, ld, es);
-        s.ld_packed = ((long long)cols * (long long)es + 15) / 16 * 16 / (long long)es;
+        // whole 128-byte lines: a K step of a row then lies in one
+        s.ld_packed = ((long long)cols * (long long)es + 127) / 128 * 128 / (long long)es;
         if (s.pack) {
             s.at = off;
             off += round256((size_t)rows * s.ld_packed * es);
