@@ -106,8 +106,8 @@ Plan plan_of(const GemmLaunch& L) {
     const bool plain = !L.gated && !L.bias && !L.residual && !L.save[0] && !L.row_scale &&
                        L.act == BVML_ACT_NONE;
     double best = 1e300;
-    for (int bn = 256; bn >= (L.b_t ? 128 : 64); bn -= 64) {
-        if (bn == 192 && L.b_t) continue;
+    const bool halves = L.gated || L.b_t;  // 256 and 128 columns only
+    for (int bn = 256; bn >= (halves ? 128 : 64); bn -= halves ? 128 : 64) {
         const int tn = cdiv(L.N, L.gated ? bn / 2 : bn);
         for (int sp = 1; sp <= (plain ? 32 : 1) && (sp == 1 || steps / sp >= 8); sp *= 2) {
             const double c = tile_cost(p.tiles_m * tn, steps, sp, bn, (double)L.M * L.N);
@@ -226,25 +226,29 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 }
 
 // Boxes of 128 bytes x box_rows in the 128-byte swizzle; what lies outside the
-// matrix reads zeros.
-cudaError_t encode(CUtensorMap* m, const Stored& s, const void* ws, int type, int box_rows) {
+// matrix reads zeros, and is not written.
+cudaError_t encode_rows(CUtensorMap* m, const void* base, long long ld, int rows, int cols,
+                        int type, int box_rows) {
     PFN_cuTensorMapEncodeTiled_v12000 fn = encoder();
     if (!fn) return cudaErrorNotSupported;
     const size_t es = elem_size(type);
-    const void* base = s.pack ? static_cast<const char*>(ws) + s.at : s.p;
-    const long long ld = s.pack || s.rows == 1 ? s.ld_packed : s.ld;
-    const cuuint64_t dims[2] = {(cuuint64_t)s.cols, (cuuint64_t)s.rows};
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * es};
     const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
     const cuuint32_t es1[2] = {1, 1};
     const CUtensorMapDataType dt = type == BVML_E4M3   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : type == BVML_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+                                   : type == BVML_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     return fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, es1,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? cudaSuccess
                : cudaErrorInvalidValue;
+}
+cudaError_t encode(CUtensorMap* m, const Stored& s, const void* ws, int type, int box_rows) {
+    return encode_rows(m, s.pack ? static_cast<const char*>(ws) + s.at : s.p,
+                       s.pack || s.rows == 1 ? s.ld_packed : s.ld, s.rows, s.cols, type, box_rows);
 }
 
 // MMA instruction descriptor: fp32 D; A and B bf16 (1), f16 or e4m3 (0);
@@ -304,12 +308,12 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     };
     const uintptr_t out = bits(L.out, L.ldo) | bits(L.out2, L.ldo2);
     const uintptr_t save = bits(L.save[0], L.lds[0]) | bits(L.save[1], L.lds[1]);
-    const uintptr_t all = out | save | bits(L.residual, L.ldr) |
+    // (a TMA store's right edge is cut in units of 16 bytes: N counts too)
+    const uintptr_t all = out | save | (uintptr_t)L.N * eo | bits(L.residual, L.ldr) |
                           reinterpret_cast<uintptr_t>(L.bias) |
                           reinterpret_cast<uintptr_t>(L.col_scale[0]) |
                           reinterpret_cast<uintptr_t>(L.col_scale[1]);
-    a.vec = ((all & 15) == 0 ? kOn16 : 0) | ((out & 31) == 0 ? kWideOut : 0) |
-            ((save & 31) == 0 ? kWideSave : 0);
+    a.vec = ((all & 15) == 0 ? kOn16 : 0) | ((save & 31) == 0 ? kWideSave : 0);
     const bool vec = (out & 15) == 0;
     if (p.skinny) {
         k.split = p.splits;
@@ -317,6 +321,14 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
         return launch_skinny(p.tok, L.in_type == BVML_E4M3, L.gated, maps, k, s);
     }
     a.idesc = idesc_of(L.in_type, L.a_t, L.b_t, 256, p.bn);
+    a.out_rows = L.out2 ? L.rows0 : L.M;
+    if ((a.vec & kOn16) && p.splits == 1) {  // one row's pitch is any multiple of 16 bytes
+        auto pitch = [&](long long ld) { return a.out_rows > 1 ? ld : ((L.N + 7LL) / 8 * 8); };
+        e = encode_rows(&maps.o[0], L.out, pitch(L.ldo), a.out_rows, L.N, L.out_type, 32);
+        if (e == cudaSuccess && L.out2)
+            e = encode_rows(&maps.o[1], L.out2, pitch(L.ldo2), a.out_rows, L.N, L.out_type, 32);
+        if (e != cudaSuccess) return e;
+    }
     if (p.splits > 1) {
         a.slab = reinterpret_cast<float*>(static_cast<char*>(ws) + p.slab);
         a.ldslab = p.ldslab;

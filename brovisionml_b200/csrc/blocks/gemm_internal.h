@@ -11,6 +11,7 @@ namespace blocks {
 struct TileMaps {
     CUtensorMap a[2];  // one a segment
     CUtensorMap b[2];  // one a segment, or gate and up
+    CUtensorMap o[2];  // out, out2: boxes of 32 rows x 128 bytes
 };
 
 // Division of n < 2^31 by d >= 2: n / d = (n mul >> 32) >> shift with 2^shift < d <=
@@ -30,9 +31,9 @@ inline Division divide_by(uint32_t d) {
 
 // TileArgs::vec
 enum : int {
-    kOn16 = 1,     // every row of 32 columns and every vector over columns starts on 16 bytes
-    kWideOut = 2,  // the outputs' (out and out2) on 32
-    kWideSave = 4  // save's on 32
+    kOn16 = 1,     // every row, and every vector over columns, starts on 16 bytes, and an
+                   // output's row ends there
+    kWideSave = 2  // save's on 32
 };
 
 struct TileArgs {
@@ -52,12 +53,13 @@ struct TileArgs {
     void* save[2];
     long long ldr, ldo, ldo2, lds[2];
     int rows0, rows1;
+    int out_rows;  // rows of out, and of out2 where there is one
     int out_type, act, vec;
     float* slab;  // splits > 1: (splits, M, ldslab) fp32 partial sums
     long long ldslab;
 };
 
-// bn: the pair's columns (256, 128, 64, 192; transposed B: 256 or 128)
+// bn: the pair's columns (256, 192, 128 or 64; gated or with B transposed: 256 or 128)
 cudaError_t launch_tile_nt(int bn, bool gated, const TileMaps& m, const TileArgs& a, int pairs,
                            cudaStream_t s);
 cudaError_t launch_tile_nt_f8(int bn, bool gated, const TileMaps& m, const TileArgs& a, int pairs,

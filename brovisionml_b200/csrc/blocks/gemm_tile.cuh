@@ -16,8 +16,8 @@
 //    of both CTAs are counted on the first CTA's barrier;
 //  * warp 1 of the first CTA issues the MMAs of the pair, and hands ring entries
 //    back to both producers by multicast commits;
-//  * warps 2-9 drain one of two accumulators in TMEM while the other fills, 32
-//    columns of a row a lane.
+//  * warps 2-9 drain one of two accumulators in TMEM while the other fills, 16
+//    columns of a row a lane at a time, and store 32 rows x 128 bytes by TMA.
 //
 // Operands come in row-major order for the forward pass; the backward pass reads
 // the same tensors with the contracted axis outermost (AT, BT) without a
@@ -51,62 +51,87 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, Division d) {
 
 // bytes of one ring entry: 128 rows of A, BN / 2 of B, 128 bytes each
 template <int BN> constexpr int tile_stage_bytes() { return (128 + BN / 2) * 128; }
+// staging of outputs: 32 rows x 128 bytes a warp, two of them where the ring leaves room
+template <int BN> constexpr int tile_buffers() { return BN == 256 ? 1 : 2; }
+template <int BN> constexpr int tile_staging_bytes() {
+    return kTileEpiWarps * 4096 * tile_buffers<BN>();
+}
 template <int BN> constexpr int tile_stages() {
-    constexpr int n = (kTileSmem - 1024 - kTileBarBytes) / tile_stage_bytes<BN>();
+    constexpr int n = (kTileSmem - 1024 - kTileBarBytes - tile_staging_bytes<BN>()) /
+                      tile_stage_bytes<BN>();
     return n < kTileMaxStages ? n : kTileMaxStages;
 }
 template <int BN> constexpr int tile_smem_bytes() {
-    return 1024 + kTileBarBytes + tile_stages<BN>() * tile_stage_bytes<BN>();
+    return 1024 + kTileBarBytes + tile_staging_bytes<BN>() +
+           tile_stages<BN>() * tile_stage_bytes<BN>();
 }
 
-// A lane finishes 32 consecutive columns of one row, as they lie in TMEM: 64
-// or 128 bytes, in 32-byte stores where the rows start on 32 bytes, so that every
-// sector is touched once. No staging through shared memory.
+// A lane finishes kW consecutive columns of one row at a time, as they lie in TMEM. The
+// output goes through shared memory: a warp's 32 rows x 128 bytes in the 128-byte
+// swizzle, written to global memory by one TMA store, whole lines at a time and
+// clipped at the edges (stores from registers, 32 bytes of 32 rows each, kept 16 warps
+// waiting 15 us of 44 on 57600 x 128 -> 576, and 8 warps 3 of 34). What a launch's
+// kernel cannot meet is left out at compile time and what is rare stands out of line:
+// a short K's epilogue is long beside its MMAs.
+constexpr int kW = 16;
+
+template <int OUT> struct OutOf;
+template <> struct OutOf<BVML_F32> { using T = float; };
+template <> struct OutOf<BVML_F16> { using T = __half; };
+template <> struct OutOf<BVML_BF16> { using T = __nv_bfloat16; };
+
 __device__ __forceinline__ void st32(void* p, const uint32_t* w) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
                  "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
 }
-template <int WORDS>
-__device__ __forceinline__ void st_words(void* p, const uint32_t (&w)[WORDS], bool wide) {
-    if (wide) {
+// kW columns to rows that start on 16 bytes (wide: on 32).
+template <typename T>
+__device__ __forceinline__ void put_row(T* p, const float (&v)[kW], bool wide) {
+    constexpr int kWords = kW * sizeof(T) / 4;
+    uint32_t w[kWords];
 #pragma unroll
-        for (int i = 0; i < WORDS / 8; ++i) st32(static_cast<uint32_t*>(p) + 8 * i, w + 8 * i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < WORDS / 4; ++i)
-            static_cast<uint4*>(p)[i] =
-                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    for (int i = 0; i < kWords; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+        else w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
     }
-}
-// 32 columns to rows that start on 16 bytes (wide: on 32).
-__device__ __forceinline__ void put_row(void* base, long long at, int type, const float (&v)[32],
-                                        bool wide) {
-    if (type == BVML_F32) {
-        uint32_t w[32];
+    if (__builtin_expect(wide, 1)) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
-        st_words(static_cast<float*>(base) + at, w, wide);
+        for (int i = 0; i < kWords; i += 8) st32(reinterpret_cast<uint32_t*>(p) + i, w + i);
     } else {
-        uint32_t w[16];
-        if (type == BVML_BF16) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack2<__nv_bfloat16>(v[2 * i], v[2 * i + 1]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack2<__half>(v[2 * i], v[2 * i + 1]);
-        }
-        st_words(static_cast<uint16_t*>(base) + at, w, wide);
+        for (int i = 0; i < kWords; i += 4)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) =
+                make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
     }
 }
 
-__device__ __forceinline__ void act_row(float (&v)[32], int act) {
+// ... to row r of a warp's staging buffer: 16-byte unit q of the row at q ^ (r & 7),
+// so that eight lanes' writes hit all banks once. c: the chunk's place in the row.
+template <typename T>
+__device__ __forceinline__ void stage_row(uint8_t* buf, int r, int c, const float (&v)[kW]) {
+    constexpr int kUnits = kW * sizeof(T) / 16;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        uint4 w;
+        if constexpr (sizeof(T) == 4)
+            w = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                           __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+        else
+            w = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                           pack2<T>(v[8 * i + 4], v[8 * i + 5]),
+                           pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+        *reinterpret_cast<uint4*>(buf + r * 128 + (((c * kUnits + i) ^ (r & 7)) << 4)) = w;
+    }
+}
+
+__device__ __forceinline__ void act_row(float (&v)[kW], int act) {
     if (act == BVML_ACT_NONE) return;
     // the switch outside the loop: the activation is the same for the whole launch
     switch (act) {
 #define BVML_ACT_ROW(code)                                                  \
     case code:                                                              \
-        _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = act_f(v[i], code); \
+        _Pragma("unroll") for (int i = 0; i < kW; ++i) v[i] = act_f(v[i], code); \
         break;
         BVML_ACT_ROW(BVML_ACT_RELU)
         BVML_ACT_ROW(BVML_ACT_SIGMOID)
@@ -118,20 +143,40 @@ __device__ __forceinline__ void act_row(float (&v)[32], int act) {
     }
 }
 
-// v[i] = v[i] * s * p[i], or v[i] + p[i], for a vector over columns on 16 bytes
-__device__ __forceinline__ void scale_cols(float (&v)[32], float s, const float* p) {
+// kW values of a vector over columns, on 16 bytes
+__device__ __forceinline__ void load_cols(const float* p, float (&c)[kW]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kW / 4; ++i) {
         const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
-        v[4 * i] *= s * f.x, v[4 * i + 1] *= s * f.y;
-        v[4 * i + 2] *= s * f.z, v[4 * i + 3] *= s * f.w;
+        c[4 * i] = f.x, c[4 * i + 1] = f.y, c[4 * i + 2] = f.z, c[4 * i + 3] = f.w;
     }
 }
-__device__ __forceinline__ void add_cols(float (&v)[32], const float* p) {
+__device__ __forceinline__ void scale_cols(float (&v)[kW], float s, const float (&c)[kW]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
-        v[4 * i] += f.x, v[4 * i + 1] += f.y, v[4 * i + 2] += f.z, v[4 * i + 3] += f.w;
+    for (int i = 0; i < kW; ++i) v[i] *= s * c[i];
+}
+// kW elements of a residual's row on 16 bytes, as stored
+template <typename T>
+struct RawRow {
+    uint4 q[kW * sizeof(T) / 16];
+};
+template <typename T>
+__device__ __forceinline__ void ask_row(const T* p, RawRow<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)(kW * sizeof(T) / 16); ++i) r.q[i] = reinterpret_cast<const uint4*>(p)[i];
+}
+template <typename T>
+__device__ __forceinline__ void add_row(float (&v)[kW], const RawRow<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)(kW * sizeof(T) / 4); ++i) {
+        const uint32_t w = (&r.q[i / 4].x)[i % 4];
+        if constexpr (sizeof(T) == 4) {
+            v[i] += __uint_as_float(w);
+        } else if constexpr (sizeof(T) == 2) {
+            const T lo = reinterpret_cast<const T*>(&w)[0], hi = reinterpret_cast<const T*>(&w)[1];
+            v[2 * i] += to_f(lo);
+            v[2 * i + 1] += to_f(hi);
+        }
     }
 }
 
@@ -146,9 +191,10 @@ __device__ __forceinline__ float get_one(const void* p, long long i, int type) {
     return static_cast<const float*>(p)[i];
 }
 
-// One output element of row m, column n from its accumulators.
+// One output element of row m, column n from its accumulators (what the backward
+// pass keeps of it is stored).
 template <bool GATED>
-__device__ __forceinline__ void finish_one(const TileArgs& a, long long m, int n, float v,
+__device__ __forceinline__ float value_one(const TileArgs& a, long long m, int n, float v,
                                            float u) {
     if (a.col_scale[0]) {
         const float rs = a.row_scale[m];
@@ -160,79 +206,73 @@ __device__ __forceinline__ void finish_one(const TileArgs& a, long long m, int n
             put_one(a.save[0], m * a.lds[0] + n, a.out_type, v);
             put_one(a.save[1], m * a.lds[1] + n, a.out_type, u);
         }
-        v = act_f(v, a.act) * u;
-    } else {
-        if (a.bias) v += a.bias[n];
-        if (a.save[0]) put_one(a.save[0], m * a.lds[0] + n, a.out_type, v);
-        v = act_f(v, a.act);
-        if (a.residual) v += get_one(a.residual, m * a.ldr + n, a.out_type);
+        return act_f(v, a.act) * u;
     }
-    if (!a.out2 || m < a.rows0) put_one(a.out, m * a.ldo + n, a.out_type, v);
-    else if (m >= a.rows1) put_one(a.out2, (m - a.rows1) * a.ldo2 + n, a.out_type, v);
+    if (a.bias) v += a.bias[n];
+    if (a.save[0]) put_one(a.save[0], m * a.lds[0] + n, a.out_type, v);
+    v = act_f(v, a.act);
+    if (a.residual) v += get_one(a.residual, m * a.ldr + n, a.out_type);
+    return v;
 }
 
-// Chunks at the right edge, and rows that start on no 16 bytes: one element after
-// the other, out of line, so that the path that every chunk takes stays short.
+// Chunks at the right edge, and rows that start on no 16 bytes (`store`: their outputs
+// go straight to memory): one element after the other, out of line.
 template <bool GATED>
-__device__ __noinline__ void finish_slowly(const TileArgs& a, int m, int n, const float* v,
-                                           const float* u) {
-    const int left = a.N - n < 32 ? a.N - n : 32;
-    for (int i = 0; i < left; ++i) finish_one<GATED>(a, m, n + i, v[i], GATED ? u[i] : 0.0f);
+__device__ __noinline__ void finish_slowly(const TileArgs& a, int m, int n, float* v,
+                                           const float* u, bool store) {
+    const int left = a.N - n < kW ? a.N - n : kW;
+    for (int i = 0; i < left; ++i) {
+        const float o = value_one<GATED>(a, m, n + i, v[i], GATED ? u[i] : 0.0f);
+        v[i] = o;
+        if (!store) continue;
+        if (!a.out2 || m < a.rows0) put_one(a.out, m * a.ldo + n + i, a.out_type, o);
+        else if (m >= a.rows1) put_one(a.out2, (m - a.rows1) * a.ldo2 + n + i, a.out_type, o);
+    }
 }
 
-// Epilogue of columns n .. n + 31 of row m, all inside and on 16 bytes; raw: the
-// 16-bit residual's.
-template <bool GATED>
-__device__ __forceinline__ void finish_row(const TileArgs& a, int m, int n, float (&v)[32],
-                                           float (&u)[GATED ? 32 : 1], float row_scale,
-                                           const uint4 (&raw)[4]) {
-    if (a.col_scale[0]) {
-        scale_cols(v, row_scale, a.col_scale[0] + n);
-        if constexpr (GATED) scale_cols(u, row_scale, a.col_scale[1] + n);
+// Epilogue of columns n .. n + kW - 1 of row m, all inside and on 16 bytes, v <- their
+// outputs; raw: the residual's, c: the columns' scales (the gate's) or, without any,
+// biases. GRAD: a backward product, whose output is the sum itself.
+template <bool F8, bool GATED, bool GRAD, int OUT>
+__device__ __forceinline__ void finish_row(const TileArgs& a, int m, int n, float (&v)[kW],
+                                           float (&u)[GATED ? kW : 1], float row_scale,
+                                           const RawRow<typename OutOf<OUT>::T>& raw,
+                                           float (&c)[kW]) {
+    using T = typename OutOf<OUT>::T;
+    if constexpr (F8) {
+        scale_cols(v, row_scale, c);
+        if constexpr (GATED) {
+            load_cols(a.col_scale[1] + n, c);
+            scale_cols(u, row_scale, c);
+        } else if (a.bias) {
+            load_cols(a.bias + n, c);
+        }
     }
     if constexpr (GATED) {
-        if (a.save[0]) {
-            put_row(a.save[0], m * a.lds[0] + n, a.out_type, v, a.vec & kWideSave);
-            put_row(a.save[1], m * a.lds[1] + n, a.out_type, u, a.vec & kWideSave);
+        if (__builtin_expect(a.save[0] != nullptr, 0)) {
+            put_row(static_cast<T*>(a.save[0]) + m * a.lds[0] + n, v, a.vec & kWideSave);
+            put_row(static_cast<T*>(a.save[1]) + m * a.lds[1] + n, u, a.vec & kWideSave);
         }
         act_row(v, a.act);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= u[i];
-    } else {
-        if (a.bias) add_cols(v, a.bias + n);
-        if (a.save[0])
-            put_row(a.save[0], m * a.lds[0] + n, a.out_type, v, a.vec & kWideSave);
-        act_row(v, a.act);
-        if (a.residual) {
-            if (a.out_type == BVML_F32) {
-                add_cols(v, static_cast<const float*>(a.residual) + m * a.ldr + n);
-            } else {
+        for (int i = 0; i < kW; ++i) v[i] *= u[i];
+    } else if constexpr (!GRAD) {
+        if (a.bias) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t w = (&raw[i / 4].x)[i % 4];
-                    if (a.out_type == BVML_BF16) {
-                        v[2 * i] += __uint_as_float(w << 16);
-                        v[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
-                    } else {
-                        const float2 f = __half22float2(reinterpret_cast<const __half2&>(w));
-                        v[2 * i] += f.x;
-                        v[2 * i + 1] += f.y;
-                    }
-                }
-            }
+            for (int i = 0; i < kW; ++i) v[i] += c[i];
         }
+        if (__builtin_expect(a.save[0] != nullptr, 0))
+            put_row(static_cast<T*>(a.save[0]) + m * a.lds[0] + n, v, a.vec & kWideSave);
+        act_row(v, a.act);
+        if (a.residual) add_row(v, raw);
     }
-    if (!a.out2 || m < a.rows0)
-        put_row(a.out, m * a.ldo + n, a.out_type, v, a.vec & kWideOut);
-    else if (m >= a.rows1)
-        put_row(a.out2, (m - a.rows1) * a.ldo2 + n, a.out_type, v, a.vec & kWideOut);
 }
 
-template <int BN, bool AT, bool BT, bool F8, bool GATED>
+template <int BN, bool AT, bool BT, bool F8, bool GATED, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
 gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     static_assert(!BT || BN % 128 == 0, "a box of B's rows is 64 wide");
-    static_assert(BN % 64 == 0, "chunks of 32 columns, half of them of each projection");
+    static_assert(BN % 64 == 0, "columns in boxes of 64");
     static_assert(!F8 || (!AT && !BT), "8-bit operands are row-major");
     constexpr int kStage = tile_stage_bytes<BN>();
     constexpr int kStages = tile_stages<BN>();
@@ -243,7 +283,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t sbase = tc::smem_u32(smem);
-    uint8_t* bar_mem = smem + kStages * kStage;
+    uint8_t* bar_mem = smem + kStages * kStage + tile_staging_bytes<BN>();
     const uint32_t bars = tc::smem_u32(bar_mem);
     const uint32_t bar_full = bars;               // kTileMaxStages, counted on the first CTA's
     const uint32_t bar_empty = bars + 64;         // kTileMaxStages, in each CTA
@@ -422,33 +462,39 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     } else {
         // ------------------------------------------------------------ epilogue
         const int quarter = warp & 3;            // the TMEM lanes this warp may read
-        constexpr int kParts = kTileEpiWarps / 4;
-        const int part = (warp - 2) >> 2;        // every kParts-th chunk of 32 columns
-        constexpr int kChunks = kCN / 32;
+        using T = typename OutOf<OUT>::T;
+        static_assert(kTileEpiWarps == 8, "two warps a quarter of the TMEM lanes");
+        const int part = (warp - 2) >> 2;        // even or odd boxes of 128-byte rows
+        constexpr int kBox = 128 / sizeof(T);    // columns of a box
+        constexpr int kBoxes = kCN / kBox;
+        static_assert(kCN % kBox == 0, "whole boxes");
+        constexpr int kBufs = tile_buffers<BN>();
+        uint8_t* stg = smem + kStages * kStage + (warp - 2) * 4096 * kBufs;
+        int filled = 0;  // boxes staged by this warp
         const uint32_t acc_empty0 = tc::map_to(bar_acc_empty, 0);
-        // whole chunks of rows on 16 bytes take the short path
+        // rows on 16 bytes take the short path
         const bool fast = (a.vec & kOn16) != 0;
-        const bool halves = !GATED && fast && a.residual && a.out_type != BVML_F32;
+        const bool ahead = !GATED && !BT && fast && a.residual;
+        const float* cols = !fast || BT ? nullptr : F8 ? a.col_scale[0] : a.bias;
         int tl = 0;
         for (int w = pair; w < works; w += pairs, ++tl) {
             int m0, n0, k0, k1, split;
             work_of(w, m0, n0, k0, k1, split);
-            const int m = m0 + quarter * 32 + lane;
+            const int mw = m0 + quarter * 32, m = mw + lane;
             const bool in = m < a.M;
-            // chunks that do not go round fall to one warp after the other
-            const int first = kChunks % kParts ? (part + tl) % kParts : part;
-            uint4 raw[4] = {};
-            auto ask = [&](int chunk) {  // the residual's
-                const int n = n0 + chunk * 32;
-                if (halves && in && chunk < kChunks && n + 32 <= a.N) {
-                    const uint4* p = reinterpret_cast<const uint4*>(
-                        static_cast<const uint16_t*>(a.residual) + m * a.ldr + n);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) raw[i] = p[i];
-                }
+            // an odd box falls to either warp in turn
+            const int first = kBoxes % 2 ? (part + tl) & 1 : part;
+            // The next chunk's residual and scales or biases are on their way while one is
+            // finished.
+            RawRow<T> raw{};
+            float cnext[kW] = {};
+            auto ask = [&](int n) {
+                if (n + kW > a.N) return;
+                if (ahead && in) ask_row(static_cast<const T*>(a.residual) + m * a.ldr + n, raw);
+                if (cols) load_cols(cols + n, cnext);
             };
-            ask(first);
-            const float row_scale = a.row_scale && in ? __ldg(a.row_scale + m) : 0.0f;
+            if (first < kBoxes) ask(n0 + first * kBox);
+            const float row_scale = F8 && in ? __ldg(a.row_scale + m) : 0.0f;
             const int buf = tl & 1, u = tl >> 1;
             if (!wait_all(bar_acc_full + 8 * buf, u & 1, 6) || gone()) break;
             tc::tc_fence_after();
@@ -458,41 +504,74 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive_cluster_relaxed(acc_empty0 + 8 * buf);
             };
-            if (first >= kChunks) hand_back();
+            if (first >= kBoxes) hand_back();
 #pragma unroll 1
-            for (int c = first; c < kChunks; c += kParts) {
-                const int n = n0 + c * 32;
-                if (c != first) ask(c);
-                float v[32], g[GATED ? 32 : 1];
-                {
-                    uint32_t x[32], y[GATED ? 32 : 1];
-                    tc::tmem_ld_32cols(acc + c * 32, x);
-                    if constexpr (GATED) tc::tmem_ld_32cols(acc + BN / 2 + c * 32, y);
-                    tc::tmem_ld_wait();
+            for (int b = first; b < kBoxes; b += 2) {
+                uint8_t* box = stg + (filled % kBufs) * 4096;
+                // the store that last read this buffer has done so
+                if (lane == 0) tc::bulk_wait_read<kBufs - 1>();
+                __syncwarp();
+#pragma unroll 1
+                for (int c = 0; c < kBox; c += kW) {
+                    const int n = n0 + b * kBox + c;
+                    float v[kW], g[GATED ? kW : 1], cnow[kW];
+                    __syncwarp();  // lanes may have gone different ways
+                    {
+                        uint32_t x[kW], y[GATED ? kW : 1];
+                        tc::tmem_ld_16cols(acc + b * kBox + c, x);
+                        if constexpr (GATED) tc::tmem_ld_16cols(acc + BN / 2 + b * kBox + c, y);
+                        tc::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(x[i]);
-                    if constexpr (GATED) {
+                        for (int i = 0; i < kW; ++i) v[i] = __uint_as_float(x[i]);
+                        if constexpr (GATED) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(y[i]);
+                            for (int i = 0; i < kW; ++i) g[i] = __uint_as_float(y[i]);
+                        }
                     }
-                }
-                if (c + kParts >= kChunks) hand_back();
-                if (!in || n >= a.N) continue;
-                if (a.slab)  // one of several shares of K, its pitch a multiple of 32
-                    put_row(a.slab, ((long long)split * a.M + m) * a.ldslab + n, BVML_F32, v, true);
-                else if (fast && n + 32 <= a.N)
-                    finish_row<GATED>(a, m, n, v, g, row_scale, raw);
-                else {
-                    // copies: an array whose address leaves lives in memory everywhere
-                    float tv[32], tg[GATED ? 32 : 1];
+                    const bool last = c + kW == kBox;
+                    if (last && b + 2 >= kBoxes) hand_back();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) tv[i] = v[i];
+                    for (int i = 0; i < kW; ++i) cnow[i] = cnext[i];
+                    const RawRow<T> now = raw;
+                    if (!last) ask(n + kW);
+                    else if (b + 2 < kBoxes) ask(n0 + (b + 2) * kBox);
+                    if (n >= a.N) continue;
+                    if (BT && a.slab) {  // one of several shares of K, its pitch a multiple of 32
+                        if (in)
+                            put_row(a.slab + ((long long)split * a.M + m) * a.ldslab + n, v, true);
+                        continue;
+                    }
+                    if (__builtin_expect(fast && n + kW <= a.N, 1)) {
+                        if (in)
+                            finish_row<F8, GATED, BT, OUT>(a, m, n, v, g, row_scale, now, cnow);
+                    } else if (in) {
+                        // copies: an array whose address leaves lives in memory everywhere
+                        float tv[kW], tg[GATED ? kW : 1];
 #pragma unroll
-                    for (int i = 0; i < (GATED ? 32 : 1); ++i) tg[i] = g[i];
-                    finish_slowly<GATED>(a, m, n, tv, tg);
+                        for (int i = 0; i < kW; ++i) tv[i] = v[i];
+#pragma unroll
+                        for (int i = 0; i < (GATED ? kW : 1); ++i) tg[i] = g[i];
+                        finish_slowly<GATED>(a, m, n, tv, tg, !fast);
+#pragma unroll
+                        for (int i = 0; i < kW; ++i) v[i] = tv[i];
+                    }
+                    if (fast) stage_row<T>(box, lane, c / kW, v);
                 }
+                if (!fast || (BT && a.slab)) continue;
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                const int n = n0 + b * kBox;
+                const bool second = AT && a.out2 && mw >= a.rows1;
+                const int row = second ? mw - a.rows1 : mw;
+                if (lane == 0) {
+                    if (n < a.N && row < a.out_rows)
+                        tc::tma_store_2d(&maps.o[second], tc::smem_u32(box), n, row);
+                    tc::bulk_commit();
+                }
+                ++filled;
             }
         }
+        if (lane == 0) tc::bulk_wait_all();  // before shared memory goes
     }
     __syncthreads();
     __syncwarp();
@@ -501,13 +580,23 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     tc::cluster_sync();
 }
 
-template <int BN, bool AT, bool BT, bool F8, bool GATED>
-cudaError_t launch_tile(const TileMaps& maps, const TileArgs& a, int pairs, cudaStream_t s) {
-    auto kern = gemm_tile_kernel<BN, AT, BT, F8, GATED>;
+template <int BN, bool AT, bool BT, bool F8, bool GATED, int OUT>
+cudaError_t launch_tile_out(const TileMaps& maps, const TileArgs& a, int pairs, cudaStream_t s) {
+    auto kern = gemm_tile_kernel<BN, AT, BT, F8, GATED, OUT>;
     constexpr int smem = tile_smem_bytes<BN>();
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, 2 * pairs, kTileThreads, smem, s, true, maps, a);
+}
+template <int BN, bool AT, bool BT, bool F8, bool GATED>
+cudaError_t launch_tile(const TileMaps& maps, const TileArgs& a, int pairs, cudaStream_t s) {
+    if (a.out_type == BVML_BF16)
+        return launch_tile_out<BN, AT, BT, F8, GATED, BVML_BF16>(maps, a, pairs, s);
+    if (a.out_type == BVML_F16)
+        return launch_tile_out<BN, AT, BT, F8, GATED, BVML_F16>(maps, a, pairs, s);
+    if constexpr (!BT)  // gradients are of the operands' type
+        return launch_tile_out<BN, AT, BT, F8, GATED, BVML_F32>(maps, a, pairs, s);
+    return cudaErrorInvalidValue;
 }
 
 // Host reader of this translation unit's error word; resets it.

@@ -8,9 +8,7 @@ cudaError_t launch_tile_nt(int bn, bool gated, const TileMaps& m, const TileArgs
                            cudaStream_t s) {
     if (gated) {
         if (bn == 256) return launch_tile<256, false, false, false, true>(m, a, pairs, s);
-        if (bn == 192) return launch_tile<192, false, false, false, true>(m, a, pairs, s);
-        if (bn == 128) return launch_tile<128, false, false, false, true>(m, a, pairs, s);
-        return launch_tile<64, false, false, false, true>(m, a, pairs, s);
+        return launch_tile<128, false, false, false, true>(m, a, pairs, s);
     }
     if (bn == 256) return launch_tile<256, false, false, false, false>(m, a, pairs, s);
     if (bn == 192) return launch_tile<192, false, false, false, false>(m, a, pairs, s);

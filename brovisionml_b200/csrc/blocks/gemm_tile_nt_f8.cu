@@ -8,9 +8,7 @@ cudaError_t launch_tile_nt_f8(int bn, bool gated, const TileMaps& m, const TileA
                            cudaStream_t s) {
     if (gated) {
         if (bn == 256) return launch_tile<256, false, false, true, true>(m, a, pairs, s);
-        if (bn == 192) return launch_tile<192, false, false, true, true>(m, a, pairs, s);
-        if (bn == 128) return launch_tile<128, false, false, true, true>(m, a, pairs, s);
-        return launch_tile<64, false, false, true, true>(m, a, pairs, s);
+        return launch_tile<128, false, false, true, true>(m, a, pairs, s);
     }
     if (bn == 256) return launch_tile<256, false, false, true, false>(m, a, pairs, s);
     if (bn == 192) return launch_tile<192, false, false, true, false>(m, a, pairs, s);

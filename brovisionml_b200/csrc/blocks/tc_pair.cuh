@@ -92,6 +92,14 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t on, uint32_t dst,
         : "memory");
 }
 
+// Tiled store of a box from this CTA's shared memory (bulk-group completion).
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(c0), "r"(c1)
+                 : "memory");
+}
+
 // Operand stored (k, rows): boxes of 64 rows `box_bytes` apart.
 __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t box_bytes) {
     uint64_t d = 0;
