@@ -8,7 +8,8 @@ or missing before this script has run.)
 Compiles each brovisionml_b200/csrc/*.cu with nvcc for
 ``-gencode arch=compute_100a,code=sm_100a`` (B200 only) and links them into
 ``brovisionml_b200/_lib/libbvml_dsine.so``, and csrc/blocks/*.cu (the
-feed-forward operators, include/bvml_blocks.h) into ``_lib/libbvml_blocks.so``.
+feed-forward operators, include/bvml_blocks.h) into ``_lib/libbvml_blocks.so``,
+with their Python binding (csrc/blocks/blocks_torch.cpp) in ``_lib/_blocks_torch.so``.
 The C++ drop-in bridge
 (csrc/dsine_ops_b200.cpp) is compiled into ``_lib/libbvml_dsine_bridge.so``
 against the stand-in brotensor header, to prove that it builds.
@@ -18,10 +19,12 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -35,6 +38,7 @@ LIB = os.path.join(LIB_DIR, "libbvml_dsine.so")
 CHECKED_LIB = os.path.join(LIB_DIR, "libbvml_dsine_checked.so")
 BLOCKS = os.path.join(CSRC, "blocks")
 BLOCKS_LIB = os.path.join(LIB_DIR, "libbvml_blocks.so")
+BLOCKS_TORCH = os.path.join(LIB_DIR, "_blocks_torch.so")  # their Python binding
 BRIDGE = os.path.join(LIB_DIR, "libbvml_dsine_bridge.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -104,6 +108,20 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
     if _stale(BLOCKS_LIB, bobjs + [__file__]):
         run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_LIB] + bobjs +
             ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
+    torch_src = os.path.join(BLOCKS, "blocks_torch.cpp")
+    if _stale(BLOCKS_TORCH, [torch_src, BLOCKS_LIB, __file__] + headers):
+        torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+        cuda = os.path.dirname(os.path.dirname(nvcc))
+        run([os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC",
+             "-shared", "-fvisibility=hidden", "-DUSE_CUDA",
+             "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(cuda, "include"),
+             "-isystem", os.path.join(torch_dir, "include"),
+             "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+             "-I" + sysconfig.get_path("include"), torch_src, "-o", BLOCKS_TORCH,
+             "-L" + LIB_DIR, "-lbvml_blocks", "-Wl,-rpath,$ORIGIN",
+             "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
+             "-ltorch_cuda", "-lc10", "-lc10_cuda",
+             "-Wl,-rpath," + os.path.join(torch_dir, "lib")])
     if _stale(LIB, objs + [__file__]):
         # Shared cudart: callers (torch, or a brotensor runtime) hand in stream
         # handles created by THEIR CUDA runtime; one shared runtime instance

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import brovisionml_b200 as bv
-from brovisionml_b200 import blocks as B
+from brovisionml_b200 import _blocks_capi as B
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "bvml_blocks.h")

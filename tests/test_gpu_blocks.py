@@ -16,7 +16,7 @@ import pytest
 import torch
 
 import brovisionml_b200 as bv
-from brovisionml_b200 import blocks as B
+from brovisionml_b200 import _blocks_capi as B
 
 pytestmark = pytest.mark.gpu
 
