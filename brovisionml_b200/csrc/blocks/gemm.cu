@@ -26,6 +26,14 @@ struct Stored {
     long long ld_packed;
 };
 
+// A matrix of the epilogue whose rows do not start on 16 bytes (or, for outputs, end
+// there): it lives in the workspace on whole lines while the kernel runs.
+struct Moved {
+    bool on;
+    size_t at;
+    long long ld;
+};
+
 struct Plan {
     bool skinny;
     int bn;        // tile: columns of a pair
@@ -34,6 +42,7 @@ struct Plan {
     int steps[2];
     int tiles_m, tiles_n;
     Stored a[2], b[2];
+    Moved residual, out[2], save[2];
     long long ldslab;
     size_t slab;   // offset of the partial sums
     size_t bytes;  // workspace
@@ -123,6 +132,22 @@ Plan plan_of(const GemmLaunch& L) {
     if (p.splits > 1) {
         p.ldslab = ((long long)L.N + 31) / 32 * 32;
         off += round256((size_t)p.splits * L.M * p.ldslab * 4);
+    } else {
+        const size_t eo = elem_size(L.out_type);
+        const long long lines = ((long long)L.N * (long long)eo + 127) / 128 * 128 / (long long)eo;
+        auto moved = [&](const void* ptr, long long ld, int rows, bool output) {
+            Moved m{};
+            m.on = ptr && (!on16(ptr, ld, eo) || (output && ((size_t)L.N * eo & 15)));
+            m.ld = m.on ? lines : ld;
+            m.at = off;
+            if (m.on) off += round256((size_t)rows * lines * eo);
+            return m;
+        };
+        const int rows = L.out2 ? L.rows0 : L.M;
+        p.residual = moved(L.residual, L.ldr, L.M, false);
+        p.out[0] = moved(L.out, L.ldo, rows, true);
+        p.out[1] = moved(L.out2, L.ldo2, rows, true);
+        for (int i = 0; i < 2; ++i) p.save[i] = moved(L.save[i], L.lds[i], L.M, true);
     }
     p.bytes = off;
     return p;
@@ -153,19 +178,51 @@ pack_kernel(const T* __restrict__ src, long long ld, int rows, int cols, T* __re
     }
 }
 
-cudaError_t pack(const Stored& s, size_t es, void* ws, cudaStream_t st) {
-    const int units = (int)(s.ld_packed * (long long)es / 16);
-    const long long total = (long long)s.rows * units;
-    const long long want = (total + 255) / 256;
+cudaError_t pack_rows(const void* src, long long ld, int rows, int cols, void* dst,
+                      long long ld_packed, size_t es, cudaStream_t st) {
+    const int units = (int)(ld_packed * (long long)es / 16);
+    const long long want = ((long long)rows * units + 255) / 256;
     const int grid = (int)(want < 148 * 16 ? want : 148 * 16);
-    void* d = static_cast<char*>(ws) + s.at;
     if (es == 1)
         return launch_pdl(pack_kernel<uint8_t>, grid, 256, 0, st, true,
-                          static_cast<const uint8_t*>(s.p), s.ld, s.rows, s.cols,
-                          static_cast<uint8_t*>(d), units);
-    return launch_pdl(pack_kernel<uint16_t>, grid, 256, 0, st, true,
-                      static_cast<const uint16_t*>(s.p), s.ld, s.rows, s.cols,
-                      static_cast<uint16_t*>(d), units);
+                          static_cast<const uint8_t*>(src), ld, rows, cols,
+                          static_cast<uint8_t*>(dst), units);
+    if (es == 2)
+        return launch_pdl(pack_kernel<uint16_t>, grid, 256, 0, st, true,
+                          static_cast<const uint16_t*>(src), ld, rows, cols,
+                          static_cast<uint16_t*>(dst), units);
+    return launch_pdl(pack_kernel<uint32_t>, grid, 256, 0, st, true,
+                      static_cast<const uint32_t*>(src), ld, rows, cols,
+                      static_cast<uint32_t*>(dst), units);
+}
+cudaError_t pack(const Stored& s, size_t es, void* ws, cudaStream_t st) {
+    return pack_rows(s.p, s.ld, s.rows, s.cols, static_cast<char*>(ws) + s.at, s.ld_packed, es, st);
+}
+
+// The way back: neighbouring lanes write neighbouring elements.
+template <typename T>
+__global__ void __launch_bounds__(256)
+unpack_kernel(const T* __restrict__ src, long long lds, int rows, int cols, T* __restrict__ dst,
+              long long ld) {
+    begin();
+    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+        const T* a = src + r * lds;
+        T* b = dst + r * ld;
+#pragma unroll 4
+        for (int c = threadIdx.x; c < cols; c += 256) b[c] = a[c];
+    }
+}
+cudaError_t unpack(const Moved& m, const void* ws, void* dst, long long ld, int rows, int cols,
+                   size_t es, cudaStream_t st) {
+    const void* src = static_cast<const char*>(ws) + m.at;
+    const int grid = rows < 148 * 32 ? rows : 148 * 32;
+    if (es == 2)
+        return launch_pdl(unpack_kernel<uint16_t>, grid, 256, 0, st, true,
+                          static_cast<const uint16_t*>(src), m.ld, rows, cols,
+                          static_cast<uint16_t*>(dst), ld);
+    return launch_pdl(unpack_kernel<uint32_t>, grid, 256, 0, st, true,
+                      static_cast<const uint32_t*>(src), m.ld, rows, cols,
+                      static_cast<uint32_t*>(dst), ld);
 }
 
 // ------------------------------------------------------------ the shares' sum
@@ -293,40 +350,48 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n;
     a.splits = p.splits;
     a.row_scale = L.row_scale;
-    for (int i = 0; i < 2; ++i) {
-        a.col_scale[i] = L.col_scale[i];
-        a.save[i] = L.save[i];
-        a.lds[i] = L.lds[i];
-    }
-    a.bias = L.bias, a.residual = L.residual, a.out = L.out, a.out2 = L.out2;
-    a.ldr = L.ldr, a.ldo = L.ldo, a.ldo2 = L.ldo2;
+    for (int i = 0; i < 2; ++i) a.col_scale[i] = L.col_scale[i];
+    a.bias = L.bias;
     a.rows0 = L.rows0, a.rows1 = L.rows1;
+    a.out_rows = L.out2 ? L.rows0 : L.M;
     a.out_type = L.out_type, a.act = L.act;
+    // the epilogue's matrices, or their places in the workspace
+    auto place = [&](const Moved& m, const void* ptr) {
+        return m.on ? static_cast<char*>(ws) + m.at : static_cast<char*>(const_cast<void*>(ptr));
+    };
+    auto pitch = [&](const Moved& m, long long ld) { return m.on ? m.ld : ld; };
+    if (p.residual.on)
+        e = pack_rows(L.residual, L.ldr, L.M, L.N, place(p.residual, nullptr), p.residual.ld, eo, s);
+    if (e != cudaSuccess) return e;
+    a.residual = place(p.residual, L.residual), a.ldr = pitch(p.residual, L.ldr);
+    a.out = place(p.out[0], L.out), a.ldo = pitch(p.out[0], L.ldo);
+    a.out2 = place(p.out[1], L.out2), a.ldo2 = pitch(p.out[1], L.ldo2);
+    for (int i = 0; i < 2; ++i) {
+        a.save[i] = place(p.save[i], L.save[i]);
+        a.lds[i] = pitch(p.save[i], L.lds[i]);
+    }
     // what the addresses and pitches that the epilogue touches have in common
     auto bits = [&](const void* ptr, long long ld) {
         return ptr ? reinterpret_cast<uintptr_t>(ptr) | (uintptr_t)ld * eo : (uintptr_t)0;
     };
-    const uintptr_t out = bits(L.out, L.ldo) | bits(L.out2, L.ldo2);
-    const uintptr_t save = bits(L.save[0], L.lds[0]) | bits(L.save[1], L.lds[1]);
-    // (a TMA store's right edge is cut in units of 16 bytes: N counts too)
-    const uintptr_t all = out | save | (uintptr_t)L.N * eo | bits(L.residual, L.ldr) |
+    const uintptr_t out = bits(a.out, a.ldo) | bits(a.out2, a.ldo2);
+    const uintptr_t save = bits(a.save[0], a.lds[0]) | bits(a.save[1], a.lds[1]);
+    const uintptr_t all = out | save | bits(a.residual, a.ldr) |
                           reinterpret_cast<uintptr_t>(L.bias) |
                           reinterpret_cast<uintptr_t>(L.col_scale[0]) |
                           reinterpret_cast<uintptr_t>(L.col_scale[1]);
     a.vec = ((all & 15) == 0 ? kOn16 : 0) | ((save & 31) == 0 ? kWideSave : 0);
-    const bool vec = (out & 15) == 0;
     if (p.skinny) {
         k.split = p.splits;
         a.idesc = idesc_of(L.in_type, false, false, 128, p.tok);
         return launch_skinny(p.tok, L.in_type == BVML_E4M3, L.gated, maps, k, s);
     }
     a.idesc = idesc_of(L.in_type, L.a_t, L.b_t, 256, p.bn);
-    a.out_rows = L.out2 ? L.rows0 : L.M;
     if ((a.vec & kOn16) && p.splits == 1) {  // one row's pitch is any multiple of 16 bytes
-        auto pitch = [&](long long ld) { return a.out_rows > 1 ? ld : ((L.N + 7LL) / 8 * 8); };
-        e = encode_rows(&maps.o[0], L.out, pitch(L.ldo), a.out_rows, L.N, L.out_type, 32);
-        if (e == cudaSuccess && L.out2)
-            e = encode_rows(&maps.o[1], L.out2, pitch(L.ldo2), a.out_rows, L.N, L.out_type, 32);
+        auto tma = [&](long long ld) { return a.out_rows > 1 ? ld : (L.N + 7LL) / 8 * 8; };
+        e = encode_rows(&maps.o[0], a.out, tma(a.ldo), a.out_rows, L.N, L.out_type, 32);
+        if (e == cudaSuccess && a.out2)
+            e = encode_rows(&maps.o[1], a.out2, tma(a.ldo2), a.out_rows, L.N, L.out_type, 32);
         if (e != cudaSuccess) return e;
     }
     if (p.splits > 1) {
@@ -347,7 +412,17 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     if (L.b_t) e = launch_tile_grad(p.bn, L.a_t, maps, a, pairs, s);
     else if (L.in_type == BVML_E4M3) e = launch_tile_nt_f8(p.bn, L.gated, maps, a, pairs, s);
     else e = launch_tile_nt(p.bn, L.gated, maps, a, pairs, s);
-    if (e != cudaSuccess || p.splits == 1) return e;
+    if (e != cudaSuccess) return e;
+    if (p.splits == 1) {
+        void* const to[4] = {L.out, L.out2, L.save[0], L.save[1]};
+        const Moved* const from[4] = {&p.out[0], &p.out[1], &p.save[0], &p.save[1]};
+        const long long ld[4] = {L.ldo, L.ldo2, L.lds[0], L.lds[1]};
+        for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+            if (from[i]->on)
+                e = unpack(*from[i], ws, to[i], ld[i], i < 2 ? a.out_rows : L.M, L.N, eo, s);
+        return e;
+    }
+    const bool vec = on16(L.out, L.ldo, eo) && (!L.out2 || on16(L.out2, L.ldo2, eo));
     if (L.out_type == BVML_F16) return join<__half>(L, p, a.slab, vec, s);
     if (L.out_type == BVML_BF16) return join<__nv_bfloat16>(L, p, a.slab, vec, s);
     return join<float>(L, p, a.slab, vec, s);

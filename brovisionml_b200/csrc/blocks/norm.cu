@@ -48,6 +48,28 @@ struct NormBwdArgs {
 // the larger of two magnitudes, NaN if either is (fmaxf would drop it)
 __device__ __forceinline__ float max_nan(float m, float a) { return (a > m || a != a) ? a : m; }
 
+// From a row's largest |s w| to its scale and to y / scale = s w 448 / max |s w|,
+// from which the root drops out. What the product and the quotient leave over in
+// 32 bits is carried along: a value next to a rounding border of the 8 bits then falls
+// where the formula has it but for the rounding of the largest value itself.
+struct Quant {
+    float scale, hi, lo;
+    __device__ __forceinline__ float operator()(float s, float w) const {
+        const float p = s * w, rest = fmaf(s, w, -p);
+        return fmaf(p, hi, fmaf(p, lo, rest * hi));
+    }
+};
+__device__ __forceinline__ Quant quant_of(float m, float rstd) {
+    const float top = m * rstd;
+    if (top < kTinyMax) return Quant{1.0f, 0.0f, 0.0f};
+    Quant f;
+    f.scale = top / 448.0f;
+    f.hi = m > 1e-30f ? 448.0f / m : rstd * (448.0f / top);  // the quotient must not overflow
+    f.lo = m > 1e-30f ? fmaf(-m, f.hi, 448.0f) / m : 0.0f;
+    if (top != top) f.hi = top;  // NaN in the row, or an infinity against 1 / infinity
+    return f;
+}
+
 // Feature index of element e of group v of lane l: eight consecutive features
 // where vectors can be used, otherwise lanes side by side.
 template <int G>
@@ -187,8 +209,16 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float (*slots)[2]
     }
 }
 
+// Blocks an SM that the forward pass is built for: 64 registers a thread with one
+// group of eight, 80 with two, 128 with four.
+constexpr int forward_blocks(int G, int VPT) {
+    const int threads = G > 32 ? G : kNormThreads;
+    const int n = (VPT == 1 ? 1024 : VPT == 2 ? 768 : 512) / threads;
+    return n > 0 ? n : 1;
+}
+
 template <typename T, int G, int VPT, bool Q>
-__global__ void __launch_bounds__(G > 32 ? G : kNormThreads)
+__global__ void __launch_bounds__(G > 32 ? G : kNormThreads, forward_blocks(G, VPT))
 rms_norm_kernel(const NormArgs a) {
     constexpr int kThreads = G > 32 ? G : kNormThreads;
     constexpr int kRows = kThreads / G;
@@ -240,28 +270,27 @@ rms_norm_kernel(const NormArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 q = fmaf(s[v][e], s[v][e], q);
-                s[v][e] *= w[v][e];
-                if constexpr (Q) m = max_nan(m, fabsf(s[v][e]));
+                if constexpr (Q) m = max_nan(m, fabsf(s[v][e] * w[v][e]));
             }
         }
         row_reduce<G, true>(q, m, slots, slot);
         if (!in) continue;
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
-        float f = rstd;
         if constexpr (Q) {
-            const float top = m * rstd;
-            const bool zero = top < kTinyMax;  // false for NaN, which goes through
-            if (l == 0) a.scale[t] = zero ? 1.0f : top * (1.0f / 448.0f);
-            f = zero ? 0.0f : rstd * (448.0f / top);
-        }
+            const Quant f = quant_of(m, rstd);
+            if (l == 0) a.scale[t] = f.scale;
 #pragma unroll
-        for (int v = 0; v < VPT; ++v)
+            for (int v = 0; v < VPT; ++v)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[v][e] *= f;
-        if constexpr (Q)
+                for (int e = 0; e < 8; ++e) s[v][e] = f(s[v][e], w[v][e]);
             store_row_e4m3<G, VPT>(static_cast<uint8_t*>(a.y) + t * a.ldy, a.K, a.vec, l, s);
-        else
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[v][e] *= w[v][e] * rstd;
             store_row<T, G, VPT>(static_cast<T*>(a.y) + t * a.ldy, a.K, a.vec, l, s);
+        }
     }
 }
 
@@ -288,18 +317,15 @@ rms_norm_long_kernel(const NormArgs a) {
         }
         row_reduce<kLongThreads, true>(q, m, slots, slot);
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
-        float f = rstd;
+        Quant f{};
         if constexpr (Q) {
-            const float top = m * rstd;
-            const bool zero = top < kTinyMax;
-            if (threadIdx.x == 0) a.scale[t] = zero ? 1.0f : top * (1.0f / 448.0f);
-            f = zero ? 0.0f : rstd * (448.0f / top);
+            f = quant_of(m, rstd);
+            if (threadIdx.x == 0) a.scale[t] = f.scale;
         }
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
             const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
-            const float y = s * wt(k) * f;
-            if constexpr (Q) static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(y);
-            else static_cast<T*>(a.y)[t * a.ldy + k] = from_f<T>(y);
+            if constexpr (Q) static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(f(s, wt(k)));
+            else static_cast<T*>(a.y)[t * a.ldy + k] = from_f<T>(s * (wt(k) * rstd));
         }
     }
 }
@@ -475,15 +501,6 @@ Shape shape_of(int K) {
     if (K <= 16384) return Shape::G512x4;
     return Shape::Long;
 }
-int block_threads(Shape h) {
-    switch (h) {
-        case Shape::G128x1: return 128;
-        case Shape::G512x2:
-        case Shape::G512x4:
-        case Shape::Long: return 512;
-        default: return 256;
-    }
-}
 int block_rows(Shape h) {
     switch (h) {
         case Shape::G8: return 32;
@@ -554,8 +571,19 @@ cudaError_t launch_rms_norm(const NormLaunch& L, cudaStream_t s) {
     const Shape h = shape_of(L.K);
     const int rows = block_rows(h);
     const long long want = ((long long)L.T + rows - 1) / rows;
-    // 1024 threads an SM with rows of a block's length, 2048 with shorter ones
-    const long long most = (long long)sms * ((rows > 1 ? 2048 : 1024) / block_threads(h));
+    // rows of a block's length: what is resident at once; shorter ones: twice that
+    // (57600 x 128: their blocks are done sooner than the next row could be asked for)
+    int blocks = 8;
+    switch (h) {
+        case Shape::G128x1: blocks = forward_blocks(128, 1); break;
+        case Shape::G256x1: blocks = forward_blocks(256, 1); break;
+        case Shape::G256x2: blocks = forward_blocks(256, 2); break;
+        case Shape::G512x2: blocks = forward_blocks(512, 2); break;
+        case Shape::G512x4: blocks = forward_blocks(512, 4); break;
+        case Shape::Long: blocks = 4; break;
+        default: break;
+    }
+    const long long most = (long long)sms * blocks;
     const int grid = (int)(want < most ? want : most);
     const bool q = L.scale != nullptr;
     if (L.type == BVML_F32) {
