@@ -38,6 +38,7 @@ LIB = os.path.join(LIB_DIR, "libbvml_dsine.so")
 CHECKED_LIB = os.path.join(LIB_DIR, "libbvml_dsine_checked.so")
 BLOCKS = os.path.join(CSRC, "blocks")
 BLOCKS_LIB = os.path.join(LIB_DIR, "libbvml_blocks.so")
+BLOCKS_CHECKED_LIB = os.path.join(LIB_DIR, "libbvml_blocks_checked.so")
 BLOCKS_TORCH = os.path.join(LIB_DIR, "_blocks_torch.so")  # their Python binding
 BRIDGE = os.path.join(LIB_DIR, "libbvml_dsine_bridge.so")
 
@@ -88,12 +89,17 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
     bheaders = headers + glob.glob(os.path.join(BLOCKS, "*.cuh")) + \
         glob.glob(os.path.join(BLOCKS, "*.h"))
     bobjs = []
+    bcobjs = []
     for src in sorted(glob.glob(os.path.join(BLOCKS, "*.cu"))):
         obj = os.path.join(OBJ_DIR, "blocks_" + os.path.basename(src)[:-3] + ".o")
         bobjs.append(obj)
         if _stale(obj, [src] + bheaders) or ptxas_info:
             jobs.append([nvcc] + ARCH + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) +
                         ["-c", src, "-o", obj])
+        cobj = os.path.join(OBJ_DIR, "checked_blocks_" + os.path.basename(src)[:-3] + ".o")
+        bcobjs.append(cobj)
+        if _stale(cobj, [src] + bheaders):
+            jobs.append([nvcc] + ARCH + NVCC_FLAGS + ["-DBVML_CHECKED", "-c", src, "-o", cobj])
 
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -107,6 +113,9 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
                 sys.stdout.write(out)
     if _stale(BLOCKS_LIB, bobjs + [__file__]):
         run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_LIB] + bobjs +
+            ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
+    if _stale(BLOCKS_CHECKED_LIB, bcobjs + [__file__]):
+        run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_CHECKED_LIB] + bcobjs +
             ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
     torch_src = os.path.join(BLOCKS, "blocks_torch.cpp")
     if _stale(BLOCKS_TORCH, [torch_src, BLOCKS_LIB, __file__] + headers):

@@ -21,7 +21,9 @@ namespace blocks {
 // Every kernel here is launched as a programmatic dependent of the one before it
 // in the stream (launch_pdl): it may be resident before that one has ended, so each
 // calls begin() before it touches global memory, once what its CTA holds on to
-// (TMEM) has been allocated; the next kernel may come then.
+// (TMEM) has been allocated; the next kernel may come then. Loads are ordinary ones:
+// what the kernel before wrote is not read-only for this one's whole life, as
+// __ldg and __restrict__ would have it.
 __device__ __forceinline__ void begin() {
     pdl_trigger();
     pdl_wait();

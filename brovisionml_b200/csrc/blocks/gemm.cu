@@ -98,7 +98,12 @@ Plan plan_of(const GemmLaunch& L) {
     }
 
     p.splits = 1;
-    if (!L.a_t && !L.b_t && L.M <= 128) {
+    // Few rows: the kernel that streams the weights, up to 64 rows, and up to 128 where
+    // the weights are many or gated. us at 128 rows, bf16, that kernel and the tiles: 512 x 512
+    // 8.7 and 6.0, 1024 x 8192 14.6 and 12.8, 8192 x 1024 12.4 and 10.0, but 4096 x 4096 14.9 and
+    // 17.2 (65 rows), 11264 x 4096 27 and 28, gated 44 and 53.
+    const bool many = L.gated || (double)L.N * L.k[0] * (double)es > 20e6;
+    if (!L.a_t && !L.b_t && L.M <= (many ? 128 : 64)) {
         p.skinny = true;
         p.tok = L.M <= 16 ? 16 : L.M <= 32 ? 32 : L.M <= 64 ? 64 : 128;
         const int tiles = cdiv(L.N, L.gated ? 64 : 128);
@@ -159,7 +164,7 @@ Plan plan_of(const GemmLaunch& L) {
 // (8-bit) elements a thread; what pads a row's last unit is zeros.
 template <typename T>
 __global__ void __launch_bounds__(256)
-pack_kernel(const T* __restrict__ src, long long ld, int rows, int cols, T* __restrict__ dst,
+pack_kernel(const T* src, long long ld, int rows, int cols, T* dst,
             int units) {
     constexpr int kE = 16 / sizeof(T);
     const long long total = (long long)rows * units;
@@ -202,7 +207,7 @@ cudaError_t pack(const Stored& s, size_t es, void* ws, cudaStream_t st) {
 // The way back: neighbouring lanes write neighbouring elements.
 template <typename T>
 __global__ void __launch_bounds__(256)
-unpack_kernel(const T* __restrict__ src, long long lds, int rows, int cols, T* __restrict__ dst,
+unpack_kernel(const T* src, long long lds, int rows, int cols, T* dst,
               long long ld) {
     begin();
     for (int r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -229,8 +234,8 @@ cudaError_t unpack(const Moved& m, const void* ws, void* dst, long long ld, int 
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-join_kernel(const float* __restrict__ slab, long long stride, long long lds, int splits, int N,
-            T* __restrict__ out, long long ldo, T* __restrict__ out2, long long ldo2, int rows0,
+join_kernel(const float* slab, long long stride, long long lds, int splits, int N,
+            T* out, long long ldo, T* out2, long long ldo2, int rows0,
             int rows1, bool vec) {
     const long long m = blockIdx.x;
     begin();

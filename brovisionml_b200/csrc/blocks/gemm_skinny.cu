@@ -35,15 +35,15 @@ struct Beside {
 };
 template <bool GATED>
 __device__ __forceinline__ void ask_beside(const TileArgs& a, long long m, int n, Beside& o) {
-    if (a.col_scale[0]) o.rs = __ldg(a.row_scale + m);
+    if (a.col_scale[0]) o.rs = a.row_scale[m];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (n + e >= a.N) break;
         if (a.col_scale[0]) {
-            o.cs[e] = __ldg(a.col_scale[0] + n + e);
-            if (GATED) o.cu[e] = __ldg(a.col_scale[1] + n + e);
+            o.cs[e] = a.col_scale[0][n + e];
+            if (GATED) o.cu[e] = a.col_scale[1][n + e];
         }
-        if (!GATED && a.bias) o.add[e] = __ldg(a.bias + n + e);
+        if (!GATED && a.bias) o.add[e] = a.bias[n + e];
         if (!GATED && a.residual) o.res[e] = get_one(a.residual, m * a.ldr + n + e, a.out_type);
     }
 }
@@ -185,6 +185,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
         tc::mbar_init(bar_acc, 1);
         tc::mbar_fence_init();
     }
+    __syncwarp();
     if (warp == 1) {
         tc::tmem_alloc(tc::smem_u32(tmem_slot), kCols);
         tc::tmem_relinquish();
@@ -210,6 +211,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
             if (!wait_all(bar_empty + 8 * slot, phase, 11)) break;
             tc::mbar_expect_tx_on(on, bar_full + 8 * slot, kStage);
             const uint32_t d = sbase + slot * kStage;
+            if (!tc::copy_ok(d, k * kStep, 128 / kStep, false, 0)) break;
             tc::tma_load_2d(on, d, &maps.b[0], bar_full + 8 * slot, k * kStep, f0);
             if constexpr (GATED)
                 tc::tma_load_2d(on, d + 8192, &maps.b[1], bar_full + 8 * slot, k * kStep, f0);
@@ -242,6 +244,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     // the accumulator, and with it every copy and MMA, is complete
     if (!tc::mbar_wait(bar_acc, 0, kTileWaitLimit)) fail(14);
     __syncthreads();  // ... also the producer's look at its last copies
+    __syncwarp();
     tc::tc_fence_after();
     // partial[token][row]: a lane is a row, so a warp writes 32 neighbours
     float* partial = reinterpret_cast<float*>(smem);
@@ -263,6 +266,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
         tc::tc_fence_before();
     }
     __syncthreads();
+    __syncwarp();
     if (warp == 1) tc::tmem_dealloc(tmem, kCols);
     __syncwarp();
     switch (split) {

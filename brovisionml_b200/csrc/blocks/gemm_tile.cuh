@@ -147,7 +147,7 @@ __device__ __forceinline__ void act_row(float (&v)[kW], int act) {
 __device__ __forceinline__ void load_cols(const float* p, float (&c)[kW]) {
 #pragma unroll
     for (int i = 0; i < kW / 4; ++i) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
+        const float4 f = reinterpret_cast<const float4*>(p)[i];
         c[4 * i] = f.x, c[4 * i + 1] = f.y, c[4 * i + 2] = f.z, c[4 * i + 3] = f.w;
     }
 }
@@ -337,6 +337,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
         tc::tma_prefetch_desc(&maps.a[0]);
         tc::tma_prefetch_desc(&maps.b[0]);
     }
+    __syncwarp();
     if (warp == 1) {
         tc::tmem_alloc_pair(tc::smem_u32(tmem_slot), kCols);
         tc::tmem_relinquish_pair();
@@ -386,6 +387,11 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                 const uint32_t sa = sbase + slot * kStage, sb = sa + 128 * 128;
                 const int seg = k >= a.steps[0];
                 const int x = (k - (seg ? a.steps[0] : 0)) * kStep;
+                if (!tc::copy_ok(sa, AT ? m0 : x, 128 / kStep, false, 0) ||
+                    !tc::copy_ok(sb, BT ? n0 : x, 128 / kStep, false, 0)) {
+                    ok = false;
+                    break;
+                }
                 if constexpr (AT) {
                     tc::tma_load_2d_pair(on, sa, &maps.a[seg], full, m0, x);
                     tc::tma_load_2d_pair(on, sa + 8192, &maps.a[seg], full, m0 + 64, x);
@@ -494,7 +500,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                 if (cols) load_cols(cols + n, cnext);
             };
             if (first < kBoxes) ask(n0 + first * kBox);
-            const float row_scale = F8 && in ? __ldg(a.row_scale + m) : 0.0f;
+            const float row_scale = F8 && in ? a.row_scale[m] : 0.0f;
             const int buf = tl & 1, u = tl >> 1;
             if (!wait_all(bar_acc_full + 8 * buf, u & 1, 6) || gone()) break;
             tc::tc_fence_after();
@@ -536,7 +542,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                     if (!last) ask(n + kW);
                     else if (b + 2 < kBoxes) ask(n0 + (b + 2) * kBox);
                     if (n >= a.N) continue;
-                    if (BT && a.slab) {  // one of several shares of K, its pitch a multiple of 32
+                    if (!GATED && a.slab) {  // one of several shares of K, its pitch a multiple of 32
                         if (in)
                             put_row(a.slab + ((long long)split * a.M + m) * a.ldslab + n, v, true);
                         continue;
@@ -557,14 +563,15 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                     }
                     if (fast) stage_row<T>(box, lane, c / kW, v);
                 }
-                if (!fast || (BT && a.slab)) continue;
+                if (!fast || (!GATED && a.slab)) continue;
                 tc::fence_proxy_async_smem();
                 __syncwarp();
                 const int n = n0 + b * kBox;
                 const bool second = AT && a.out2 && mw >= a.rows1;
                 const int row = second ? mw - a.rows1 : mw;
                 if (lane == 0) {
-                    if (n < a.N && row < a.out_rows)
+                    if (n < a.N && row < a.out_rows &&
+                        tc::copy_ok(tc::smem_u32(box), n, sizeof(T), true, row))
                         tc::tma_store_2d(&maps.o[second], tc::smem_u32(box), n, row);
                     tc::bulk_commit();
                 }
@@ -574,7 +581,6 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
         if (lane == 0) tc::bulk_wait_all();  // before shared memory goes
     }
     __syncthreads();
-    __syncwarp();
     tc::cluster_sync();  // the pair's copies, MMAs and arrivals are all done
     if (warp == 1) tc::tmem_dealloc_pair(tmem, kCols);
     tc::cluster_sync();
@@ -600,12 +606,16 @@ cudaError_t launch_tile(const TileMaps& maps, const TileArgs& a, int pairs, cuda
 }
 
 // Host reader of this translation unit's error word; resets it.
-#define BVML_TILE_ERROR_READER(fn)                                            \
-    cudaError_t fn(int* word) {                                               \
+// Checked builds: or 1000 and what the checks recorded.
+#define BVML_TILE_ERROR_READER(fn)                                             \
+    BVML_CHECK_READER(fn##_checks)                                             \
+    cudaError_t fn(int* word) {                                                \
         cudaError_t e = cudaMemcpyFromSymbol(word, g_tile_error, sizeof(int)); \
-        if (e != cudaSuccess || *word == 0) return e;                         \
-        const int zero = 0;                                                   \
-        return cudaMemcpyToSymbol(g_tile_error, &zero, sizeof(int));          \
+        if (e != cudaSuccess) return e;                                        \
+        const int zero = 0;                                                    \
+        if (*word) e = cudaMemcpyToSymbol(g_tile_error, &zero, sizeof(int));   \
+        if (const unsigned c = fn##_checks(true)) *word = 1000 + (int)c;       \
+        return e;                                                              \
     }
 
 }  // namespace blocks

@@ -468,7 +468,7 @@ rms_norm_backward_long_kernel(const NormBwdArgs a) {
 // 16 columns a block, 32 rows side by side
 template <typename T>
 __global__ void __launch_bounds__(512)
-column_sum_kernel(const float* __restrict__ part, int rows, int cols, T* __restrict__ out) {
+column_sum_kernel(const float* part, int rows, int cols, T* out) {
     __shared__ float sh[32][17];
     const int x = threadIdx.x % 16, c = blockIdx.x * 16 + x, r0 = threadIdx.x / 16;
     begin();

@@ -10,6 +10,7 @@
 // instruction descriptor's transpose bit (15 for A, 16 for B) is set.
 #pragma once
 
+#include "../bvml_common.cuh"
 #include "../tc_common.cuh"
 
 namespace bvml {
@@ -20,9 +21,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// Every thread of the cluster, whole warps. The warps are together before (the aligned
+// forms want that) and after: tcgen05's .sync.aligned instructions and the uniform
+// datapath must not meet a warp whose lanes left a barrier one by one.
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncwarp();
 }
 // The address, in CTA `rank` of the cluster, of this CTA's shared address a.
 __device__ __forceinline__ uint32_t map_to(uint32_t a, uint32_t rank) {
@@ -44,6 +50,14 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote)
                  : "memory");
+}
+
+// Checked builds (-DBVML_CHECKED): a copy whose innermost coordinate or shared-memory
+// address is off its alignment, or a store at a negative coordinate, is recorded and left
+// out. `inner`: bytes of an element.
+__device__ __forceinline__ bool copy_ok(uint32_t smem, int x, int inner, bool store, int y) {
+    return check_ok((smem & 127) == 0 && (x * inner) % 16 == 0 && (!store || (x >= 0 && y >= 0)),
+                    kChkConvTma);
 }
 
 // One lane of the warp, chosen by the hardware. The loops that feed the tensor

@@ -216,6 +216,22 @@ def test_linear(T, K, N, dt, act, bias, res):
     assert torch.equal(bv.linear(x, w, b, act=act, residual=r), y)
 
 
+@pytest.mark.parametrize("T,K,N", [(129, 1536, 200), (200, 2048, 64), (130, 4096, 520),
+                                   (300, 1100, 72), (129, 4096, 4096)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_linear_long_sums(T, K, N, dt):
+    """Few output tiles and a long K, where K is shared out over work items and
+    the shares are joined by a second kernel -- unless there is an epilogue."""
+    x, w, b = rnd(T, K, dt=dt), rnd(N, K, dt=dt, scale=K ** -0.5, seed=1), rnd(N, seed=2)
+    ref, tol = product(x, w)
+    for out in (None, F32):
+        for _ in range(6):  # one after the other, each while the last one ends
+            y = bv.linear(x, w, out_dtype=out)
+        close(y, ref, tol)
+        close(bv.linear(x, w, b, out_dtype=out), ref + b.double(), tol + 4 * E * ref.abs())
+    bv.blocks_status()
+
+
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("out", [None, F32])
 @pytest.mark.parametrize("T", [9, 200])
@@ -641,3 +657,95 @@ def test_python_argument_errors():
         bv.rms_norm(x, rnd(64), x[:2])
     with pytest.raises(RuntimeError, match="share a device"):
         bv.linear(x, w.cpu())
+
+
+def _c_call(lib, name, args):
+    """A C entry point of `lib` with a workspace of its own."""
+    fn, size = getattr(lib, name), getattr(lib, name + "_workspace_bytes")
+    ref = getattr(B.blocks_lib, name)
+    fn.argtypes, fn.restype = ref.argtypes, ref.restype
+    size.argtypes, size.restype = ref.argtypes[:1], ctypes.c_size_t
+    need = size(ctypes.byref(args))
+    ws = torch.empty(max(need, 1), device="cuda", dtype=torch.uint8)
+    assert fn(ctypes.byref(args), ws.data_ptr(), need,
+              torch.cuda.current_stream().cuda_stream) == 0
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 8, 8), (16, 256, 640), (128, 136, 72), (129, 2048, 264),
+                                   (257, 65, 129), (520, 328, 1032)])
+def test_checked_build(T, K, N):
+    """The checked build (every TMA copy's coordinate and address tested before it is
+    issued) records nothing and computes what the release build does."""
+    import os
+
+    path = os.path.join(os.path.dirname(bv.BLOCKS_LIB_PATH), "libbvml_blocks_checked.so")
+    checked = ctypes.CDLL(path)
+    checked.bvml_blocks_status.argtypes = [ctypes.c_void_p]
+    x, w, w2, dy = (rnd(n, c, dt=BF16, seed=s) for s, (n, c) in
+                    enumerate(((T, K), (N, K), (N, K), (T, N))))
+    outs = {}
+    for lib in (B.blocks_lib, checked):
+        y, h, g, u = (torch.empty(T, N, device="cuda", dtype=BF16) for _ in range(4))
+        dx, dw, dg, du = (torch.empty(n, K, device="cuda", dtype=BF16) for n in (T, N, N, N))
+        _c_call(lib, "bvml_linear", B.LinearArgs(
+            x=x.data_ptr(), w=w.data_ptr(), y=y.data_ptr(), ldx=K, ldw=K, ldy=N, T=T, K=K, N=N,
+            in_type=2, out_type=2, act=0))
+        _c_call(lib, "bvml_gated_linear", B.GatedArgs(
+            x=x.data_ptr(), w_gate=w.data_ptr(), w_up=w2.data_ptr(), h=h.data_ptr(),
+            g=g.data_ptr(), u=u.data_ptr(), ldx=K, ldw_gate=K, ldw_up=K, ldh=N, ldg=N, ldu=N,
+            T=T, K=K, F=N, in_type=2, out_type=2, act=4))
+        _c_call(lib, "bvml_linear_backward", B.LinearBackwardArgs(
+            dy=dy.data_ptr(), z=g.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(),
+            dw=dw.data_ptr(), lddy=N, ldz=N, ldx=K, ldw=K, lddx=K, lddw=K, T=T, K=K, N=N, type=2,
+            act=5))
+        dx2 = torch.empty_like(dx)
+        _c_call(lib, "bvml_gated_linear_backward", B.GatedBackwardArgs(
+            dh=dy.data_ptr(), g=g.data_ptr(), u=u.data_ptr(), x=x.data_ptr(),
+            w_gate=w.data_ptr(), w_up=w2.data_ptr(), dx=dx2.data_ptr(), dw_gate=dg.data_ptr(),
+            dw_up=du.data_ptr(), lddh=N, ldg=N, ldu=N, ldx=K, ldw_gate=K, ldw_up=K, lddx=K,
+            lddw_gate=K, lddw_up=K, T=T, K=K, F=N, type=2, act=4))
+        assert lib.bvml_blocks_status(torch.cuda.current_stream().cuda_stream) == 0
+        outs[lib] = (y, h, g, u, dx, dw, dx2, dg, du)
+    assert all(torch.equal(p, q) for p, q in zip(outs[B.blocks_lib], outs[checked]))
+
+
+def test_misaligned_vectors():
+    """A bias and scales that start on no 16 bytes, with few and many rows."""
+    for T in (7, 150):
+        x, w, b = rnd(T, 64, dt=BF16), rnd(96, 64, dt=BF16), rnd(97)
+        ref, tol = product(x, w)
+        close(bv.linear(x, w, b[1:], act="relu"), torch.relu(ref + b[1:].double()),
+              tol + 8 * E * (ref.abs() + 4))
+        (q, s), (v, t) = quantized(T, 64, 0), quantized(96, 64, 1)
+        t1 = torch.cat([t[:1], t])[1:]
+        assert torch.equal(bv.linear(q, v, x_scale=s, w_scale=t1),
+                           bv.linear(q, v, x_scale=s, w_scale=t))
+        assert torch.equal(bv.gated_linear(q, v, v, x_scale=s, gate_scale=t1, up_scale=t),
+                           bv.gated_linear(q, v, v, x_scale=s, gate_scale=t, up_scale=t))
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last rows are what they are alone."""
+    T, K, N = 270_000, 8192, 64
+    x = torch.empty(T, K, device="cuda", dtype=BF16)
+    x[:256] = rnd(256, K, dt=BF16)
+    x[256:-300] = 0
+    x[-300:] = rnd(300, K, dt=BF16, seed=1)
+    w, nw = rnd(N, K, dt=BF16, scale=0.02), rnd(K) + 1
+    assert x.numel() > 2 ** 31
+    y = bv.linear(x, w)
+    # (many rows and few are summed in another order)
+    ref, tol = product(x[-300:], w)
+    close(y[-300:], ref, tol)
+    assert (y[256:-300] == 0).all()
+    n = bv.rms_norm(x, nw)
+    assert torch.equal(n[-300:], bv.rms_norm(x[-300:], nw))
+    assert torch.equal(n[:256], bv.rms_norm(x[:256], nw))
+    dx, _ = bv.rms_norm_backward(n, x, nw)
+    want = bv.rms_norm_backward(n[-300:], x[-300:], nw)[0]
+    assert torch.equal(dx[-300:], want)
+    del dx, n
+    dy = rnd(T, N, dt=BF16, seed=3)
+    dx, _, _ = bv.linear_backward(dy, x, w, dw=False)
+    ref = dy[-300:].double() @ w.double()
+    close(dx[-300:], ref, (N + 4) * 2 * E * (dy[-300:].double().abs() @ w.double().abs()))
