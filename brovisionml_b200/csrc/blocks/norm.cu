@@ -45,13 +45,11 @@ struct NormBwdArgs {
     float eps;
 };
 
-// the larger of two magnitudes, NaN if either is (fmaxf would drop it)
-__device__ __forceinline__ float max_nan(float m, float a) { return (a > m || a != a) ? a : m; }
-
 // From a row's largest |s w| to its scale and to y / scale = s w 448 / max |s w|,
-// from which the root drops out. What the product and the quotient leave over in
-// 32 bits is carried along: a value next to a rounding border of the 8 bits then falls
-// where the formula has it but for the rounding of the largest value itself.
+// from which the root drops out. What the products and the quotient leave over in
+// 32 bits is carried along (`rest` of the largest, `lo` of the quotient): a value
+// next to a rounding border of the 8 bits then falls where the formula has it, but
+// for the one rounding to 32 bits before the one to 8.
 struct Quant {
     float scale, hi, lo;
     __device__ __forceinline__ float operator()(float s, float w) const {
@@ -59,15 +57,27 @@ struct Quant {
         return fmaf(p, hi, fmaf(p, lo, rest * hi));
     }
 };
-__device__ __forceinline__ Quant quant_of(float m, float rstd) {
+__device__ __forceinline__ Quant quant_of(float m, float rest, float rstd) {
     const float top = m * rstd;
     if (top < kTinyMax) return Quant{1.0f, 0.0f, 0.0f};
     Quant f;
     f.scale = top / 448.0f;
     f.hi = m > 1e-30f ? 448.0f / m : rstd * (448.0f / top);  // the quotient must not overflow
-    f.lo = m > 1e-30f ? fmaf(-m, f.hi, 448.0f) / m : 0.0f;
+    f.lo = m > 1e-30f ? (fmaf(-m, f.hi, 448.0f) - rest * f.hi) / m : 0.0f;
     if (top != top) f.hi = top;  // NaN in the row, or an infinity against 1 / infinity
     return f;
+}
+// The larger of two magnitudes, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
+    return a;
+}
+// The largest |s w| so far and what its product left over; NaN stays.
+__device__ __forceinline__ void largest(float s, float w, float& m, float& rest) {
+    const float p = fabsf(s) * fabsf(w), left = fmaf(fabsf(s), fabsf(w), -p);
+    const float n = max_nan(m, p);
+    if (n != m) rest = left;
+    m = n;
 }
 
 // Feature index of element e of group v of lane l: eight consecutive features
@@ -179,17 +189,28 @@ __device__ __forceinline__ void store_row_e4m3(uint8_t* p, int K, int vec, int l
     }
 }
 
-// Sum of a and (MAX) largest of b, or sum of both, over the G threads of a
-// row; every thread gets the result. G > 32: the whole block takes part;
+// Sum of a over the G threads of a row, and of b, or (MAX) the largest b and the c that
+// belongs to it; every thread gets the result. G > 32: the whole block takes part;
 // `slot` alternates between rows, so that one barrier a row is enough.
+template <bool MAX>
+__device__ __forceinline__ void join_pair(float& a, float& b, float& c, float oa, float ob,
+                                          float oc) {
+    a += oa;
+    if constexpr (MAX) {
+        if (ob > b || ob != ob) b = ob, c = oc;
+    } else {
+        b += ob;
+    }
+}
 template <int G, bool MAX>
-__device__ __forceinline__ void row_reduce(float& a, float& b, float (*slots)[2][16], int slot) {
-    constexpr int kW = G < 32 ? G : 32;
+__device__ __forceinline__ void row_reduce(float& a, float& b, float& c, float (*slots)[3][16],
+                                           int slot) {
+    constexpr int kWidth = G < 32 ? G : 32;
 #pragma unroll
-    for (int d = kW / 2; d > 0; d >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, d);
-        const float o = __shfl_xor_sync(0xffffffffu, b, d);
-        b = MAX ? max_nan(b, o) : b + o;
+    for (int d = kWidth / 2; d > 0; d >>= 1) {
+        const float oa = __shfl_xor_sync(0xffffffffu, a, d);
+        const float ob = __shfl_xor_sync(0xffffffffu, b, d);
+        join_pair<MAX>(a, b, c, oa, ob, MAX ? __shfl_xor_sync(0xffffffffu, c, d) : 0.0f);
     }
     if constexpr (G > 32) {
         constexpr int kN = G / 32;
@@ -197,15 +218,16 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float (*slots)[2]
         if ((threadIdx.x & 31) == 0) {
             slots[slot][0][warp] = a;
             slots[slot][1][warp] = b;
+            if (MAX) slots[slot][2][warp] = c;
         }
         __syncthreads();
         a = slots[slot][0][0];
         b = slots[slot][1][0];
+        if (MAX) c = slots[slot][2][0];
 #pragma unroll
-        for (int i = 1; i < kN; ++i) {
-            a += slots[slot][0][i];
-            b = MAX ? max_nan(b, slots[slot][1][i]) : b + slots[slot][1][i];
-        }
+        for (int i = 1; i < kN; ++i)
+            join_pair<MAX>(a, b, c, slots[slot][0][i], slots[slot][1][i],
+                           MAX ? slots[slot][2][i] : 0.0f);
     }
 }
 
@@ -222,7 +244,7 @@ __global__ void __launch_bounds__(G > 32 ? G : kNormThreads, forward_blocks(G, V
 rms_norm_kernel(const NormArgs a) {
     constexpr int kThreads = G > 32 ? G : kNormThreads;
     constexpr int kRows = kThreads / G;
-    __shared__ float slots[2][2][16];
+    __shared__ float slots[2][3][16];
     const int l = threadIdx.x % G, g = threadIdx.x / G;
     begin();
     float w[VPT][8];
@@ -264,20 +286,20 @@ rms_norm_kernel(const NormArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[v][e] = 0.0f;
         }
-        float q = 0.0f, m = 0.0f;
+        float q = 0.0f, m = 0.0f, rest = 0.0f;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 q = fmaf(s[v][e], s[v][e], q);
-                if constexpr (Q) m = max_nan(m, fabsf(s[v][e] * w[v][e]));
+                if constexpr (Q) largest(s[v][e], w[v][e], m, rest);
             }
         }
-        row_reduce<G, true>(q, m, slots, slot);
+        row_reduce<G, Q>(q, m, rest, slots, slot);
         if (!in) continue;
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         if constexpr (Q) {
-            const Quant f = quant_of(m, rstd);
+            const Quant f = quant_of(m, rest, rstd);
             if (l == 0) a.scale[t] = f.scale;
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
@@ -298,7 +320,7 @@ rms_norm_kernel(const NormArgs a) {
 template <typename T, bool Q>
 __global__ void __launch_bounds__(kLongThreads)
 rms_norm_long_kernel(const NormArgs a) {
-    __shared__ float slots[2][2][16];
+    __shared__ float slots[2][3][16];
     begin();
     const float inv_k = 1.0f / (float)a.K;
     int slot = 0;
@@ -308,18 +330,18 @@ rms_norm_long_kernel(const NormArgs a) {
     for (long long t = blockIdx.x; t < a.T; t += gridDim.x, slot ^= 1) {
         const T* x = static_cast<const T*>(a.x) + t * a.ldx;
         const T* r = a.r ? static_cast<const T*>(a.r) + t * a.ldr : nullptr;
-        float q = 0.0f, m = 0.0f;
+        float q = 0.0f, m = 0.0f, rest = 0.0f;
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
             const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
             if (a.sum) static_cast<T*>(a.sum)[t * a.lds + k] = from_f<T>(s);
             q = fmaf(s, s, q);
-            if constexpr (Q) m = max_nan(m, fabsf(s * wt(k)));
+            if constexpr (Q) largest(s, wt(k), m, rest);
         }
-        row_reduce<kLongThreads, true>(q, m, slots, slot);
+        row_reduce<kLongThreads, Q>(q, m, rest, slots, slot);
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         Quant f{};
         if constexpr (Q) {
-            f = quant_of(m, rstd);
+            f = quant_of(m, rest, rstd);
             if (threadIdx.x == 0) a.scale[t] = f.scale;
         }
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
@@ -343,7 +365,7 @@ __global__ void __launch_bounds__(G > 32 ? G : kNormThreads, backward_blocks(G, 
 rms_norm_backward_kernel(const NormBwdArgs a) {
     constexpr int kThreads = G > 32 ? G : kNormThreads;
     constexpr int kRows = kThreads / G;
-    __shared__ float slots[2][2][16];
+    __shared__ float slots[2][3][16];
     __shared__ float part[kRows > 1 ? kThreads * VPT * 8 : 1];
     const int l = threadIdx.x % G, g = threadIdx.x / G;
     begin();
@@ -380,7 +402,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[v][e] = dy[v][e] = 0.0f;
         }
-        float q = 0.0f, p = 0.0f;
+        float q = 0.0f, p = 0.0f, none = 0.0f;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
 #pragma unroll
@@ -389,7 +411,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
                 p = fmaf(dy[v][e] * w[v][e], s[v][e], p);
             }
         }
-        row_reduce<G, false>(q, p, slots, slot);
+        row_reduce<G, false>(q, p, none, slots, slot);
         if (!in) continue;
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         const float c = p * inv_k * rstd * rstd;
@@ -433,7 +455,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads)
 rms_norm_backward_long_kernel(const NormBwdArgs a) {
-    __shared__ float slots[2][2][16];
+    __shared__ float slots[2][3][16];
     begin();
     const float inv_k = 1.0f / (float)a.K;
     float* out = a.partial + (long long)blockIdx.x * a.K;
@@ -445,13 +467,13 @@ rms_norm_backward_long_kernel(const NormBwdArgs a) {
     for (long long t = blockIdx.x; t < a.T; t += gridDim.x, slot ^= 1) {
         const T* s = static_cast<const T*>(a.s) + t * a.lds;
         const T* dy = static_cast<const T*>(a.dy) + t * a.lddy;
-        float q = 0.0f, p = 0.0f;
+        float q = 0.0f, p = 0.0f, none = 0.0f;
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
             const float sv = to_f(s[k]);
             q = fmaf(sv, sv, q);
             p = fmaf(to_f(dy[k]) * wt(k), sv, p);
         }
-        row_reduce<kLongThreads, false>(q, p, slots, slot);
+        row_reduce<kLongThreads, false>(q, p, none, slots, slot);
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         const float c = p * inv_k * rstd * rstd;
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
