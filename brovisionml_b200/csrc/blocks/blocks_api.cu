@@ -115,6 +115,15 @@ int check_workspace(const char* op, const void* ws, size_t have, size_t need) {
     return BVML_OK;
 }
 
+// The kernels' indexes are 32 bits past the last tile, their count of tiles too.
+// (2^44 elements are 32 TB: no matrix that exists is refused by the product.)
+constexpr int kMostRows = (1 << 30) - 64;
+bool shape_ok(int T, int K, int N = 1) {
+    auto size = [](int a, int b) { return (long long)a * b <= 1LL << 44; };
+    return T >= 0 && K >= 1 && N >= 1 && T <= kMostRows && K <= kMostRows && N <= kMostRows &&
+           size(T, K) && size(T, N) && size(N, K);
+}
+
 bool type16(int t) { return t == BVML_F16 || t == BVML_BF16; }
 bool act_ok(int act) { return act >= BVML_ACT_NONE && act <= BVML_ACT_GELU; }
 
@@ -128,7 +137,7 @@ int norm_entry(const char* op, const void* x, long long ldx, const void* r, long
     if (type != BVML_F32 && !type16(type)) return einval(op, "rows must be fp32, fp16 or bf16");
     if (wtype != BVML_F32 && wtype != type)
         return einval(op, "weights must be fp32 or of the rows' type");
-    if (T < 0 || K < 1) return einval(op, "bad shape");
+    if (!shape_ok(T, K)) return einval(op, "bad shape");
     if (!(eps >= 0.0f)) return einval(op, "eps must not be negative");
     if (!w) return einval(op, "weight is null");
     if (sum && !r) return einval(op, "the sum is an output of the residual's addition");
@@ -147,7 +156,7 @@ int norm_entry(const char* op, const void* x, long long ldx, const void* r, long
 }
 
 size_t norm_backward_bytes(int T, int K) {
-    return T < 0 || K < 1 ? 0 : round256((size_t)norm_backward_parts(T, K) * K * 4);
+    return !shape_ok(T, K) ? 0 : round256((size_t)norm_backward_parts(T, K) * K * 4);
 }
 
 // ------------------------------------------------------------------ products
@@ -283,7 +292,7 @@ cudaError_t zero_rows(void* p, long long ld, int rows, int cols, size_t es, cuda
 int check_linear(const bvml_linear_args* a) {
     const char* op = "linear";
     if (!a) return einval(op, "no arguments");
-    if (a->T < 0 || a->K < 1 || a->N < 1) return einval(op, "bad shape");
+    if (!shape_ok(a->T, a->K, a->N)) return einval(op, "bad shape");
     if (const char* e = forward_types(a->in_type, a->out_type, a->x_scale, a->w_scale, a->w_scale))
         return einval(op, e);
     if (a->in_type != BVML_E4M3 && (a->x_scale || a->w_scale))
@@ -305,7 +314,7 @@ int check_linear(const bvml_linear_args* a) {
 int check_gated(const bvml_gated_args* a) {
     const char* op = "gated_linear";
     if (!a) return einval(op, "no arguments");
-    if (a->T < 0 || a->K < 1 || a->F < 1) return einval(op, "bad shape");
+    if (!shape_ok(a->T, a->K, a->F)) return einval(op, "bad shape");
     if (const char* e =
             forward_types(a->in_type, a->out_type, a->x_scale, a->gate_scale, a->up_scale))
         return einval(op, e);
@@ -330,7 +339,7 @@ int check_gated(const bvml_gated_args* a) {
 int check_linear_backward(const bvml_linear_backward_args* a) {
     const char* op = "linear_backward";
     if (!a) return einval(op, "no arguments");
-    if (a->T < 0 || a->K < 1 || a->N < 1) return einval(op, "bad shape");
+    if (!shape_ok(a->T, a->K, a->N)) return einval(op, "bad shape");
     if (!type16(a->type)) return einval(op, "matrices must be fp16 or bf16");
     if (!act_ok(a->act)) return einval(op, "unknown activation");
     if (a->act == BVML_ACT_NONE && a->z) return einval(op, "z belongs to an activation");
@@ -348,7 +357,7 @@ int check_linear_backward(const bvml_linear_backward_args* a) {
 int check_gated_backward(const bvml_gated_backward_args* a) {
     const char* op = "gated_linear_backward";
     if (!a) return einval(op, "no arguments");
-    if (a->T < 0 || a->K < 1 || a->F < 1 || a->F > (1 << 30) - 64) return einval(op, "bad shape");
+    if (!shape_ok(a->T, a->K, a->F)) return einval(op, "bad shape");
     if (!type16(a->type)) return einval(op, "matrices must be fp16 or bf16");
     if (!act_ok(a->act) || a->act == BVML_ACT_NONE) return einval(op, "unknown activation");
     if (!a->dw_gate != !a->dw_up) return einval(op, "dw_gate and dw_up are computed together");
@@ -413,7 +422,7 @@ int bvml_rms_norm_backward(const void* dy, long long lddy, const void* s, long l
     if (dtype != BVML_F32 && !type16(dtype)) return einval(op, "rows must be fp32, fp16 or bf16");
     if (weight_dtype != BVML_F32 && weight_dtype != dtype)
         return einval(op, "weights must be fp32 or of the rows' type");
-    if (T < 0 || K < 1) return einval(op, "bad shape");
+    if (!shape_ok(T, K)) return einval(op, "bad shape");
     if (!(eps >= 0.0f)) return einval(op, "eps must not be negative");
     const size_t es = elem_size(dtype), ew = elem_size(weight_dtype);
     Mats in, out;

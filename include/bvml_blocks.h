@@ -10,7 +10,11 @@
  *    a pointer and a row stride `ld` in elements (>= the columns); its last
  *    axis is contiguous. Pointers are aligned to their element. Rows that
  *    start on 16 bytes (pointer and stride) are read in place; others are
- *    accepted and laid out anew in the workspace first.
+ *    accepted and laid out anew in the workspace first. Outputs of the
+ *    products whose rows do not start and end on 16 bytes likewise go through
+ *    the workspace. The *_workspace_bytes calls look at the pointers'
+ *    alignment, so they take the arguments of the call itself.
+ *  - A dimension is at most 2^30 - 64.
  *  - Types: BVML_F32, BVML_F16 (bvml_dsine.h), BVML_BF16, BVML_E4M3. Sums and
  *    statistics are 32-bit; results are rounded once, to nearest.
  *  - `stream` is a cudaStream_t (NULL = the legacy default stream). Calls are
@@ -57,7 +61,8 @@ int bvml_blocks_version(void);
  * Waits inside the matrix-product kernels are bounded; one that gives up (the
  * GPU stopped making progress) is recorded per device instead of hanging, and
  * the results of that call are unspecified. Synchronises `stream`, returns
- * BVML_OK, or BVML_ECUDA once for what was recorded since the last call.
+ * BVML_OK, or BVML_ECUDA once for what was recorded since the last call. Not for a
+ * stream that is being captured.
  */
 int bvml_blocks_status(void* stream);
 

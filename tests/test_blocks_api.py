@@ -232,6 +232,31 @@ def test_norm_scale_and_backward_refusals():
     assert rc == EINVAL and "dx overlaps s" in err()
 
 
+def test_sizes_past_the_indexes_are_refused():
+    """Shapes beyond 32-bit indexes or counts of tiles: refused, and no workspace is named."""
+    lib, most = B.blocks_lib, (1 << 30) - 64
+    for kw in (dict(T=most + 1), dict(K=most + 1), dict(N=2**31 - 1), dict(T=1 << 25, N=1 << 25)):
+        kw = dict(ldx=1 << 31, ldw=1 << 31, ldy=1 << 31, ldz=1 << 31) | kw
+        a = linear_args(**kw)
+        assert lib.bvml_linear(ctypes.byref(a), None, 0, None) == EINVAL and "bad shape" in err()
+        assert lib.bvml_linear_workspace_bytes(ctypes.byref(a)) == 0
+        a = linear_backward_args(**kw)
+        assert lib.bvml_linear_backward(ctypes.byref(a), None, 0, None) == EINVAL
+        assert "bad shape" in err()
+        assert lib.bvml_linear_backward_workspace_bytes(ctypes.byref(a)) == 0
+        kw = {("F" if k == "N" else k): v for k, v in kw.items() if k[:2] != "ld"}
+        a = gated_args(**kw)
+        assert lib.bvml_gated_linear(ctypes.byref(a), None, 0, None) == EINVAL
+        assert "bad shape" in err()
+        a = gated_backward_args(**kw)
+        assert lib.bvml_gated_linear_backward(ctypes.byref(a), None, 0, None) == EINVAL
+        assert "bad shape" in err()
+    for T, K in ((most + 1, 64), (16, 2**31 - 1)):
+        assert lib.bvml_rms_norm(at(0), 1 << 31, None, 0, at(1), T, K, BF16, F32, 1e-6, at(2),
+                                 1 << 31, None, 0, None) == EINVAL and "bad shape" in err()
+        assert lib.bvml_rms_norm_backward_workspace_bytes(T, K) == 0
+
+
 def test_python_refusals():
     x, w = torch.zeros(4, 8), torch.zeros(6, 8)
     with pytest.raises(RuntimeError, match="dsine ops: linear: .*CUDA-resident"):
