@@ -54,13 +54,16 @@ int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 // that the pairs take, times the longer of a tile's K steps and its epilogue. Both were
 // measured: a step takes as long as its operands take to arrive, (128 + bn / 2) rows a
 // CTA, whatever the tensor cores need for a narrower tile (8192 x 4096 x 8192: 310 us
-// with 256 columns); an epilogue 0.054 steps a column and one more a tile (57600 x 128
-// -> 576: 36 us with 192 columns, 44 with 256). Shares of K are written and read once
-// more (6.5 TB/s), which fewer idle pairs have to earn back.
-double tile_cost(int tiles, int steps, int splits, int bn, double outputs) {
+// with 256 columns). An epilogue of scales and biases at most (`light`) takes 0.027 steps a
+// column and 0.7 more a tile (57600 x 128 -> 1024: 32.8, 33.8, 34.4 and 38.4 us with 256,
+// 192, 128 and 64 columns; -> 576: 25.9, 20.7, 23.7 and 23.8), any other twice that.
+// Shares of K are written and read once more (6.5 TB/s), which fewer idle pairs have to
+// earn back.
+double tile_cost(int tiles, int steps, int splits, int bn, double outputs, bool light) {
     const double rate = (128 + bn / 2) / 256.0;
     const long long turns = ((long long)tiles * splits + kPairs - 1) / kPairs;
-    const double main = rate * steps / splits, epilogue = 0.054 * bn + 1.0;
+    const double main = rate * steps / splits;
+    const double epilogue = light ? 0.027 * bn + 0.7 : 0.054 * bn + 1.0;
     const double join = splits > 1 ? 7.0 + outputs * (6.0 * splits + 2.0) / 6.5e6 / 0.3 : 0.0;
     return turns * (main > epilogue ? main : epilogue) + epilogue + join;
 }
@@ -115,16 +118,16 @@ Plan plan_of(const GemmLaunch& L) {
         return p;
     }
     p.tiles_m = cdiv(L.M, 256);
-    // K is shared out only where nothing but the sum is wanted (the gradients):
-    // long sums over few output tiles
-    const bool plain = !L.gated && !L.bias && !L.residual && !L.save[0] && !L.row_scale &&
-                       L.act == BVML_ACT_NONE;
+    // K is shared out only where nothing but the sum is wanted: long sums over few
+    // output tiles
+    const bool light = !L.gated && !L.residual && !L.save[0] && L.act == BVML_ACT_NONE;
+    const bool plain = light && !L.bias && !L.row_scale;
     double best = 1e300;
     const bool halves = L.gated || L.b_t;  // 256 and 128 columns only
     for (int bn = 256; bn >= (halves ? 128 : 64); bn -= halves ? 128 : 64) {
         const int tn = cdiv(L.N, L.gated ? bn / 2 : bn);
         for (int sp = 1; sp <= (plain ? 32 : 1) && (sp == 1 || steps / sp >= 8); sp *= 2) {
-            const double c = tile_cost(p.tiles_m * tn, steps, sp, bn, (double)L.M * L.N);
+            const double c = tile_cost(p.tiles_m * tn, steps, sp, bn, (double)L.M * L.N, light);
             if (c < best * 0.999) {
                 best = c;
                 p.bn = bn;

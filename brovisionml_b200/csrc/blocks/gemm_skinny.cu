@@ -193,7 +193,15 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    begin();
+    pdl_trigger();
+    if (warp == 0) {
+        const uint32_t on = tc::elect_one();
+        for (int k = k0; k < k1 && k < k0 + kStages; ++k) {
+            tc::tma_prefetch_2d(on, &maps.b[0], k * kStep, f0);
+            if constexpr (GATED) tc::tma_prefetch_2d(on, &maps.b[1], k * kStep, f0);
+        }
+    }
+    pdl_wait();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     auto fail = [&](int code) { atomicExch(&g_tile_error, code); };

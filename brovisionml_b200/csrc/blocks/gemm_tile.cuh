@@ -69,8 +69,8 @@ template <int BN> constexpr int tile_smem_bytes() {
 // A lane finishes kW consecutive columns of one row at a time, as they lie in TMEM. The
 // output goes through shared memory: a warp's 32 rows x 128 bytes in the 128-byte
 // swizzle, written to global memory by one TMA store, whole lines at a time and
-// clipped at the edges (stores from registers, 32 bytes of 32 rows each, kept 16 warps
-// waiting 15 us of 44 on 57600 x 128 -> 576, and 8 warps 3 of 34). What a launch's
+// clipped at the edges (stores from registers, 32 bytes of 32 rows each, cost 57600 x
+// 128 -> 576 3 us). What a launch's
 // kernel cannot meet is left out at compile time and what is rare stands out of line:
 // a short K's epilogue is long beside its MMAs.
 constexpr int kW = 16;
@@ -285,7 +285,7 @@ __device__ __forceinline__ void load_some(const float* p, int at, int end, float
 
 // A whole box (32 rows x 128 bytes of output) of a product whose epilogue is scales and
 // biases at most, rows on 16 bytes: all its columns at once, without the chunks' loop.
-// 57600 x 128 -> 576: xx us, by chunks 32. read(): called when TMEM has been read.
+// 57600 x 128 -> 576: 21 us, by chunks 32. read(): called when TMEM has been read.
 template <bool F8, bool GRAD, int OUT, typename Read>
 __device__ __forceinline__ void plain_box(const TileArgs& a, uint32_t acc, int n, float row_scale,
                                           uint8_t* box, int lane, Read read) {

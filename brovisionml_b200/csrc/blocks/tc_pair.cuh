@@ -92,6 +92,18 @@ __device__ __forceinline__ void tma_load_2d(uint32_t on, uint32_t dst, const CUt
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(on)
         : "memory");
 }
+// Towards L2 only: nothing waits for it, and what another kernel writes there
+// meanwhile is seen by the load that follows.
+__device__ __forceinline__ void tma_prefetch_2d(uint32_t on, const CUtensorMap* map, int c0,
+                                                int c1) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "@q cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n\t}" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(c0), "r"(c1), "r"(on)
+        : "memory");
+}
 // The same, its bytes counted on a barrier of either CTA of the pair (`bar` a
 // shared::cluster address).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t on, uint32_t dst,
