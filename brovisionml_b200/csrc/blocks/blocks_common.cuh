@@ -77,13 +77,22 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     }
 }
 
-// sigmoid: exp overflows to infinity for z below -88, where 1 / inf = 0 is the
-// value. The fast exponential and division: a relative error of a few 2^-24 and
-// |z| 2^-24 (on what is rounded to 16 bits as a rule), in a third of the
-// instructions, which bound the elementwise kernels.
-__device__ __forceinline__ float sigmoid_f(float z) {
-    return __fdividef(1.0f, 1.0f + __expf(-z));
+// The hardware's 2^x and 1 / x, results below 2^-126 flushed to zero: what is added
+// to 1 or rounded to 16 bits next loses nothing by it, and the instructions that
+// subnormal results would take bound the elementwise kernels.
+__device__ __forceinline__ float ex2(float x) {
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+    return x;
 }
+__device__ __forceinline__ float rcp(float x) {
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+    return x;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+// sigmoid: exp overflows to infinity for z below -88, where 1 / inf = 0 is the
+// value. A relative error of a few 2^-24 and |z| 2^-24, on what is rounded to 16
+// bits as a rule.
+__device__ __forceinline__ float sigmoid_f(float z) { return rcp(1.0f + ex2(-kLog2E * z)); }
 
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
@@ -95,8 +104,8 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 // is smooth in t on (0, 1]: a polynomial of degree 8, fitted here for the least relative
 // error (2e-8 in exact arithmetic; in fp32 6e-7 of Phi for |z| < 4).
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
-    const float t = __fdividef(1.0f, fmaf(0.3f * kSqrtHalf, fabsf(z), 1.0f));
-    e = __expf(-0.5f * z * z);
+    const float t = rcp(fmaf(0.3f * kSqrtHalf, fabsf(z), 1.0f));
+    e = ex2(-0.5f * kLog2E * z * z);
     float q = -0.12952278554439545f;
     q = fmaf(q, t, 0.48556262254714966f);
     q = fmaf(q, t, -0.5122768878936768f);

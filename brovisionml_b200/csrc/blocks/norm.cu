@@ -13,6 +13,10 @@
 // time out of L2. A block keeps its weights in registers over its rows, and the
 // backward pass its sums of dw, which it writes once: the sums over blocks
 // are a second small kernel, in a fixed order (no atomics).
+//
+// us (TB/s): 57600 x 128 fp16 6.7 (4.4), 8197 x 4096 bf16 with residual to 8 bits 41 - 45
+// (5.2 - 5.7), backward 16384 x 2048 bf16 52.6 (5.1, the second kernel included); one row
+// of 4096 5.0, the launch.
 #include "blocks_common.cuh"
 #include "blocks_internal.h"
 
