@@ -14,7 +14,7 @@
 // backward pass its sums of dw, which it writes once: the sums over blocks
 // are a second small kernel, in a fixed order (no atomics).
 //
-// us (TB/s): 57600 x 128 fp16 6.7 (4.4), 8197 x 4096 bf16 with residual to 8 bits 41 - 45
+// us (TB/s): 57600 x 128 fp16 6.6 (4.5; sums of squares and of the residual in pairs, 6.85 one by one), 8197 x 4096 bf16 with residual to 8 bits 41 - 45
 // (5.2 - 5.7), backward 16384 x 2048 bf16 52.6 (5.1, the second kernel included); one row
 // of 4096 5.0, the launch.
 #include "blocks_common.cuh"
@@ -280,7 +280,11 @@ rms_norm_kernel(const NormArgs a) {
 #pragma unroll
                 for (int v = 0; v < VPT; ++v)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) s[v][e] += r[v][e];
+                    for (int e = 0; e < 8; e += 2) {
+                        const float2 d = __fadd2_rn(make_float2(s[v][e], s[v][e + 1]),
+                                                    make_float2(r[v][e], r[v][e + 1]));
+                        s[v][e] = d.x, s[v][e + 1] = d.y;
+                    }
             }
             ask(t + stride);
             if (a.sum) store_row<T, G, VPT>(static_cast<T*>(a.sum) + t * a.lds, a.K, a.vec, l, s);
@@ -290,15 +294,20 @@ rms_norm_kernel(const NormArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[v][e] = 0.0f;
         }
-        float q = 0.0f, m = 0.0f, rest = 0.0f;
+        float2 q2 = make_float2(0.0f, 0.0f);
+        float m = 0.0f, rest = 0.0f;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                q = fmaf(s[v][e], s[v][e], q);
+                if (e % 2 == 0) {
+                    const float2 d = make_float2(s[v][e], s[v][e + 1]);
+                    q2 = __ffma2_rn(d, d, q2);
+                }
                 if constexpr (Q) largest(s[v][e], w[v][e], m, rest);
             }
         }
+        float q = q2.x + q2.y;
         row_reduce<G, Q>(q, m, rest, slots, slot);
         if (!in) continue;
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
