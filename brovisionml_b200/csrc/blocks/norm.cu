@@ -14,9 +14,10 @@
 // backward pass its sums of dw, which it writes once: the sums over blocks
 // are a second small kernel, in a fixed order (no atomics).
 //
-// us (TB/s): 57600 x 128 fp16 6.6 (4.5; sums of squares and of the residual in pairs, 6.85 one by one), 8197 x 4096 bf16 with residual to 8 bits 41 - 45
-// (5.2 - 5.7), backward 16384 x 2048 bf16 52.6 (5.1, the second kernel included); one row
-// of 4096 5.0, the launch.
+// us (TB/s): 57600 x 128 fp16 6.6 (4.5; 6.85 with sums of squares and of the residual
+// element by element and not in pairs), 8197 x 4096 bf16 with residual to 8 bits 41 to
+// 45 (5.2 to 5.7; in pairs its quotients took 2 us longer), backward 16384 x 2048 bf16
+// 52.6 (5.1, the second kernel included); one row of 4096 5.0, the launch.
 #include "blocks_common.cuh"
 #include "blocks_internal.h"
 
