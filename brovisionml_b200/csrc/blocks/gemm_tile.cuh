@@ -130,13 +130,14 @@ __device__ __forceinline__ void stage_row(uint8_t* buf, int r, int c, const floa
     }
 }
 
-__device__ __forceinline__ void act_row(float (&v)[kW], int act) {
+template <int n>
+__device__ __forceinline__ void act_row(float (&v)[n], int act) {
     if (act == BVML_ACT_NONE) return;
     // the switch outside the loop: the activation is the same for the whole launch
     switch (act) {
 #define BVML_ACT_ROW(code)                                                  \
     case code:                                                              \
-        _Pragma("unroll") for (int i = 0; i < kW; ++i) v[i] = act_f(v[i], code); \
+        _Pragma("unroll") for (int i = 0; i < n; ++i) v[i] = act_f(v[i], code); \
         break;
         BVML_ACT_ROW(BVML_ACT_RELU)
         BVML_ACT_ROW(BVML_ACT_SIGMOID)
@@ -288,11 +289,13 @@ __device__ __forceinline__ void load_some(const float* p, int at, int end, float
     }
 }
 
-// A whole box (32 rows x 128 bytes of output) of a product whose epilogue is scales and
-// biases at most, rows on 16 bytes: all its columns at once, without the chunks' loop.
-// 57600 x 128 -> 576: 21 us, by chunks 32. read(): called when TMEM has been read.
+// A whole box (32 rows x 128 bytes of output) of a product that is not gated, adds no
+// residual and keeps nothing, rows on 16 bytes: all its columns at once, without the
+// chunks' loop. us, and by chunks: 57600 x 128 -> 576 21.8 (32), with relu 25 (38.5), gelu
+// 49 (58). A residual's rows hold it back: 55 (57). read(): called when TMEM has been
+// read.
 template <bool F8, bool GRAD, int OUT, typename Read>
-__device__ __forceinline__ void plain_box(const TileArgs& a, uint32_t acc, int n, float row_scale,
+__device__ __forceinline__ void whole_box(const TileArgs& a, uint32_t acc, int n, float row_scale,
                                           uint8_t* box, int lane, Read read) {
     using T = typename OutOf<OUT>::T;
     constexpr int kBox = 128 / sizeof(T);
@@ -318,6 +321,7 @@ __device__ __forceinline__ void plain_box(const TileArgs& a, uint32_t acc, int n
             for (int i = 0; i < kBox; ++i) v[i] += c[i];
         }
     }
+    if constexpr (!GRAD) act_row(v, a.act);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         uint4 w;
@@ -544,10 +548,9 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
         const uint32_t acc_empty0 = tc::map_to(bar_acc_empty, 0);
         // rows on 16 bytes take the short path
         const bool fast = (a.vec & kOn16) != 0;
-        const bool plain = !GATED && fast && !a.slab && !a.save[0] && !a.residual &&
-                           a.act == BVML_ACT_NONE;
+        const bool whole = !GATED && fast && !a.slab && !a.save[0] && !a.residual;
         const bool ahead = !GATED && !BT && fast && a.residual;
-        const float* cols = !fast || BT || plain ? nullptr : F8 ? a.col_scale[0] : a.bias;
+        const float* cols = !fast || BT || whole ? nullptr : F8 ? a.col_scale[0] : a.bias;
         int tl = 0;
         for (int w = pair; w < works; w += pairs, ++tl) {
             int m0, n0, k0, k1, split;
@@ -583,11 +586,12 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                 // the store that last read this buffer has done so
                 if (lane == 0) tc::bulk_wait_read<kBufs - 1>();
                 __syncwarp();
-                if (!GATED && plain)
-                    plain_box<F8, BT, OUT>(a, acc + b * kBox, n0 + b * kBox, row_scale, box, lane,
-                                           [&]() { if (b + 2 >= kBoxes) hand_back(); });
+                const bool done = b + 2 >= kBoxes;
+                if (!GATED && whole)
+                    whole_box<F8, BT, OUT>(a, acc + b * kBox, n0 + b * kBox, row_scale, box, lane,
+                                           [&]() { if (done) hand_back(); });
 #pragma unroll 1
-                for (int c = 0; c < kBox && !plain; c += kW) {
+                for (int c = 0; c < kBox && !whole; c += kW) {
                     const int n = n0 + b * kBox + c;
                     float v[kW], g[GATED ? kW : 1], cnow[kW];
                     __syncwarp();  // lanes may have gone different ways
@@ -604,12 +608,12 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                         }
                     }
                     const bool last = c + kW == kBox;
-                    if (last && b + 2 >= kBoxes) hand_back();
+                    if (last && done) hand_back();
 #pragma unroll
                     for (int i = 0; i < kW; ++i) cnow[i] = cnext[i];
                     const RawRow<T> now = raw;
                     if (!last) ask(n + kW);
-                    else if (b + 2 < kBoxes) ask(n0 + (b + 2) * kBox);
+                    else if (!done) ask(n0 + (b + 2) * kBox);
                     if (n >= a.N) continue;
                     if (!GATED && a.slab) {  // one of several shares of K, its pitch a multiple of 32
                         if (in)
