@@ -244,6 +244,23 @@ def test_linear_activations(act, out, T):
     close(y, val, 1.13 * tol + 32 * E * (ref.abs() + 1))
 
 
+@pytest.mark.parametrize("T,K,N", [(129, 64, 8), (200, 72, 200), (300, 128, 584), (513, 200, 264),
+                                   (140, 65, 131)])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "tanh"])
+@pytest.mark.parametrize("dt,out", [(BF16, None), (F16, None), (F16, F32)])
+def test_linear_bias_activation_edges(T, K, N, act, dt, out):
+    """A bias and an activation without a residual, output widths that end inside a tile's
+    store, with and without the pre-activation kept."""
+    x, w = rnd(T, K, dt=dt), rnd(N, K, dt=dt, scale=K ** -0.5, seed=1)
+    b = rnd(N, seed=2)
+    ref, tol = product(x, w)
+    ref = ref + b.double()
+    val = ACTS[act][0](ref)
+    bound = 1.13 * tol + 16 * E * (ref.abs() + val.abs() + 1)
+    close(bv.linear(x, w, b, act=act, out_dtype=out), val, bound)
+    close(bv.linear(x, w, b, act=act, out_dtype=out, save=True)[0], val, bound)
+
+
 def quantized(n, k, seed, scale=1.0):
     q, s = bv.pack_weight_e4m3(rnd(n, k, scale=scale, seed=seed))
     return q, s
