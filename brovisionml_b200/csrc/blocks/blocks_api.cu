@@ -209,10 +209,11 @@ GemmLaunch grad_w_gemm(const void* dz, long long lddz, const void* x, long long 
     return L;
 }
 
-const char* forward_types(int in_type, int out_type, const void* xs, const void* ws0,
+// An empty batch's row scales may be null, as its rows may.
+const char* forward_types(int in_type, int out_type, int T, const void* xs, const void* ws0,
                           const void* ws1) {
     if (in_type == BVML_E4M3) {
-        if (!xs || !ws0 || !ws1) return "e4m3 inputs need their scales";
+        if ((!xs && T > 0) || !ws0 || !ws1) return "e4m3 inputs need their scales";
         if (!type16(out_type) && out_type != BVML_F32) return "output must be fp16, bf16 or fp32";
         return nullptr;
     }
@@ -293,7 +294,8 @@ int check_linear(const bvml_linear_args* a) {
     const char* op = "linear";
     if (!a) return einval(op, "no arguments");
     if (!shape_ok(a->T, a->K, a->N)) return einval(op, "bad shape");
-    if (const char* e = forward_types(a->in_type, a->out_type, a->x_scale, a->w_scale, a->w_scale))
+    if (const char* e =
+            forward_types(a->in_type, a->out_type, a->T, a->x_scale, a->w_scale, a->w_scale))
         return einval(op, e);
     if (a->in_type != BVML_E4M3 && (a->x_scale || a->w_scale))
         return einval(op, "scales belong to e4m3 inputs");
@@ -316,7 +318,7 @@ int check_gated(const bvml_gated_args* a) {
     if (!a) return einval(op, "no arguments");
     if (!shape_ok(a->T, a->K, a->F)) return einval(op, "bad shape");
     if (const char* e =
-            forward_types(a->in_type, a->out_type, a->x_scale, a->gate_scale, a->up_scale))
+            forward_types(a->in_type, a->out_type, a->T, a->x_scale, a->gate_scale, a->up_scale))
         return einval(op, e);
     if (a->in_type != BVML_E4M3 && (a->x_scale || a->gate_scale || a->up_scale))
         return einval(op, "scales belong to e4m3 inputs");
