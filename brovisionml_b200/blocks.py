@@ -71,7 +71,8 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     """rms_norm with y in 8 bits, as ``linear`` and ``gated_linear`` take it:
     (q, scale) or, with a residual, (q, scale, s); q (..., K) float8_e4m3fn, scale (...)
     fp32, y ~ q * scale[..., None]. The row's largest magnitude becomes 448
-    (scale 1 for a row of zeros; a row with NaN or infinities has a NaN scale)."""
+    (zeros and scale 1 where that magnitude is below 2^-110; a row with NaN or infinities has
+    a NaN scale)."""
     return _binding.rms_norm_e4m3(x, weight, residual, eps)
 
 

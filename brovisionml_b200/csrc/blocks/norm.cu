@@ -27,8 +27,13 @@ namespace {
 
 constexpr int kNormThreads = 256;  // rows of at most a warp share a block of this size
 constexpr int kLongThreads = 512;
-// Below this a row's largest value counts as zero: 448 / max would overflow.
-constexpr float kTinyMax = 7.7e-34f;  // 2^-110
+// Below this a row's largest |y| counts as zero (its scale would come near the smallest
+// normal numbers).
+constexpr float kTinyMax = 0x1p-110f;
+// Rows whose largest |s w| is below kSmallMax are lifted by a power of two on their way to
+// 8 bits: 448 / max |s w| would overflow.
+constexpr float kSmallMax = 0x1p-100f, kLift = 0x1p60f;
+__device__ __forceinline__ float lift_of(float m) { return m < kSmallMax ? kLift : 1.0f; }
 
 struct NormArgs {
     const void *x, *r, *w;
@@ -54,7 +59,7 @@ struct NormBwdArgs {
 // from which the root drops out. What the products and the quotient leave over in
 // 32 bits is carried along (`rest` of the largest, `lo` of the quotient): a value
 // next to a rounding border of the 8 bits then falls where the formula has it, but
-// for the one rounding to 32 bits before the one to 8.
+// for the one rounding to 32 bits before the one to 8. s: the row's, times lift_of(m).
 struct Quant {
     float scale, hi, lo;
     __device__ __forceinline__ float operator()(float s, float w) const {
@@ -67,9 +72,11 @@ __device__ __forceinline__ Quant quant_of(float m, float rest, float rstd) {
     if (top < kTinyMax) return Quant{1.0f, 0.0f, 0.0f};
     Quant f;
     f.scale = top / 448.0f;
-    f.hi = m > 1e-30f ? 448.0f / m : rstd * (448.0f / top);  // the quotient must not overflow
-    f.lo = m > 1e-30f ? (fmaf(-m, f.hi, 448.0f) - rest * f.hi) / m : 0.0f;
-    if (top != top) f.hi = top;  // NaN in the row, or an infinity against 1 / infinity
+    const float most = m * lift_of(m);
+    f.hi = 448.0f / most;
+    f.lo = (fmaf(-most, f.hi, 448.0f) - rest * lift_of(m) * f.hi) / most;
+    // NaN or an infinity in the row (1 / infinity is zero), or |s w| past the largest number
+    if (!(top <= 3.4028235e38f)) f.scale = f.hi = __int_as_float(0x7fffffff);
     return f;
 }
 // The larger of two magnitudes, NaN if either is.
@@ -315,6 +322,12 @@ rms_norm_kernel(const NormArgs a) {
         if constexpr (Q) {
             const Quant f = quant_of(m, rest, rstd);
             if (l == 0) a.scale[t] = f.scale;
+            if (m < kSmallMax) {
+#pragma unroll
+                for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[v][e] *= kLift;
+            }
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
@@ -360,7 +373,7 @@ rms_norm_long_kernel(const NormArgs a) {
         }
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
             const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
-            if constexpr (Q) static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(f(s, wt(k)));
+            if constexpr (Q) static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(f(s * lift_of(m), wt(k)));
             else static_cast<T*>(a.y)[t * a.ldy + k] = from_f<T>(s * (wt(k) * rstd));
         }
     }

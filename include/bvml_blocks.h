@@ -78,9 +78,10 @@ int bvml_rms_norm(const void* x, long long ldx, const void* residual, long long 
                   void* y, long long ldy, void* sum, long long lds, void* stream);
 
 /*
- * bvml_rms_norm with y in 8 bits: scale[t] = max_k |y[t, k]| / 448 (fp32; 1 for a row
- * of zeros), q[t, k] = y[t, k] / scale[t] rounded to nearest e4m3, so y ~ q * scale.
- * A row with NaN or infinities has a NaN scale. `q` (T, K) e4m3.
+ * bvml_rms_norm with y in 8 bits: scale[t] = max_k |y[t, k]| / 448 (fp32),
+ * q[t, k] = y[t, k] / scale[t] rounded to nearest e4m3, so y ~ q * scale. A row whose
+ * largest |y| is below 2^-110 counts as zeros: q = 0, scale = 1. A row with NaN or
+ * infinities in s or y (zeros with eps = 0 are 0 / 0) has a NaN scale. `q` (T, K) e4m3.
  */
 int bvml_rms_norm_e4m3(const void* x, long long ldx, const void* residual, long long ldr,
                        const void* weight, int T, int K, int dtype, int weight_dtype, float eps,

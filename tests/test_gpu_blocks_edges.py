@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import brovisionml_b200 as bv
-from test_gpu_blocks import BF16, E4M3, F32, quantized, rnd
+from test_gpu_blocks import BF16, E, E4M3, F32, quantized, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,33 @@ def test_empty_batches_in_8_bits(lead):
     assert h.shape == (*lead, 40) and h.dtype == BF16
     y, z = bv.linear(q, w, rnd(40), x_scale=scale, w_scale=ws, out_dtype=F32, save=True)
     assert y.shape == z.shape == (*lead, 40) and y.dtype == F32
+
+
+@pytest.mark.parametrize("K", [64, 65, 640, 4096, 16400])
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_rms_norm_e4m3_of_small_rows(K, dt):
+    """Rows near and below the smallest normal numbers: finite where the norm is, as the
+    formula has them (their |s w| rounded to 32 bits: half of 2^-149 at least), zeros below
+    2^-110."""
+    sizes = (1e-30, 7e-31, 1e-33, 1e-35, 1.4e-36, 1.2e-36, 1e-36, 8e-37, 6e-37, 1e-37, 2e-39)
+    for eps in (1e-6, 1e-12):
+        x = rnd(len(sizes), K)
+        x = (x / x.abs().amax(1, keepdim=True) * torch.tensor(sizes, device="cuda")[:, None]).to(dt)
+        w = rnd(K, seed=1).abs() * 0.1 + 0.9
+        q, scale = bv.rms_norm_e4m3(x, w, eps=eps)
+        y = x.double() * w.double() * (x.double().square().mean(1, keepdim=True) + eps).rsqrt()
+        top = y.abs().amax(1)
+        zero, some = top < 2.0 ** -110 * (1 - 1e-3), top > 2.0 ** -110 * (1 + 1e-3)
+        assert some.sum() > 3
+        assert (scale[zero] == 1).all() and (q[zero].float() == 0).all()
+        y, top, q, scale = y[some], top[some], q[some].double(), scale[some].double()
+        # |s w| is off by half a step, which below 2^-126 is 2^-150, times the root
+        fine = (K / 2 + 16) * E
+        step = 2.0 ** -150 * eps ** -0.5
+        assert ((scale - top / 448).abs() <= fine * top / 448 + step / 448).all()
+        off = ((q * scale[:, None] - y).abs()
+               - (2.0 ** -4 + 2 * fine) * y.abs() - scale[:, None] * 2.0 ** -10 - 2 * step)
+        assert (off <= 0).all(), off.max()
+    z = torch.zeros(2, K, device="cuda", dtype=dt)
+    q, scale = bv.rms_norm_e4m3(z, w, eps=0.0)
+    assert scale.isnan().all() and q.float().isnan().all()  # 0 / 0
