@@ -79,17 +79,43 @@ __device__ __forceinline__ Quant quant_of(float m, float rest, float rstd) {
     if (!(top <= 3.4028235e38f)) f.scale = f.hi = __int_as_float(0x7fffffff);
     return f;
 }
-// The larger of two magnitudes, NaN if either is.
+// The larger of two, NaN if either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
     return a;
 }
-// The largest |s w| so far and what its product left over; NaN stays.
-__device__ __forceinline__ void largest(float s, float w, float& m, float& rest) {
-    const float p = fabsf(s) * fabsf(w), left = fmaf(fabsf(s), fabsf(w), -p);
-    const float n = max_nan(m, p);
-    if (n != m) rest = left;
-    m = n;
+// A thread's largest |s w| as its product rounded to 32 bits, m, and what that left over,
+// the larger of two where the rounded products are equal: every thread of a row, in whatever
+// order, must arrive at the same pair. Rounding keeps the products' order, so that rest is
+// the largest of |s w| - m, exact for m's own product. Each group of eight on its own,
+// then joined, as chains of maxima are what a row waits for. m: NaN stays.
+template <int VPT>
+__device__ __forceinline__ void largest(const float (&s)[VPT][8], const float (&w)[VPT][8],
+                                        float& m, float& rest) {
+    float g[VPT][2], r[VPT][2];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            g[v][h] = fabsf(s[v][h] * w[v][h]);
+#pragma unroll
+            for (int e = 2 + h; e < 8; e += 2) g[v][h] = max_nan(g[v][h], fabsf(s[v][e] * w[v][e]));
+        }
+    m = max_nan(g[0][0], g[0][1]);
+#pragma unroll
+    for (int v = 1; v < VPT; ++v) m = max_nan(m, max_nan(g[v][0], g[v][1]));
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            r[v][h] = fmaf(fabsf(s[v][h]), fabsf(w[v][h]), -m);
+#pragma unroll
+            for (int e = 2 + h; e < 8; e += 2)
+                r[v][h] = fmaxf(r[v][h], fmaf(fabsf(s[v][e]), fabsf(w[v][e]), -m));
+        }
+    rest = fmaxf(r[0][0], r[0][1]);
+#pragma unroll
+    for (int v = 1; v < VPT; ++v) rest = fmaxf(rest, fmaxf(r[v][0], r[v][1]));
 }
 
 // Feature index of element e of group v of lane l: eight consecutive features
@@ -201,28 +227,16 @@ __device__ __forceinline__ void store_row_e4m3(uint8_t* p, int K, int vec, int l
     }
 }
 
-// Sum of a over the G threads of a row, and of b, or (MAX) the largest b and the c that
-// belongs to it; every thread gets the result. G > 32: the whole block takes part;
-// `slot` alternates between rows, so that one barrier a row is enough.
-template <bool MAX>
-__device__ __forceinline__ void join_pair(float& a, float& b, float& c, float oa, float ob,
-                                          float oc) {
-    a += oa;
-    if constexpr (MAX) {
-        if (ob > b || ob != ob) b = ob, c = oc;
-    } else {
-        b += ob;
-    }
-}
-template <int G, bool MAX>
-__device__ __forceinline__ void row_reduce(float& a, float& b, float& c, float (*slots)[3][16],
-                                           int slot) {
+// Sum of a over the G threads of a row, and of b; every thread gets the result. G > 32: the
+// whole block takes part; `slot` alternates between rows, so that one barrier a row is
+// enough.
+template <int G>
+__device__ __forceinline__ void row_reduce(float& a, float& b, float (*slots)[3][16], int slot) {
     constexpr int kWidth = G < 32 ? G : 32;
 #pragma unroll
     for (int d = kWidth / 2; d > 0; d >>= 1) {
-        const float oa = __shfl_xor_sync(0xffffffffu, a, d);
-        const float ob = __shfl_xor_sync(0xffffffffu, b, d);
-        join_pair<MAX>(a, b, c, oa, ob, MAX ? __shfl_xor_sync(0xffffffffu, c, d) : 0.0f);
+        a += __shfl_xor_sync(0xffffffffu, a, d);
+        b += __shfl_xor_sync(0xffffffffu, b, d);
     }
     if constexpr (G > 32) {
         constexpr int kN = G / 32;
@@ -230,16 +244,66 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float& c, float (
         if ((threadIdx.x & 31) == 0) {
             slots[slot][0][warp] = a;
             slots[slot][1][warp] = b;
-            if (MAX) slots[slot][2][warp] = c;
         }
         __syncthreads();
         a = slots[slot][0][0];
         b = slots[slot][1][0];
-        if (MAX) c = slots[slot][2][0];
 #pragma unroll
-        for (int i = 1; i < kN; ++i)
-            join_pair<MAX>(a, b, c, slots[slot][0][i], slots[slot][1][i],
-                           MAX ? slots[slot][2][i] : 0.0f);
+        for (int i = 1; i < kN; ++i) {
+            a += slots[slot][0][i];
+            b += slots[slot][1][i];
+        }
+    }
+}
+// ... and the largest m (not negative; NaN if one is) with the largest c beside it.
+__device__ __forceinline__ float warp_max_nan(float v) {
+    asm("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+    asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    return v;
+}
+template <int G>
+__device__ __forceinline__ void row_reduce_max(float& a, float& m, float& c, float (*slots)[3][16],
+                                               int slot) {
+    constexpr int kWidth = G < 32 ? G : 32;
+#pragma unroll
+    for (int d = kWidth / 2; d > 0; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
+    float most = m;
+    if constexpr (G < 32) {
+#pragma unroll
+        for (int d = kWidth / 2; d > 0; d >>= 1)
+            most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+        c = m == most ? c : -INFINITY;
+#pragma unroll
+        for (int d = kWidth / 2; d > 0; d >>= 1)
+            c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, d));
+    } else {
+        most = warp_max_nan(m);
+        c = warp_max(m == most ? c : -INFINITY);
+    }
+    m = most;
+    if constexpr (G > 32) {
+        constexpr int kN = G / 32;
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) {
+            slots[slot][0][warp] = a;
+            slots[slot][1][warp] = m;
+            slots[slot][2][warp] = c;
+        }
+        __syncthreads();
+        a = slots[slot][0][0];
+        m = slots[slot][1][0];
+#pragma unroll
+        for (int i = 1; i < kN; ++i) {
+            a += slots[slot][0][i];
+            m = max_nan(m, slots[slot][1][i]);
+        }
+        c = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            c = fmaxf(c, slots[slot][1][i] == m ? slots[slot][2][i] : -INFINITY);
     }
 }
 
@@ -307,16 +371,15 @@ rms_norm_kernel(const NormArgs a) {
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (e % 2 == 0) {
-                    const float2 d = make_float2(s[v][e], s[v][e + 1]);
-                    q2 = __ffma2_rn(d, d, q2);
-                }
-                if constexpr (Q) largest(s[v][e], w[v][e], m, rest);
+            for (int e = 0; e < 8; e += 2) {
+                const float2 d = make_float2(s[v][e], s[v][e + 1]);
+                q2 = __ffma2_rn(d, d, q2);
             }
         }
+        if constexpr (Q) largest<VPT>(s, w, m, rest);
         float q = q2.x + q2.y;
-        row_reduce<G, Q>(q, m, rest, slots, slot);
+        if constexpr (Q) row_reduce_max<G>(q, m, rest, slots, slot);
+        else row_reduce<G>(q, m, slots, slot);
         if (!in) continue;
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         if constexpr (Q) {
@@ -362,9 +425,14 @@ rms_norm_long_kernel(const NormArgs a) {
             const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
             if (a.sum) static_cast<T*>(a.sum)[t * a.lds + k] = from_f<T>(s);
             q = fmaf(s, s, q);
-            if constexpr (Q) largest(s, wt(k), m, rest);
+            if constexpr (Q) {
+                const float p = fabsf(s * wt(k)), left = fmaf(fabsf(s), fabsf(wt(k)), -p);
+                if (!(p < m) && !(p == m && left <= rest)) rest = left;
+                m = max_nan(m, p);
+            }
         }
-        row_reduce<kLongThreads, Q>(q, m, rest, slots, slot);
+        if constexpr (Q) row_reduce_max<kLongThreads>(q, m, rest, slots, slot);
+        else row_reduce<kLongThreads>(q, m, slots, slot);
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         Quant f{};
         if constexpr (Q) {
@@ -429,7 +497,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[v][e] = dy[v][e] = 0.0f;
         }
-        float q = 0.0f, p = 0.0f, none = 0.0f;
+        float q = 0.0f, p = 0.0f;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
 #pragma unroll
@@ -438,7 +506,7 @@ rms_norm_backward_kernel(const NormBwdArgs a) {
                 p = fmaf(dy[v][e] * w[v][e], s[v][e], p);
             }
         }
-        row_reduce<G, false>(q, p, none, slots, slot);
+        row_reduce<G>(q, p, slots, slot);
         if (!in) continue;
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         const float c = p * inv_k * rstd * rstd;
@@ -494,13 +562,13 @@ rms_norm_backward_long_kernel(const NormBwdArgs a) {
     for (long long t = blockIdx.x; t < a.T; t += gridDim.x, slot ^= 1) {
         const T* s = static_cast<const T*>(a.s) + t * a.lds;
         const T* dy = static_cast<const T*>(a.dy) + t * a.lddy;
-        float q = 0.0f, p = 0.0f, none = 0.0f;
+        float q = 0.0f, p = 0.0f;
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
             const float sv = to_f(s[k]);
             q = fmaf(sv, sv, q);
             p = fmaf(to_f(dy[k]) * wt(k), sv, p);
         }
-        row_reduce<kLongThreads, false>(q, p, none, slots, slot);
+        row_reduce<kLongThreads>(q, p, slots, slot);
         const float rstd = rsqrtf(fmaf(q, inv_k, a.eps));
         const float c = p * inv_k * rstd * rstd;
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {

@@ -50,3 +50,30 @@ def test_rms_norm_e4m3_of_small_rows(K, dt):
     z = torch.zeros(2, K, device="cuda", dtype=dt)
     q, scale = bv.rms_norm_e4m3(z, w, eps=0.0)
     assert scale.isnan().all() and q.float().isnan().all()  # 0 / 0
+
+
+@pytest.mark.parametrize("K", [64, 65, 128, 200, 500, 1000, 1001, 4096, 16400])
+def test_rms_norm_e4m3_of_equal_largest_products(K):
+    """Two elements whose products with their weights are equal in 32 bits and not beyond:
+    the larger one gives the row's scale for all of the row, wherever the two stand. The
+    values beside them lie next to rounding borders of the 8 bits (17, 23, 272, ...)."""
+    h = float.fromhex
+    tops = [(h("0x1.63c556p+0"), h("0x1.432a7p+0")), (h("0x1.48dfd4p+0"), h("0x1.5d986ep+0"))]
+    assert len({float(torch.tensor(a) * torch.tensor(b)) for a, b in tops}) == 1
+    beside = [h(v) for v in ("0x1.10ad04p-4", "0x1.70ea14p-4", "0x1.d12724p-4", "0x1.10ad04p+0",
+                             "0x1.70ea14p+0")]
+    most = max(a * b for a, b in tops)
+    want = torch.tensor([v * 448 / most for v in beside]).to(E4M3).float()
+    x = torch.zeros(6, K, device="cuda")
+    w = torch.ones(6, K, device="cuda")
+    at = [(0, 40, 1), (1, 63, 2), (K - 1, 7, K // 2), (K // 2, K - 2, 5), (8, 9, 17), (33, 2, 44)]
+    for t, (i, j, k) in enumerate(at):
+        x[t, i], w[t, i] = tops[t % 2]
+        x[t, j], w[t, j] = tops[1 - t % 2]
+        free = [p for p in range(K) if p not in (i, j)]
+        for n, p in enumerate(free):
+            x[t, p] = beside[n % 5]
+        q, scale = bv.rms_norm_e4m3(x[t:t + 1], w[t])
+        got = q[0, free].float().cpu()
+        assert torch.equal(got, want.repeat(K // 5 + 1)[:len(free)]), t
+        assert (q[0, [i, j]].float() == 448).all()
