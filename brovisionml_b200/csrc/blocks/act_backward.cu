@@ -57,9 +57,16 @@ __device__ __forceinline__ void times_grad(int act, const float (&z)[8], float (
             v[e] *= d;                                    \
         }                                                 \
         break;
+        // one path for these two: with one each the kernel spills (12 bytes loaded -> 36)
+        case BVML_ACT_SIGMOID:
+        case BVML_ACT_TANH: {
+            const float k = act == BVML_ACT_TANH ? -2.0f * kLog2E : -kLog2E;
+            const float c = act == BVML_ACT_TANH ? 4.0f : 1.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= bell_f(z[e], k, c);
+            break;
+        }
         BVML_TIMES_GRAD(BVML_ACT_RELU)
-        BVML_TIMES_GRAD(BVML_ACT_SIGMOID)
-        BVML_TIMES_GRAD(BVML_ACT_TANH)
         BVML_TIMES_GRAD(BVML_ACT_SILU)
         BVML_TIMES_GRAD(BVML_ACT_GELU)
 #undef BVML_TIMES_GRAD

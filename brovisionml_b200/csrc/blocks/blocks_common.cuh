@@ -132,6 +132,14 @@ __device__ __forceinline__ float act_f(float z, int act) {
     }
 }
 
+// Sigmoid's and tanh's derivatives: c a / (1 + a)^2 with a = 2^(k |z|), that is exp(-|z|)
+// and c = 1 or exp(-2 |z|) and c = 4. f (1 - f) and 1 - f^2 cancel, at z = 8 down to a
+// seventh of tanh's value. Relative error below (4 |z| + 16) 2^-24.
+__device__ __forceinline__ float bell_f(float z, float k, float c) {
+    const float a = ex2(k * fabsf(z)), r = rcp(1.0f + a);
+    return a * r * (c * r);
+}
+
 // ... and their derivatives: value and derivative share what they can.
 __device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d) {
     switch (act) {
@@ -141,12 +149,12 @@ __device__ __forceinline__ void act_grad_f(float z, int act, float& f, float& d)
             break;
         case BVML_ACT_SIGMOID: {
             f = sigmoid_f(z);
-            d = f * (1.0f - f);
+            d = bell_f(z, -kLog2E, 1.0f);
             break;
         }
         case BVML_ACT_TANH: {
             f = tanhf(z);
-            d = 1.0f - f * f;
+            d = bell_f(z, -2.0f * kLog2E, 4.0f);
             break;
         }
         case BVML_ACT_SILU: {

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import brovisionml_b200 as bv
-from test_gpu_blocks import BF16, E, E4M3, F32, quantized, rnd
+from test_gpu_blocks import BF16, E, E4M3, F16, F32, quantized, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,33 @@ def test_rms_norm_e4m3_of_equal_largest_products(K):
         got = q[0, free].float().cpu()
         assert torch.equal(got, want.repeat(K // 5 + 1)[:len(free)]), t
         assert (q[0, [i, j]].float() == 448).all()
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "tanh"])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_derivatives_far_from_zero(act, dt):
+    """Derivatives that go to zero keep their figures: e^-|z| (e^-2|z|) from a rounded
+    argument and the hardware's 2^x and 1 / x are good to (4 |z| + 16) 2^-24 together, and
+    below 2^-126 flush to zero. Alone (the bias gradient of one row) and through the gate."""
+    z = torch.cat([torch.linspace(-60, 60, 961), torch.tensor([3e38, -3e38])]).cuda().to(dt)
+    z[0], z[1] = float("inf"), float("-inf")
+    N = z.numel()
+    one = torch.ones(1, N, device="cuda", dtype=dt)
+    x, w = torch.ones(1, 8, device="cuda", dtype=dt), torch.zeros(N, 8, device="cuda", dtype=dt)
+    _, _, db = bv.linear_backward(one, x, w, z[None], act=act, bias=True, dx=False, dw=False)
+    v = z.double().abs()
+    a = torch.exp(-v if act == "sigmoid" else -2 * v)
+    ref = a / (1 + a) ** 2 * (1 if act == "sigmoid" else 4)
+    rel = torch.where(v.isinf(), torch.zeros_like(v), (4 * v + 16) * E * ref)
+    assert ((db.double() - ref).abs() <= rel + 2.0 ** -123).all()
+    x[0, 1:] = 0  # dw_gate[:, 0] = dg = dh u act'(g)
+    _, dg, du = bv.gated_linear_backward(one, x, w, w, z[None], one, act=act, dx=False)
+    small = torch.finfo(dt).tiny * torch.finfo(dt).eps  # the smallest step, halved twice
+    assert ((dg[:, 0].double() - ref).abs()
+            <= rel + (ref + rel) * torch.finfo(dt).eps / 2 + small / 2 + 2.0 ** -123).all()
+    f = torch.sigmoid(z.double()) if act == "sigmoid" else torch.tanh(z.double())
+    assert ((du[:, 0].double() - f).abs() <= f.abs() * (torch.finfo(dt).eps / 2 + 200 * E)
+            + small / 2 + 2.0 ** -123).all()
+    nan = torch.full_like(one, float("nan"))
+    _, _, db = bv.linear_backward(one, x, w, nan, act=act, bias=True, dx=False, dw=False)
+    assert db.isnan().all()
