@@ -8,7 +8,8 @@ sequence), the kernels of libbvml_blocks.so (include/bvml_blocks.h):
 
 each with its backward pass as a function of its own (``*_backward``): the
 operators take no part in torch's autograd, and refuse inputs that require
-gradients while it records.
+gradients while it records, that carry a forward-mode tangent, or that belong to a trace,
+a transform (vmap, torch.func) or a tensor class that torch dispatches on.
 
 Matrices are 2-D, or have leading axes that are taken as rows; the last axis
 is contiguous and rows may be further apart than they are long (a column range

@@ -10,8 +10,11 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -44,16 +47,37 @@ struct Call {
         throw Refusal{std::string("dsine ops: ") + op + ": " + what};
     }
 
-    // Every given tensor on one CUDA device, and none that autograd would follow.
+    // Every given tensor on one CUDA device, and none that torch would follow past the
+    // kernels: through autograd, forward-mode derivatives, a trace, a transform (vmap,
+    // functionalize, ...) or a class of its own. These calls do not pass its dispatcher, so
+    // that what it follows would be dropped, or held as a constant, without a word.
     void device(std::initializer_list<const Tensor*> ts) {
+        using c10::DispatchKey;
+        using Mode = c10::impl::TorchDispatchModeTLS;
+        constexpr c10::DispatchKeySet kWrapped{
+            DispatchKey::Python,      DispatchKey::Functionalize,
+            DispatchKey::Batched,     DispatchKey::BatchedNestedTensor,
+            DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper};
         const Tensor& first = **ts.begin();
-        const bool grad = c10::GradMode::is_enabled();
+        const c10::AutogradState& state = c10::AutogradState::get_tls_state();
+        const bool grad = state.get_grad_mode(), forward = state.get_fw_grad_mode();
+        if (at::tracer::impl::is_dispatch_enabled() ||
+            (c10::impl::dispatch_mode_enabled() &&
+             (Mode::get_mode(c10::impl::TorchDispatchModeKey::PROXY) ||
+              Mode::get_mode(c10::impl::TorchDispatchModeKey::FAKE) ||
+              Mode::get_mode(c10::impl::TorchDispatchModeKey::FUNCTIONAL))))
+            refuse("cannot be traced");
         for (const Tensor* t : ts) {
             if (!t->defined()) continue;
             if (t->device() != first.device()) refuse("all inputs must share a device");
             if (grad && t->requires_grad())
                 refuse("no autograd: pass detached tensors, or call under torch.no_grad() "
                        "(the gradients have functions of their own, *_backward)");
+            if (forward && t->_fw_grad(0).defined())
+                refuse("no forward-mode derivatives: pass tensors without a tangent");
+            if (t->key_set().has_any(kWrapped))
+                refuse("tensors of torch's transforms and of classes that torch dispatches "
+                       "on are not followed: pass plain tensors");
             if (t->layout() != at::kStrided) refuse("tensors must be strided");
         }
         if (!first.is_cuda())

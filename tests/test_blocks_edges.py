@@ -2,7 +2,10 @@
 import ctypes
 
 import pytest
+import torch
+import torch.autograd.forward_ad as fwad
 
+import brovisionml_b200 as bv
 from brovisionml_b200 import _blocks_capi as B
 from test_blocks_api import BF16, E4M3, EINVAL, at, err, gated_args, linear_args
 
@@ -23,3 +26,60 @@ def test_empty_batches_in_8_bits(x, x_scale):
     a = linear_args(T=1, in_type=E4M3, w_scale=at(6))
     assert B.blocks_lib.bvml_linear(ctypes.byref(a), None, 0, None) == EINVAL
     assert "need their scales" in err()
+
+
+def calls(t, w, v):
+    """Every operator, with t among its tensors (rows for the inner axis of 8)."""
+    return [lambda: bv.rms_norm(t, v), lambda: bv.rms_norm(w, v, t),
+            lambda: bv.rms_norm_e4m3(t, v), lambda: bv.rms_norm_backward(w, t, v),
+            lambda: bv.rms_norm_backward(t, w, v), lambda: bv.linear(t, w),
+            lambda: bv.linear(w, t), lambda: bv.linear(w, w, residual=t[:, :6]),
+            lambda: bv.linear_backward(t[:, :6], w, w), lambda: bv.gated_linear(w, w, t),
+            lambda: bv.gated_linear_backward(w[:, :6], w, w, w, w[:, :6], t[:, :6])]
+
+
+def test_what_torch_follows_is_refused():
+    """Forward-mode tangents, traces, transforms and tensor classes would be dropped without
+    a word: refused, whichever argument carries them."""
+    w, v = torch.ones(6, 8), torch.ones(8)
+    with fwad.dual_level():
+        t = fwad.make_dual(torch.ones(6, 8), torch.ones(6, 8))
+        for call in calls(t, w, v):
+            with pytest.raises(RuntimeError, match="dsine ops: .*forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            bv.linear(t, w)  # no_grad() does not end forward mode
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="CUDA-resident"):
+            bv.linear(t, w)  # ... which inference_mode() does
+        with pytest.raises(RuntimeError, match="CUDA-resident"):
+            bv.linear(fwad.unpack_dual(t).primal, w)
+
+    def inside(t):
+        for call in calls(t, w, v):
+            with pytest.raises(RuntimeError, match="dsine ops: .*(transforms|autograd|forward)"):
+                call()
+        return t.sum()
+
+    torch.vmap(inside)(torch.ones(2, 6, 8))
+    torch.func.grad(inside)(torch.ones(6, 8))
+    torch.func.jvp(inside, (torch.ones(6, 8),), (torch.ones(6, 8),))
+    torch.func.functionalize(inside)(torch.ones(6, 8))
+
+    class Named(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with pytest.raises(RuntimeError, match="plain tensors"):
+        bv.linear(torch.Tensor._make_subclass(Named, torch.ones(6, 8)), w)
+
+    def traced(t):
+        with pytest.raises(RuntimeError, match="dsine ops: linear: cannot be traced"):
+            bv.linear(w, w)
+        return t + 1
+
+    torch.jit.trace(traced, torch.ones(2), check_trace=False)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    make_fx(traced)(torch.ones(2))
+    with pytest.raises(RuntimeError, match="CUDA-resident"):  # and after all that as before
+        bv.linear(w, w)
