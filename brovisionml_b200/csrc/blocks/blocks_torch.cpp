@@ -78,6 +78,9 @@ struct Call {
             if (t->key_set().has_any(kWrapped))
                 refuse("tensors of torch's transforms and of classes that torch dispatches "
                        "on are not followed: pass plain tensors");
+            if (t->is_neg() || t->_is_zerotensor())
+                refuse("a tensor's memory must hold its values: call resolve_neg() on a lazy "
+                       "negation, clone() a zero tensor");
             if (t->layout() != at::kStrided) refuse("tensors must be strided");
         }
         if (!first.is_cuda())

@@ -83,3 +83,15 @@ def test_what_torch_follows_is_refused():
     make_fx(traced)(torch.ones(2))
     with pytest.raises(RuntimeError, match="CUDA-resident"):  # and after all that as before
         bv.linear(w, w)
+
+
+def test_lazy_values_are_refused():
+    """Tensors whose memory does not hold their values: a negation that torch has put off
+    (the imaginary part of a conjugate), zeros without memory."""
+    w, v = torch.ones(6, 8), torch.ones(8)
+    for t in (torch._neg_view(torch.ones(6, 8)), torch._efficientzerotensor(6, 8)):
+        for call in calls(t, w, v):
+            with pytest.raises(RuntimeError, match="dsine ops: .*hold its values"):
+                call()
+    with pytest.raises(RuntimeError, match="CUDA-resident"):
+        bv.linear(torch._neg_view(torch.ones(6, 8)).resolve_neg(), w)
