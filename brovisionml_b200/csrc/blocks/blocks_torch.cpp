@@ -37,6 +37,7 @@ using at::Tensor;
 struct Refusal {
     std::string what;
 };
+struct Raised {};  // a Python exception is set already
 
 // One call: its name, device, and the checks that every operator makes.
 struct Call {
@@ -220,7 +221,11 @@ Tensor needed(PyObject* o, const char* name) {
     if (o == Py_None) throw Refusal{std::string("dsine ops: ") + name + " must be a tensor"};
     return tensor(o, name);
 }
-bool flag(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool flag(PyObject* o) {  // read before anything else, as it may run Python code
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raised{};
+    return v == 1;
+}
 std::optional<ScalarType> dtype(PyObject* o) {
     if (o == Py_None) return std::nullopt;
     if (!THPDtype_Check(o)) throw Refusal{"dsine ops: out_dtype must be a torch.dtype"};
@@ -261,6 +266,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t) {
         return F(args);
     } catch (const Refusal& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what.c_str());
+    } catch (const Raised&) {
     } catch (...) {  // torch's own: out of memory and the like
         torch::translate_exception_to_python(std::current_exception());
     }
@@ -365,6 +371,7 @@ ScalarType out_type(const Call& c, ScalarType in, std::optional<ScalarType> want
 
 PyObject* linear(PyObject* const* a) {
     Call c{"linear"};
+    const bool save = flag(a[8]);
     const Tensor x = needed(a[0], "x"), w = needed(a[1], "weight"), b = tensor(a[2], "bias"),
                  r = tensor(a[4], "residual"), xs = tensor(a[5], "x_scale"),
                  ws = tensor(a[6], "w_scale");
@@ -387,7 +394,7 @@ PyObject* linear(PyObject* const* a) {
         const Rows rr = rows_of(c, r, "residual", g.N, g.T, o);
         g.residual = rr.p, g.ldr = rr.ld;
     }
-    const Tensor y = like(x, o, g.N), z = flag(a[8]) ? like(x, o, g.N) : Tensor();
+    const Tensor y = like(x, o, g.N), z = save ? like(x, o, g.N) : Tensor();
     g.y = y.data_ptr(), g.z = ptr(z);
     g.ldy = g.ldz = g.N;
     run(c, bvml_linear, bvml_linear_workspace_bytes, g);
@@ -396,6 +403,7 @@ PyObject* linear(PyObject* const* a) {
 
 PyObject* linear_backward(PyObject* const* a) {
     Call c{"linear_backward"};
+    const bool want_db = flag(a[5]), want_dx = flag(a[6]), want_dw = flag(a[7]);
     const Tensor dy = needed(a[0], "dy"), x = needed(a[1], "x"), w = needed(a[2], "weight"),
                  z = tensor(a[3], "z");
     c.device({&dy, &x, &w, &z});
@@ -417,9 +425,9 @@ PyObject* linear_backward(PyObject* const* a) {
     g.dy = rd.p, g.lddy = rd.ld;
     g.x = rx.p, g.ldx = rx.ld;
     g.w = rw.p, g.ldw = rw.ld;
-    const Tensor db = flag(a[5]) ? make({g.N}, ScalarType::Float, c.dev) : Tensor();
-    const Tensor dx = flag(a[6]) ? like(x, t) : Tensor();
-    const Tensor dw = flag(a[7]) ? make({g.N, g.K}, t, c.dev) : Tensor();
+    const Tensor db = want_db ? make({g.N}, ScalarType::Float, c.dev) : Tensor();
+    const Tensor dx = want_dx ? like(x, t) : Tensor();
+    const Tensor dw = want_dw ? make({g.N, g.K}, t, c.dev) : Tensor();
     g.dx = ptr(dx), g.dw = ptr(dw), g.dbias = static_cast<float*>(ptr(db));
     g.lddx = g.lddw = g.K;
     run(c, bvml_linear_backward, bvml_linear_backward_workspace_bytes, g);
@@ -428,6 +436,7 @@ PyObject* linear_backward(PyObject* const* a) {
 
 PyObject* gated_linear(PyObject* const* a) {
     Call c{"gated_linear"};
+    const bool save = flag(a[8]);
     const Tensor x = needed(a[0], "x"), wg = needed(a[1], "w_gate"), wu = needed(a[2], "w_up"),
                  xs = tensor(a[4], "x_scale"), gs = tensor(a[5], "gate_scale"),
                  us = tensor(a[6], "up_scale");
@@ -447,7 +456,6 @@ PyObject* gated_linear(PyObject* const* a) {
     g.x_scale = vec_of(c, xs, "x_scale", g.T);
     g.gate_scale = vec_of(c, gs, "gate_scale", g.F);
     g.up_scale = vec_of(c, us, "up_scale", g.F);
-    const bool save = flag(a[8]);
     const Tensor h = like(x, o, g.F), pg = save ? like(x, o, g.F) : Tensor(),
                  pu = save ? like(x, o, g.F) : Tensor();
     g.h = h.data_ptr(), g.g = ptr(pg), g.u = ptr(pu);
@@ -458,6 +466,7 @@ PyObject* gated_linear(PyObject* const* a) {
 
 PyObject* gated_linear_backward(PyObject* const* a) {
     Call c{"gated_linear_backward"};
+    const bool want_dx = flag(a[7]), want_dw = flag(a[8]);
     const Tensor dh = needed(a[0], "dh"), x = needed(a[1], "x"), wg = needed(a[2], "w_gate"),
                  wu = needed(a[3], "w_up"), pg = needed(a[4], "g"), pu = needed(a[5], "u");
     c.device({&dh, &x, &wg, &wu, &pg, &pu});
@@ -478,10 +487,9 @@ PyObject* gated_linear_backward(PyObject* const* a) {
     g.x = rx.p, g.ldx = rx.ld;
     g.w_gate = rg.p, g.ldw_gate = rg.ld;
     g.w_up = ru.p, g.ldw_up = ru.ld;
-    const Tensor dx = flag(a[7]) ? like(x, t) : Tensor();
-    const bool dw = flag(a[8]);
-    const Tensor dg = dw ? make({g.F, g.K}, t, c.dev) : Tensor(),
-                 du = dw ? make({g.F, g.K}, t, c.dev) : Tensor();
+    const Tensor dx = want_dx ? like(x, t) : Tensor();
+    const Tensor dg = want_dw ? make({g.F, g.K}, t, c.dev) : Tensor(),
+                 du = want_dw ? make({g.F, g.K}, t, c.dev) : Tensor();
     g.dx = ptr(dx), g.dw_gate = ptr(dg), g.dw_up = ptr(du);
     g.lddx = g.lddw_gate = g.lddw_up = g.K;
     run(c, bvml_gated_linear_backward, bvml_gated_linear_backward_workspace_bytes, g);

@@ -95,3 +95,26 @@ def test_lazy_values_are_refused():
                 call()
     with pytest.raises(RuntimeError, match="CUDA-resident"):
         bv.linear(torch._neg_view(torch.ones(6, 8)).resolve_neg(), w)
+
+
+class Untrue:
+    def __bool__(self):
+        raise ValueError("neither true nor false")
+
+
+def test_flags_without_a_truth_value_raise_their_error():
+    """... and not a SystemError from a result returned beside a pending exception."""
+    w = torch.ones(6, 8)
+    d = w[:, :6]
+    for call in (lambda f: bv.linear(w, w, save=f), lambda f: bv.gated_linear(w, w, w, save=f),
+                 lambda f: bv.linear_backward(d, w, w, bias=f),
+                 lambda f: bv.linear_backward(d, w, w, dx=f),
+                 lambda f: bv.linear_backward(d, w, w, dw=f),
+                 lambda f: bv.gated_linear_backward(d, w, w, w, d, d, dx=f),
+                 lambda f: bv.gated_linear_backward(d, w, w, w, d, d, dw=f)):
+        with pytest.raises(ValueError, match="neither true nor false"):
+            call(Untrue())
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call(torch.ones(2))
+        with pytest.raises(RuntimeError, match="CUDA-resident"):
+            call(True)
