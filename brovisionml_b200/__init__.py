@@ -7,9 +7,10 @@ reference's op interface (``brovisionml::dsine::ray_relu`` /
 brotensor convex-upsample / L2-normalise / slice calls of
 src/dsine_refine.cpp:277-292) for Python callers, with torch tensors as the
 device-memory carrier. Beside it, libbvml_blocks.so (``include/bvml_blocks.h``) holds the
-feed-forward operators over rows of features (``blocks.py``). Every op runs in the CUDA library; there is no CPU or
-PyTorch fallback, and importing the package fails loudly when the library is
-missing.
+feed-forward operators over rows of features (``blocks.py``), loaded by their first call.
+Every op runs in the CUDA library; there is no CPU or PyTorch fallback: importing the
+package fails loudly when libbvml_dsine.so is missing, calling a feed-forward operator when
+theirs is.
 
 Errors raise ``RuntimeError`` carrying the library's message, worded like the
 reference's exceptions ("dsine ops: ..." / "dsine cuda: ...").

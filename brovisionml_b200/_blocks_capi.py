@@ -10,9 +10,9 @@ from __future__ import annotations
 import ctypes
 import os
 
-from ._capi import BVML_OK, LIB_PATH
+from ._capi import BVML_OK
+from .blocks import BLOCKS_LIB_PATH
 
-BLOCKS_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libbvml_blocks.so")
 BVML_BF16 = 2
 BVML_E4M3 = 3
 BVML_EWORKSPACE = 4

@@ -28,9 +28,9 @@ import os
 
 import torch
 
-from . import _blocks_capi
-from ._blocks_capi import BLOCKS_LIB_PATH
+from ._capi import LIB_PATH
 
+BLOCKS_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libbvml_blocks.so")
 _BINDING_PATH = os.path.join(os.path.dirname(BLOCKS_LIB_PATH), "_blocks_torch.so")
 
 
@@ -46,7 +46,17 @@ def _load_binding():
     return module
 
 
-_binding = _load_binding()
+class _Unloaded:
+    """Stands for the binding until the first call of an operator here, which loads it: it
+    is bound to one torch and one Python, and without it the rest of the package works."""
+
+    def __getattr__(self, name):
+        global _binding
+        _binding = _load_binding()
+        return getattr(_binding, name)
+
+
+_binding = _Unloaded()
 
 BLOCK_ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "silu": 4, "gelu": 5}
 
@@ -143,6 +153,8 @@ def blocks_status(device: torch.device | int | None = None) -> None:
     """Synchronises the device's current stream and raises if a matrix
     product's pipeline gave up waiting since the last call (its result is then
     unspecified)."""
+    from . import _blocks_capi
+
     dev = torch.device("cuda", device) if isinstance(device, int) else device
     with torch.cuda.device(dev):
         _blocks_capi.check(_blocks_capi.status(torch.cuda.current_stream().cuda_stream))

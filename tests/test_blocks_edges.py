@@ -1,5 +1,9 @@
 """CPU tests of the feed-forward operators at the edges of what their documents allow."""
 import ctypes
+import os
+import shutil
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -118,3 +122,31 @@ def test_flags_without_a_truth_value_raise_their_error():
             call(torch.ones(2))
         with pytest.raises(RuntimeError, match="CUDA-resident"):
             call(True)
+
+
+def test_the_package_works_without_these_operators(tmp_path):
+    """A missing library or binding of the feed-forward operators is an ImportError of their
+    first call, and takes nothing else of the package with it."""
+    src = os.path.dirname(os.path.abspath(bv.__file__))
+    dst = tmp_path / "brovisionml_b200"
+    (dst / "_lib").mkdir(parents=True)
+    for f in os.listdir(src):
+        if f.endswith(".py"):
+            shutil.copy(os.path.join(src, f), dst / f)
+    os.symlink(os.path.join(src, "_lib", "libbvml_dsine.so"), dst / "_lib" / "libbvml_dsine.so")
+    code = """
+import brovisionml_b200 as bv, torch
+assert bv.abi_version() > 0 and bv.refine_workspace_bytes(1, 8, 8) > 0 and callable(bv.refine)
+w = torch.ones(6, 8)
+q, s = bv.pack_weight_e4m3(w)
+for call in (lambda: bv.linear(w, w), lambda: bv.rms_norm(w, w[0]), lambda: bv.blocks_status(None)):
+    for _ in range(2):
+        try:
+            call()
+        except ImportError as e:
+            assert 'not built' in str(e), e
+        else:
+            raise SystemExit('no ImportError')
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
