@@ -31,15 +31,17 @@ import torch
 from ._capi import LIB_PATH
 
 BLOCKS_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libbvml_blocks.so")
-_BINDING_PATH = os.path.join(os.path.dirname(BLOCKS_LIB_PATH), "_blocks_torch.so")
 
 
 def _load_binding():
-    if not os.path.exists(_BINDING_PATH):
+    from .build import blocks_torch_path
+
+    path = blocks_torch_path(torch.__version__)
+    if not os.path.exists(path):
         raise ImportError(
-            f"brovisionml_b200: binding not built ({_BINDING_PATH} missing); run "
-            "`python brovisionml_b200/build.py` (nvcc for sm_100a)")
-    loader = importlib.machinery.ExtensionFileLoader("_blocks_torch", _BINDING_PATH)
+            f"brovisionml_b200: binding not built for torch {torch.__version__} and this Python "
+            f"({path} missing); run `python brovisionml_b200/build.py` (nvcc for sm_100a)")
+    loader = importlib.machinery.ExtensionFileLoader("_blocks_torch", path)
     spec = importlib.util.spec_from_loader("_blocks_torch", loader)
     module = importlib.util.module_from_spec(spec)
     loader.exec_module(module)

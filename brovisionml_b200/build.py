@@ -9,7 +9,8 @@ Compiles each brovisionml_b200/csrc/*.cu with nvcc for
 ``-gencode arch=compute_100a,code=sm_100a`` (B200 only) and links them into
 ``brovisionml_b200/_lib/libbvml_dsine.so``, and csrc/blocks/*.cu (the
 feed-forward operators, include/bvml_blocks.h) into ``_lib/libbvml_blocks.so``,
-with their Python binding (csrc/blocks/blocks_torch.cpp) in ``_lib/_blocks_torch.so``.
+with their Python binding (csrc/blocks/blocks_torch.cpp) for this torch and Python in
+``_lib/_blocks_torch.<Python's ABI>.torch<version>.so``.
 The C++ drop-in bridge
 (csrc/dsine_ops_b200.cpp) is compiled into ``_lib/libbvml_dsine_bridge.so``
 against the stand-in brotensor header, to prove that it builds.
@@ -21,6 +22,7 @@ import concurrent.futures as cf
 import glob
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -39,7 +41,6 @@ CHECKED_LIB = os.path.join(LIB_DIR, "libbvml_dsine_checked.so")
 BLOCKS = os.path.join(CSRC, "blocks")
 BLOCKS_LIB = os.path.join(LIB_DIR, "libbvml_blocks.so")
 BLOCKS_CHECKED_LIB = os.path.join(LIB_DIR, "libbvml_blocks_checked.so")
-BLOCKS_TORCH = os.path.join(LIB_DIR, "_blocks_torch.so")  # their Python binding
 BRIDGE = os.path.join(LIB_DIR, "libbvml_dsine_bridge.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -52,6 +53,24 @@ def _nvcc() -> str:
         if cand and os.path.exists(cand):
             return cand
     raise RuntimeError("nvcc not found: the CUDA toolkit is needed to build brovisionml_b200")
+
+
+def torch_version() -> str | None:
+    """torch.__version__ without importing torch; None where there is no torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.origin:
+        return None
+    with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:
+        m = re.search(r"^__version__\s*=\s*['\"]([^'\"]+)['\"]", f.read(), re.M)
+    return m.group(1) if m else None
+
+
+def blocks_torch_path(torch_ver: str) -> str:
+    """The feed-forward operators' Python binding for this Python and a torch, whose C++
+    interfaces differ from version to version: one file each, so that none is loaded by
+    another, and a new torch or Python has its own built."""
+    abi = sysconfig.get_config_var("SOABI")
+    return os.path.join(LIB_DIR, f"_blocks_torch.{abi}.torch{torch_ver}.so")
 
 
 def _stale(target: str, deps: list[str]) -> bool:
@@ -118,7 +137,8 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
         run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_CHECKED_LIB] + bcobjs +
             ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
     torch_src = os.path.join(BLOCKS, "blocks_torch.cpp")
-    if _stale(BLOCKS_TORCH, [torch_src, BLOCKS_LIB, __file__] + headers):
+    blocks_torch = blocks_torch_path(torch_version())
+    if _stale(blocks_torch, [torch_src, BLOCKS_LIB, __file__] + headers):
         torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
         cuda = os.path.dirname(os.path.dirname(nvcc))
         run([os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC",
@@ -126,7 +146,7 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
              "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(cuda, "include"),
              "-isystem", os.path.join(torch_dir, "include"),
              "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
-             "-I" + sysconfig.get_path("include"), torch_src, "-o", BLOCKS_TORCH,
+             "-I" + sysconfig.get_path("include"), torch_src, "-o", blocks_torch,
              "-L" + LIB_DIR, "-lbvml_blocks", "-Wl,-rpath,$ORIGIN",
              "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
              "-ltorch_cuda", "-lc10", "-lc10_cuda",

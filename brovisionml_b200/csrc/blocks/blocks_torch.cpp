@@ -1,6 +1,6 @@
 // Python binding of the feed-forward operators: torch tensors in, torch tensors
 // out, over the C ABI (include/bvml_blocks.h). Compiled into
-// _lib/_blocks_torch.so (CPython and torch's C++ API): a call checks its
+// _lib/_blocks_torch.*.so (CPython and torch's C++ API): a call checks its
 // tensors, allocates its outputs and launches in half the host time of the same
 // steps in Python (one-token rms_norm with residual: 11.5 us a call there), which is
 // what a decoding step with one-token operators is bound by.

@@ -4,6 +4,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 import pytest
 import torch
@@ -150,3 +151,22 @@ for call in (lambda: bv.linear(w, w), lambda: bv.rms_norm(w, w[0]), lambda: bv.b
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_the_binding_belongs_to_one_torch_and_python(monkeypatch):
+    """Its file name has both versions: the build makes one for each, and another version's
+    is never loaded."""
+    from brovisionml_b200 import blocks, build
+
+    assert build.torch_version() == torch.__version__
+    path = build.blocks_torch_path(torch.__version__)
+    assert os.path.exists(path)
+    assert sysconfig.get_config_var("SOABI") in path and torch.__version__ in path
+    assert blocks._load_binding().__file__ == path
+    monkeypatch.setattr(torch, "__version__", "0.1.2")
+    with pytest.raises(ImportError, match="not built for torch 0.1.2"):
+        blocks._load_binding()
+    monkeypatch.undo()
+    monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "cpython-27-x")
+    with pytest.raises(ImportError, match="not built for torch"):
+        blocks._load_binding()
