@@ -81,64 +81,82 @@ def _stale(target: str, deps: list[str]) -> bool:
 
 
 def build(verbose: bool = False, ptxas_info: bool = False) -> str:
-    """Compile (if stale) and return the path of libbvml_dsine.so."""
+    """Compile (if stale) and return the path of libbvml_dsine.so. The refinement's
+    libraries come first and need nvcc and a C++ compiler alone; the feed-forward
+    operators' library next (CUDA 12.9: 32-byte stores), their binding last, and only where
+    torch is installed."""
     nvcc = _nvcc()
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
     headers = (glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))
                + glob.glob(os.path.join(ROOT, "include", "*.h")))
-    sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
-    jobs = []
-    objs = []
-    cobjs = []
-    for src in sources:
-        obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-3] + ".o")
-        objs.append(obj)
-        if _stale(obj, [src] + headers) or ptxas_info:
-            cmd = [nvcc] + ARCH + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + \
-                  ["-c", src, "-o", obj]
-            jobs.append(cmd)
-        cobj = os.path.join(OBJ_DIR, "checked_" + os.path.basename(src)[:-3] + ".o")
-        cobjs.append(cobj)
-        if _stale(cobj, [src] + headers):
-            jobs.append([nvcc] + ARCH + NVCC_FLAGS + ["-DBVML_CHECKED", "-c", src, "-o", cobj])
-
-    # the feed-forward operators: a library of their own, so that the ABI of
-    # libbvml_dsine.so stays as it is
-    bheaders = headers + glob.glob(os.path.join(BLOCKS, "*.cuh")) + \
-        glob.glob(os.path.join(BLOCKS, "*.h"))
-    bobjs = []
-    bcobjs = []
-    for src in sorted(glob.glob(os.path.join(BLOCKS, "*.cu"))):
-        obj = os.path.join(OBJ_DIR, "blocks_" + os.path.basename(src)[:-3] + ".o")
-        bobjs.append(obj)
-        if _stale(obj, [src] + bheaders) or ptxas_info:
-            jobs.append([nvcc] + ARCH + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) +
-                        ["-c", src, "-o", obj])
-        cobj = os.path.join(OBJ_DIR, "checked_blocks_" + os.path.basename(src)[:-3] + ".o")
-        bcobjs.append(cobj)
-        if _stale(cobj, [src] + bheaders):
-            jobs.append([nvcc] + ARCH + NVCC_FLAGS + ["-DBVML_CHECKED", "-c", src, "-o", cobj])
 
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+            raise RuntimeError(os.path.basename(cmd[0]) + " failed:\n" + " ".join(cmd) + "\n" +
+                               r.stdout + r.stderr)
         return r.stdout + r.stderr
 
-    with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
-        for out in ex.map(run, jobs):
-            if verbose or ptxas_info:
-                sys.stdout.write(out)
-    if _stale(BLOCKS_LIB, bobjs + [__file__]):
-        run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_LIB] + bobjs +
-            ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
-    if _stale(BLOCKS_CHECKED_LIB, bcobjs + [__file__]):
-        run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", BLOCKS_CHECKED_LIB] + bcobjs +
-            ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
-    torch_src = os.path.join(BLOCKS, "blocks_torch.cpp")
-    blocks_torch = blocks_torch_path(torch_version())
-    if _stale(blocks_torch, [torch_src, BLOCKS_LIB, __file__] + headers):
+    def libraries(sources, deps, prefix, lib, checked_lib):
+        """The sources' objects and checked objects (all at once), and a library of each."""
+        jobs, objs, cobjs = [], [], []
+        for src in sources:
+            name = prefix + os.path.basename(src)[:-3] + ".o"
+            obj, cobj = os.path.join(OBJ_DIR, name), os.path.join(OBJ_DIR, "checked_" + name)
+            objs.append(obj)
+            cobjs.append(cobj)
+            if _stale(obj, [src] + deps) or ptxas_info:
+                jobs.append([nvcc] + ARCH + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else [])
+                            + ["-c", src, "-o", obj])
+            if _stale(cobj, [src] + deps):
+                jobs.append([nvcc] + ARCH + NVCC_FLAGS + ["-DBVML_CHECKED", "-c", src, "-o", cobj])
+        with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
+            for out in ex.map(run, jobs):
+                if verbose or ptxas_info:
+                    sys.stdout.write(out)
+        for target, parts in ((lib, objs), (checked_lib, cobjs)):
+            if _stale(target, parts + [__file__]):
+                # Shared cudart: callers (torch, or a brotensor runtime) hand in stream
+                # handles created by THEIR CUDA runtime; one shared runtime instance
+                # per process is what makes those handles valid here too.
+                run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", target] + parts +
+                    ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
+
+    libraries(sorted(glob.glob(os.path.join(CSRC, "*.cu"))), headers, "", LIB, CHECKED_LIB)
+    _build_bridge(nvcc, headers, run)
+    # the feed-forward operators: a library of their own, so that the ABI of
+    # libbvml_dsine.so stays as it is
+    libraries(sorted(glob.glob(os.path.join(BLOCKS, "*.cu"))),
+              headers + glob.glob(os.path.join(BLOCKS, "*.cuh")) +
+              glob.glob(os.path.join(BLOCKS, "*.h")), "blocks_", BLOCKS_LIB, BLOCKS_CHECKED_LIB)
+    _build_binding(nvcc, headers, run)
+    return LIB
+
+
+def _build_bridge(nvcc, headers, run):
+    bridge_src = os.path.join(CSRC, "dsine_ops_b200.cpp")
+    if not os.path.exists(bridge_src):
+        return
+    deps = [bridge_src, LIB] + headers + glob.glob(os.path.join(CSRC, "brotensor_shim", "*", "*.h"))
+    if _stale(BRIDGE, deps):
+        cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+        cuda = os.path.dirname(os.path.dirname(nvcc))
+        run([cxx, "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", "-Wextra",
+             "-I" + os.path.join(CSRC, "brotensor_shim"), "-I" + os.path.join(ROOT, "include"),
+             "-I" + os.path.join(cuda, "include"), "-DBVML_SHIM_CUDA", bridge_src, "-o", BRIDGE,
+             "-L" + LIB_DIR, "-lbvml_dsine", "-Wl,-rpath,$ORIGIN",
+             "-L" + os.path.join(cuda, "lib64"), "-lcudart", "-Wl,--exclude-libs,ALL"])
+
+
+def _build_binding(nvcc, headers, run):
+    version = torch_version()
+    if version is None:
+        print("no torch here: the feed-forward operators' Python binding is left out",
+              file=sys.stderr)
+        return
+    src, target = os.path.join(BLOCKS, "blocks_torch.cpp"), blocks_torch_path(version)
+    if _stale(target, [src, BLOCKS_LIB, __file__] + headers):
         torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
         cuda = os.path.dirname(os.path.dirname(nvcc))
         run([os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC",
@@ -146,34 +164,11 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
              "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(cuda, "include"),
              "-isystem", os.path.join(torch_dir, "include"),
              "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
-             "-I" + sysconfig.get_path("include"), torch_src, "-o", blocks_torch,
+             "-I" + sysconfig.get_path("include"), src, "-o", target,
              "-L" + LIB_DIR, "-lbvml_blocks", "-Wl,-rpath,$ORIGIN",
              "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
              "-ltorch_cuda", "-lc10", "-lc10_cuda",
              "-Wl,-rpath," + os.path.join(torch_dir, "lib")])
-    if _stale(LIB, objs + [__file__]):
-        # Shared cudart: callers (torch, or a brotensor runtime) hand in stream
-        # handles created by THEIR CUDA runtime; one shared runtime instance
-        # per process is what makes those handles valid here too.
-        run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", LIB] + objs +
-            ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
-    if _stale(CHECKED_LIB, cobjs + [__file__]):
-        run([nvcc] + ARCH + ["-shared", "-cudart", "shared", "-o", CHECKED_LIB] + cobjs +
-            ["-Xlinker", "-rpath,/usr/local/cuda/lib64"])
-
-    bridge_src = os.path.join(CSRC, "dsine_ops_b200.cpp")
-    if os.path.exists(bridge_src):
-        deps = [bridge_src, LIB] + headers + glob.glob(os.path.join(CSRC, "brotensor_shim", "*", "*.h"))
-        if _stale(BRIDGE, deps):
-            cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
-            cuda_inc = os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")
-            cmd = [cxx, "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", "-Wextra",
-                   "-I" + os.path.join(CSRC, "brotensor_shim"), "-I" + os.path.join(ROOT, "include"),
-                   "-I" + cuda_inc, "-DBVML_SHIM_CUDA", bridge_src, "-o", BRIDGE,
-                   "-L" + LIB_DIR, "-lbvml_dsine", "-Wl,-rpath,$ORIGIN",
-                   "-L" + os.path.join(os.path.dirname(os.path.dirname(nvcc)), "lib64"), "-lcudart", "-Wl,--exclude-libs,ALL"]
-            run(cmd)
-    return LIB
 
 
 if __name__ == "__main__":

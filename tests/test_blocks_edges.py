@@ -1,5 +1,6 @@
 """CPU tests of the feed-forward operators at the edges of what their documents allow."""
 import ctypes
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -170,3 +171,58 @@ def test_the_binding_belongs_to_one_torch_and_python(monkeypatch):
     monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "cpython-27-x")
     with pytest.raises(ImportError, match="not built for torch"):
         blocks._load_binding()
+
+
+@pytest.fixture
+def fake_build(tmp_path, monkeypatch):
+    """The build script with its outputs under tmp_path and its commands recorded, not run;
+    fake_build.fails: a text whose commands fail."""
+    spec = importlib.util.spec_from_file_location("fake_build", os.path.join(
+        os.path.dirname(os.path.abspath(bv.__file__)), "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    for name in [n for n in vars(build) if n.isupper()]:
+        v = getattr(build, name)
+        if isinstance(v, str) and name not in ("HERE", "ROOT", "CSRC", "BLOCKS"):
+            monkeypatch.setattr(build, name, str(tmp_path / os.path.relpath(v, build.HERE)))
+    build.done, build.fails = [], "nothing"
+
+    def run(cmd, **kw):
+        build.done.append(cmd)
+        bad = any(build.fails in a for a in cmd)
+        if not bad:
+            open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, int(bad), "", "no")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "_nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    return build
+
+
+def test_build_without_torch(fake_build, monkeypatch, capsys):
+    """The C and C++ libraries need no torch: the binding alone is left out."""
+    monkeypatch.setattr(fake_build.importlib.util, "find_spec", lambda name: None)
+    fake_build.build()
+    for lib in (fake_build.LIB, fake_build.CHECKED_LIB, fake_build.BRIDGE, fake_build.BLOCKS_LIB,
+                fake_build.BLOCKS_CHECKED_LIB):
+        assert os.path.exists(lib)
+    assert "binding is left out" in capsys.readouterr().err
+    assert not any("blocks_torch" in a for cmd in fake_build.done for a in cmd)
+
+
+@pytest.mark.parametrize("fails", ["blocks_torch.cpp", "gemm_tile_nt.cu"])
+def test_build_makes_the_refinement_first(fake_build, fails):
+    """What fails in the feed-forward operators' part is an error, after the refinement's
+    libraries are there."""
+    fake_build.fails = fails
+    with pytest.raises(RuntimeError, match=fails):
+        fake_build.build()
+    assert all(os.path.exists(p) for p in (fake_build.LIB, fake_build.CHECKED_LIB,
+                                           fake_build.BRIDGE))
+    fake_build.fails, fake_build.done = "nothing", []
+    fake_build.build()
+    assert os.path.exists(fake_build.BLOCKS_LIB)
+    assert os.path.exists(fake_build.blocks_torch_path(torch.__version__))
+    fake_build.done = []
+    fake_build.build()
+    assert not fake_build.done  # all of it is up to date
