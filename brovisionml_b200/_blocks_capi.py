@@ -19,6 +19,7 @@ BVML_EWORKSPACE = 4
 
 # Every symbol include/bvml_blocks.h declares (checked by the CPU test suite).
 EXPORTS = ("bvml_blocks_last_error", "bvml_blocks_version", "bvml_blocks_status",
+           "bvml_blocks_wait_limit",
            "bvml_rms_norm", "bvml_rms_norm_e4m3", "bvml_rms_norm_backward",
            "bvml_rms_norm_backward_workspace_bytes", "bvml_linear",
            "bvml_linear_workspace_bytes", "bvml_linear_backward",
@@ -77,6 +78,7 @@ def _bind(name, restype, argtypes):
 last_error = _bind("bvml_blocks_last_error", ctypes.c_char_p, [])
 _bind("bvml_blocks_version", _i, [])
 status = _bind("bvml_blocks_status", _i, [_vp])
+_bind("bvml_blocks_wait_limit", ctypes.c_uint, [ctypes.c_uint])
 _bind("bvml_rms_norm", _i, [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _f, _vp, _ll, _vp,
                                     _ll, _vp])
 _bind("bvml_rms_norm_e4m3", _i, [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _f, _vp,

@@ -396,6 +396,8 @@ int bvml_blocks_status(void* stream) {
     return finish(cudaSuccess, "");
 }
 
+unsigned bvml_blocks_wait_limit(unsigned attempts) { return gemm_wait_limit(attempts); }
+
 int bvml_rms_norm(const void* x, long long ldx, const void* residual, long long ldr,
                   const void* weight, int T, int K, int dtype, int weight_dtype, float eps,
                   void* y, long long ldy, void* sum, long long lds, void* stream) {

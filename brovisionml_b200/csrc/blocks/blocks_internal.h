@@ -77,6 +77,9 @@ size_t gemm_workspace_bytes(const GemmLaunch& L);
 cudaError_t launch_gemm(const GemmLaunch& L, void* workspace, cudaStream_t s);
 // 0, or what a bounded wait that gave up recorded; resets it (synchronous).
 cudaError_t gemm_errors(int* word);
+// Attempts of each wait between a kernel's roles for the launches that follow, in every
+// thread; returns those before. Waits for what is in flight keep a limit of their own.
+uint32_t gemm_wait_limit(uint32_t attempts);
 
 // -------------------------------------------------- the products' derivatives
 // dz = dy act'(z) (T, N) of `type` into dz (row stride lddz) unless dz is null,

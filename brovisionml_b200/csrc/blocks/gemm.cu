@@ -16,6 +16,9 @@ namespace {
 // a workspace's size needs no device; the launch takes the device's own count.
 constexpr int kPairs = 74;
 
+constexpr uint32_t kWaitLimit = 1u << 22;
+std::atomic<uint32_t> g_wait_limit{kWaitLimit};
+
 // An operand as stored: rows x cols, cols contiguous.
 struct Stored {
     const void* p;
@@ -363,6 +366,7 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     a.rows0 = L.rows0, a.rows1 = L.rows1;
     a.out_rows = L.out2 ? L.rows0 : L.M;
     a.out_type = L.out_type, a.act = L.act;
+    a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
     // the epilogue's matrices, or their places in the workspace
     auto place = [&](const Moved& m, const void* ptr) {
         return m.on ? static_cast<char*>(ws) + m.at : static_cast<char*>(const_cast<void*>(ptr));
@@ -435,6 +439,8 @@ cudaError_t launch_gemm(const GemmLaunch& L, void* ws, cudaStream_t s) {
     if (L.out_type == BVML_BF16) return join<__nv_bfloat16>(L, p, a.slab, vec, s);
     return join<float>(L, p, a.slab, vec, s);
 }
+
+uint32_t gemm_wait_limit(uint32_t attempts) { return g_wait_limit.exchange(attempts); }
 
 cudaError_t gemm_errors(int* word) {
     *word = 0;

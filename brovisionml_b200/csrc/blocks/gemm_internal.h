@@ -55,6 +55,7 @@ struct TileArgs {
     int rows0, rows1;
     int out_rows;  // rows of out, and of out2 where there is one
     int out_type, act, vec;
+    uint32_t wait_limit;  // attempts of a wait between the kernel's roles (gemm_wait_limit)
     float* slab;  // splits > 1: (splits, M, ldslab) fp32 partial sums
     long long ldslab;
 };

@@ -212,9 +212,9 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
     pdl_wait();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-    auto fail = [&](int code) { atomicExch(&g_tile_error, code); };
-    auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {  // a whole warp's wait
-        const bool done = tc::mbar_wait_pipe(bar, parity, kTileWaitLimit);
+    auto fail = [&](int code) { atomicCAS(&g_tile_error, 0, code); };
+    auto wait_all = [&](uint32_t bar, uint32_t parity, uint32_t limit, int code) {  // a warp's
+        const bool done = tc::mbar_wait_pipe(bar, parity, limit);
         if (__all_sync(0xffffffffu, done)) return true;
         if (lane == 0) fail(code);
         return false;
@@ -224,10 +224,10 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
         int i = 0, slot = 0;
         uint32_t phase = 1;
         for (int k = k0; k < k1; ++k, ++i) {
-            if (!wait_all(bar_empty + 8 * slot, phase, 11)) break;
-            tc::mbar_expect_tx_on(on, bar_full + 8 * slot, kStage);
+            if (!wait_all(bar_empty + 8 * slot, phase, a.wait_limit, 11)) break;
             const uint32_t d = sbase + slot * kStage;
             if (!tc::copy_ok(d, k * kStep, 128 / kStep, false, 0)) break;
+            tc::mbar_expect_tx_on(on, bar_full + 8 * slot, kStage);
             tc::tma_load_2d(on, d, &maps.b[0], bar_full + 8 * slot, k * kStep, f0);
             if constexpr (GATED)
                 tc::tma_load_2d(on, d + 8192, &maps.b[1], bar_full + 8 * slot, k * kStep, f0);
@@ -236,7 +236,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
         }
         // no copy may still be landing when the ring is used anew
         for (int q = i > kStages ? i - kStages : 0; q < i; ++q)
-            if (!wait_all(bar_full + 8 * (q % kStages), (q / kStages) & 1, 12)) break;
+            if (!wait_all(bar_full + 8 * (q % kStages), (q / kStages) & 1, kTileWaitLimit, 12)) break;
     } else if (warp == 1) {
         const uint32_t on = tc::elect_one();
         int slot = 0;
@@ -244,7 +244,7 @@ skinny_kernel(const __grid_constant__ TileMaps maps, const SkinnyArgs sa) {
         const uint64_t dw0 = tc::umma_desc_k_sw128(sbase);
         const uint64_t dx0 = tc::umma_desc_k_sw128(sbase + 128 * 128);
         for (int k = k0; k < k1; ++k) {
-            if (!wait_all(bar_full + 8 * slot, phase, 13)) break;
+            if (!wait_all(bar_full + 8 * slot, phase, a.wait_limit, 13)) break;
             tc::tc_fence_after();
             const uint64_t dw = dw0 + (uint32_t)(slot * (kStage >> 4));
             const uint64_t dx = dx0 + (uint32_t)(slot * (kStage >> 4));

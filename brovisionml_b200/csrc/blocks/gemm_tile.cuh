@@ -24,8 +24,9 @@
 // transposed copy. A second segment of K steps with tensors of its own adds
 // the other half of the gated backward's dx.
 //
-// Every wait is bounded; one that gives up records an error and both CTAs tear
-// down, meeting at a cluster barrier before either leaves.
+// Every wait is bounded (TileArgs::wait_limit); one that gives up records an error and stops
+// the roles of both CTAs. They meet at a cluster barrier, wait for what is still in flight,
+// bounded again, and neither leaves or frees TMEM before that.
 //
 // Bound by the tensor cores where K is long (87 % busy at 4096 x 4096 x 8192, and then
 // by the power limit: 8192 x 4096 x 8192 bf16 takes 334 us alone, 1.65 PFLOP/s, and 435
@@ -359,7 +360,10 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     const uint32_t bar_acc_empty = bars + 144;    // 2, the first CTA's
     const uint32_t bar_end = bars + 160;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_mem + 168);
+    // words that both CTAs write or read when they tear down
     int* abort_flag = reinterpret_cast<int*>(bar_mem + 172);
+    const uint32_t issued = bars + 176;     // ring entries issued by each CTA, the first CTA's
+    const uint32_t committed = bars + 184;  // K steps and tiles whose MMAs were, in each CTA
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
@@ -418,14 +422,14 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     auto fail = [&](int code) {
-        atomicExch(&g_tile_error, code);
-        *reinterpret_cast<volatile int*>(abort_flag) = 1;
+        atomicCAS(&g_tile_error, 0, code);  // the first one
+        for (uint32_t r = 0; r < 2; ++r) tc::st_cluster(tc::map_to(bars + 172, r), 1);
     };
     auto aborted = [&]() { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
 
     // A wait of a whole warp: every lane polls, and they agree.
     auto wait_all = [&](uint32_t bar, uint32_t parity, int code) {
-        const bool done = tc::mbar_wait_pipe(bar, parity, kTileWaitLimit);
+        const bool done = tc::mbar_wait_pipe(bar, parity, a.wait_limit);
         if (__all_sync(0xffffffffu, done)) return true;
         if (lane == 0) fail(code);
         return false;
@@ -450,7 +454,6 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                     ok = false;
                     break;
                 }
-                tc::mbar_expect_tx_on(first_on, bar_full + 8 * slot, 2 * kStage);
                 const uint32_t full = full0 + 8 * slot;
                 const uint32_t sa = sbase + slot * kStage, sb = sa + 128 * 128;
                 const int seg = k >= a.steps[0];
@@ -460,6 +463,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                     ok = false;
                     break;
                 }
+                tc::mbar_expect_tx_on(first_on, bar_full + 8 * slot, 2 * kStage);
                 if constexpr (AT) {
                     tc::tma_load_2d_pair(on, sa, &maps.a[seg], full, m0, x);
                     tc::tma_load_2d_pair(on, sa + 8192, &maps.a[seg], full, m0 + 64, x);
@@ -483,21 +487,26 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
             }
         }
         // nothing may still arrive in shared memory when the pair leaves: the last
-        // round's entries have been consumed and handed back (to both CTAs);
-        // after an abort the copies at least have landed (the first CTA's
-        // barriers count both CTAs' bytes)
-        const int q0 = i > kStages ? i - kStages : 0;
-        for (int q = q0; ok && q < i; ++q)
-            ok = wait_all(bar_empty + 8 * (q % kStages), (q / kStages) & 1, 2);
-        if (!ok && rank == 0)
-            for (int q = q0; q < i; ++q)
-                if (!wait_all(bar_full + 8 * (q % kStages), (q / kStages) & 1, 2)) break;
+        // round's entries have been consumed and handed back (to both CTAs), or, where a
+        // wait gave up, the teardown below waits for them
+        for (int q = i > kStages ? i - kStages : 0; ok && q < i; ++q) {
+            uint32_t n = kTileWaitLimit / 1024;
+            bool done = false;
+            while (!done && n-- && !gone())
+                done = __all_sync(0xffffffffu,
+                                  tc::mbar_wait_pipe(bar_empty + 8 * (q % kStages),
+                                                     (q / kStages) & 1, 1024));
+            if (!done && lane == 0) fail(2);
+            ok = done;
+        }
+        if (lane == 0) tc::st_cluster(tc::map_to(issued + 4 * rank, 0), i);
     } else if (warp == 1) {
         if (rank == 0) {
             // ----------------------------------------------------------- MMA
             const uint32_t on = tc::elect_one();
             int slot = 0, tl = 0;
             uint32_t parity = 0;
+            int done_steps = 0, done_tiles = 0;
             bool ok = true;
             const uint64_t da0 = AT ? tc::umma_desc_mn_sw128(sbase, 8192)
                                     : tc::umma_desc_k_sw128(sbase);
@@ -525,13 +534,22 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                         tc::umma_pair<F8>(on, acc, da + q * (AT ? 128 : 2),
                                           db + q * (BT ? 128 : 2), a.idesc, k > k0 || q > 0);
                     tc::umma_commit_pair(on, bar_empty + 8 * slot);
+                    ++done_steps;
                     if (++slot == kStages) slot = 0, parity ^= 1;
                 }
-                if (ok) tc::umma_commit_pair(on, bar_acc_full + 8 * buf);
+                if (ok) {
+                    tc::umma_commit_pair(on, bar_acc_full + 8 * buf);
+                    ++done_tiles;
+                }
             }
             // every issued MMA has completed, after an abort too
             tc::umma_commit_pair_local(on, bar_end);
-            wait_all(bar_end, 0, 5);
+            if (!tc::mbar_wait(bar_end, 0, kTileWaitLimit)) fail(5);
+            __syncwarp();
+            if (lane < 2) {
+                tc::st_cluster(tc::map_to(committed, lane), done_steps);
+                tc::st_cluster(tc::map_to(committed + 4, lane), done_tiles);
+            }
         }
     } else {
         // ------------------------------------------------------------ epilogue
@@ -654,7 +672,30 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
         if (lane == 0) tc::bulk_wait_all();  // before shared memory goes
     }
     __syncthreads();
-    tc::cluster_sync();  // the pair's copies, MMAs and arrivals are all done
+    // The pair's MMAs and stores are done, and, unless a wait gave up, its copies and
+    // arrivals.
+    tc::cluster_sync();
+    if (warp == 0 && gone()) {
+        const volatile int* words = reinterpret_cast<volatile int*>(bar_mem + 176);
+        // arrivals of the MMAs' commits on this CTA's barriers
+        const int steps_done = words[2], tiles_done = words[3];
+        for (int q = steps_done > kStages ? steps_done - kStages : 0; q < steps_done; ++q)
+            tc::mbar_wait_landed(bar_empty + 8 * (q % kStages), (q / kStages) & 1);
+        for (int j = tiles_done > 2 ? tiles_done - 2 : 0; j < tiles_done; ++j)
+            tc::mbar_wait_landed(bar_acc_full + 8 * (j & 1), (j >> 1) & 1);
+        // Copies of both CTAs, counted here: entries before the last kStages that either
+        // issued have been consumed. One that only one CTA issued is made up to what its
+        // phase expects.
+        const int n0 = words[0], n1 = words[1], n = n0 > n1 ? n0 : n1;
+        for (int q = rank == 0 ? (n > kStages ? n - kStages : 0) : n; q < n; ++q) {
+            const uint32_t full = bar_full + 8 * (q % kStages);
+            if (lane == 0 && q >= n0) tc::mbar_expect_tx(full, kStage);
+            if (lane == 0 && q >= n1) tc::mbar_complete_tx(full, kStage);
+            __syncwarp();
+            tc::mbar_wait_landed(full, (q / kStages) & 1);
+        }
+    }
+    __syncwarp();
     if (warp == 1) tc::tmem_dealloc_pair(tmem, kCols);
     tc::cluster_sync();
 }

@@ -52,6 +52,24 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote) {
                  : "memory");
 }
 
+__device__ __forceinline__ void st_cluster(uint32_t remote, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+// Counts bytes on a barrier of this CTA as if a copy had brought them.
+__device__ __forceinline__ void mbar_complete_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+// A wait of teardown after another wait gave up: what is in flight lands within
+// microseconds, and some 10 ms are waited for at most.
+__device__ __forceinline__ bool mbar_wait_landed(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < 1 << 16; ++i) {
+        if (mbar_wait_pipe(bar, parity, 1)) return true;
+        __nanosleep(100);
+    }
+    return false;
+}
+
 // Checked builds (-DBVML_CHECKED): a copy whose innermost coordinate or shared-memory
 // address is off its alignment, or a store at a negative coordinate, is recorded and left
 // out. `inner`: bytes of an element.

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import brovisionml_b200 as bv
+from brovisionml_b200 import _blocks_capi as B
 from test_gpu_blocks import BF16, E, E4M3, F16, F32, quantized, rnd
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +108,57 @@ def test_derivatives_far_from_zero(act, dt):
     nan = torch.full_like(one, float("nan"))
     _, _, db = bv.linear_backward(one, x, w, nan, act=act, bias=True, dx=False, dw=False)
     assert db.isnan().all()
+
+
+def _waits(case):
+    """(a call and its outputs) for a kernel of the products."""
+    T, K, N = case["size"]
+    x, w, w2, dy = (rnd(*s, dt=BF16, scale=0.1, seed=i) for i, s in
+                    enumerate([(T, K), (N, K), (N, K), (T, N)]))
+    if case["op"] == "linear":
+        return lambda: (bv.linear(x, w),)
+    if case["op"] == "gated":
+        return lambda: (bv.gated_linear(x, w, w2),)
+    if case["op"] == "backward":
+        return lambda: bv.linear_backward(dy, x, w)[:2]
+    (q, s), (v, t) = quantized(T, K, 0), quantized(N, K, 1)
+    return lambda: (bv.linear(q, v, x_scale=s, w_scale=t),)
+
+
+@pytest.mark.parametrize("case", [
+    dict(op="linear", size=(5, 4096, 1000)),  # few rows, K over a cluster
+    dict(op="gated", size=(100, 2048, 600)),
+    dict(op="e4m3", size=(60, 4096, 500)),
+    dict(op="linear", size=(520, 64, 264)),  # tiles: fewer K steps than the ring holds
+    dict(op="linear", size=(520, 2048, 1032)),
+    dict(op="linear", size=(200, 4096, 256)),  # shares of K
+    dict(op="gated", size=(1300, 320, 4000)),  # several tiles a pair
+    dict(op="e4m3", size=(3000, 640, 2600)),
+    dict(op="backward", size=(2900, 2900, 264)),
+], ids=lambda c: f"{c['op']}-{'x'.join(map(str, c['size']))}")
+def test_waits_that_give_up(case):
+    """A short limit on the waits between a product's copies, MMAs and epilogue: the call
+    ends, the status tells of it, and the next call on the stream is what it was. With one
+    attempt the first MMA never finds its operands; with more the waits that give up are
+    spread over the kernel, or none does and the result stands."""
+    call = _waits(case)
+    bv.blocks_status()
+    want = call()
+    bv.blocks_status()
+    limit = B.blocks_lib.bvml_blocks_wait_limit
+    for attempts in (1, 2, 3, 5, 9, 17, 33):
+        assert limit(attempts) == 4194304
+        try:
+            got, gave_up = call(), False
+            torch.cuda.synchronize()
+            try:
+                bv.blocks_status()
+            except RuntimeError as e:
+                assert "pipeline gave up" in str(e)
+                gave_up = True
+        finally:
+            limit(4194304)
+        assert gave_up or attempts > 1
+        assert gave_up or all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(call(), want)), attempts
+        bv.blocks_status()
