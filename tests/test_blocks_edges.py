@@ -13,7 +13,7 @@ import torch.autograd.forward_ad as fwad
 
 import brovisionml_b200 as bv
 from brovisionml_b200 import _blocks_capi as B
-from test_blocks_api import BF16, E4M3, EINVAL, at, err, gated_args, linear_args
+from test_blocks_api import (BF16, E4M3, EINVAL, EWORKSPACE, at, err, gated_args, linear_args)
 
 
 @pytest.mark.parametrize("x,x_scale", [(None, None), (at(0), at(5))])
@@ -226,3 +226,26 @@ def test_build_makes_the_refinement_first(fake_build, fails):
     fake_build.done = []
     fake_build.build()
     assert not fake_build.done  # all of it is up to date
+
+
+def test_neighbouring_columns_of_one_buffer_are_accepted():
+    """An output in the columns beside its input (64 + 32 elements of rows of 96), its last
+    byte before the next row and its first after the input's last: past the overlap checks
+    and turned down only for want of a workspace, before any launch. One element nearer to
+    either side is an overlap."""
+    lib = B.blocks_lib
+    # an input on an odd address is laid out anew in the workspace
+    base = at(0) + 2
+
+    def call(off, ldx=96):
+        a = linear_args(x=base, ldx=ldx, ldy=ldx, y=base + off)
+        return (lib.bvml_linear(ctypes.byref(a), None, 0, None),
+                lib.bvml_linear_workspace_bytes(ctypes.byref(a)))
+
+    rc, need = call(128)
+    assert rc == EWORKSPACE and need > 0, err()
+    for off, ldx in ((126, 96), (130, 96), (128, 95), (-62, 96), (-66, 96)):
+        rc, need = call(off, ldx)
+        assert rc == EINVAL and need == 0 and "y overlaps x" in err(), (off, ldx)
+    rc, need = call(-64)  # before it, in the columns of the row before
+    assert rc == EWORKSPACE and need > 0, err()

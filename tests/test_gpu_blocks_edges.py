@@ -5,7 +5,8 @@ import torch
 
 import brovisionml_b200 as bv
 from brovisionml_b200 import _blocks_capi as B
-from test_gpu_blocks import BF16, E, E4M3, F16, F32, quantized, rnd
+from test_gpu_blocks import (ACTS, BF16, E, E4M3, F16, F32, close, grads, product, quantized,
+                             rnd)
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +163,97 @@ def test_waits_that_give_up(case):
         assert gave_up or all(torch.equal(a, b) for a, b in zip(got, want))
         assert all(torch.equal(a, b) for a, b in zip(call(), want)), attempts
         bv.blocks_status()
+
+
+# More tiles than pairs of SMs (74): every pair takes several, over both accumulators, with
+# the ring's state going on from tile to tile.
+MANY = [(3000, 200, 2600), (1300, 72, 5000), (20000, 136, 520)]
+
+
+@pytest.mark.parametrize("T,K,N", MANY)
+@pytest.mark.parametrize("dt,out,act,whole", [(BF16, None, "none", True), (F16, F32, "gelu", False),
+                                              (E4M3, BF16, "none", True), (E4M3, F32, "silu", False),
+                                              (E4M3, F16, "relu", True)])
+def test_linear_of_many_tiles(T, K, N, dt, out, act, whole):
+    if dt == E4M3:
+        (x, xs), (w, ws) = quantized(T, K, 0), quantized(N, K, 1, K ** -0.5)
+        ref, tol = product(x, w, xs, ws)
+        scales = dict(x_scale=xs, w_scale=ws)
+    else:
+        x, w, scales = rnd(T, K, dt=dt), rnd(N, K, dt=dt, scale=K ** -0.5, seed=1), {}
+        ref, tol = product(x, w)
+    b = rnd(N, seed=2)
+    r = None if whole else rnd(T, N, dt=out or dt, seed=3)
+    y = bv.linear(x, w, b, act=act, residual=r, out_dtype=out, **scales)
+    ref = ref + b.double()
+    val = ACTS[act][0](ref) + (0 if whole else r.double())
+    close(y, val, 1.13 * tol + 16 * E * (ref.abs() + val.abs() + 1))
+    assert torch.equal(bv.linear(x, w, b, act=act, residual=r, out_dtype=out, **scales), y)
+    bv.blocks_status()
+
+
+@pytest.mark.parametrize("T,K,F", MANY)
+@pytest.mark.parametrize("dt", [BF16, E4M3])
+def test_gated_linear_of_many_tiles(T, K, F, dt):
+    if dt == E4M3:
+        (x, xs), (wg, gs), (wu, us) = (quantized(T, K, 0), quantized(F, K, 1, K ** -0.5),
+                                       quantized(F, K, 2, K ** -0.5))
+        scales = dict(x_scale=xs, gate_scale=gs, up_scale=us)
+        (rg, tg), (ru, tu) = product(x, wg, xs, gs), product(x, wu, xs, us)
+    else:
+        x, scales = rnd(T, K, dt=dt), {}
+        wg, wu = (rnd(F, K, dt=dt, scale=K ** -0.5, seed=s) for s in (1, 2))
+        (rg, tg), (ru, tu) = product(x, wg), product(x, wu)
+    h, g, u = bv.gated_linear(x, wg, wu, save=True, **scales)
+    close(g, rg, tg + 4 * E * rg.abs(), "g")
+    close(u, ru, tu + 4 * E * ru.abs(), "u")
+    a = ACTS["silu"][0](rg)
+    close(h, a * ru, 1.13 * tg * (ru.abs() + tu) + a.abs() * tu + 16 * E * (rg.abs() + 1) * ru.abs())
+    assert torch.equal(bv.gated_linear(x, wg, wu, **scales), h)
+    bv.blocks_status()
+
+
+@pytest.mark.parametrize("T,K,N", [(264, 2700, 2700), (2700, 2700, 264), (130, 5000, 1300)])
+def test_gradients_of_many_tiles(T, K, N):
+    dt = BF16
+    x, dy = rnd(T, K, dt=dt), rnd(T, N, dt=dt, seed=2)
+    w, w2 = (rnd(N, K, dt=dt, scale=K ** -0.5, seed=s) for s in (1, 3))
+    dx, dw, _ = bv.linear_backward(dy, x, w)
+    rx, tx, rw, tw = grads(dy, w, x, 0.0)
+    close(dx, rx, tx, "dx")
+    close(dw, rw, tw, "dw")
+    g, u = rnd(T, N, dt=dt, seed=4), rnd(T, N, dt=dt, seed=5)
+    dx, dwg, dwu = bv.gated_linear_backward(dy, x, w, w2, g, u, act="relu")
+    # relu's dg and du are one product and one selection: rounded to 16 bits once, exact in 32
+    dg = torch.where(g > 0, dy.float() * u.float(), 0).to(dt)
+    du = torch.where(g > 0, dy.float() * g.float(), 0).to(dt)
+    gx, tgx, gw, tgw = grads(dg, w, x, 0.0)
+    ux, tux, uw, tuw = grads(du, w2, x, 0.0)
+    # one sum over both halves: up to twice either's number of terms
+    close(dx, gx + ux, 2 * (tgx + tux), "dx")
+    close(dwg, gw, tgw, "dw_gate")
+    close(dwu, uw, tuw, "dw_up")
+    bv.blocks_status()
+
+
+@pytest.mark.parametrize("T,K,N", [(130, 1, 1), (300, 3, 2), (520, 2, 7), (140, 1, 300),
+                                   (140, 300, 1)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_many_rows_of_few_features(T, K, N, dt):
+    """Widths below a store of 16 bytes on the tile kernels, forward and backward."""
+    x, dy = rnd(T, K, dt=dt), rnd(T, N, dt=dt, seed=2)
+    w, w2 = rnd(N, K, dt=dt, seed=1), rnd(N, K, dt=dt, seed=3)
+    ref, tol = product(x, w)
+    close(bv.linear(x, w), ref, tol)
+    ru, tu = product(x, w2)
+    g, u = bv.gated_linear(x, w, w2, save=True)[1:]
+    close(g, ref, tol)
+    close(u, ru, tu)
+    dx, dw, db = bv.linear_backward(dy, x, w, bias=True)
+    rx, tx, rw, tw = grads(dy, w, x, 0.0)
+    close(dx, rx, tx)
+    close(dw, rw, tw)
+    close(db, dy.double().sum(0), (T + 32) * E * dy.double().abs().sum(0))
+    (q, s), (v, t) = quantized(T, K, 4), quantized(N, K, 5)
+    ref, tol = product(q, v, s, t)
+    close(bv.linear(q, v, x_scale=s, w_scale=t, out_dtype=F32), ref, tol + 4 * E * ref.abs())
