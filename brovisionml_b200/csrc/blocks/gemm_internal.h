@@ -31,8 +31,8 @@ inline Division divide_by(uint32_t d) {
 
 // TileArgs::vec
 enum : int {
-    kOn16 = 1,     // every row, and every vector over columns, starts on 16 bytes, and an
-                   // output's row ends there
+    kOn16 = 1,     // few rows: every row and every vector over columns starts on 16 bytes (for
+                   // the tiles always, and an output's row ends there)
     kWideSave = 2  // save's on 32
 };
 

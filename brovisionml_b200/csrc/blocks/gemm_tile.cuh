@@ -222,22 +222,16 @@ __device__ __forceinline__ float value_one(const TileArgs& a, long long m, int n
     return v;
 }
 
-// Chunks at the right edge, and rows that start on no 16 bytes (`store`: their outputs
-// go straight to memory): one element after the other, out of line.
+// Chunks at the right edge: one element after the other, out of line.
 template <bool GATED>
 __device__ __noinline__ void finish_slowly(const TileArgs& a, int m, int n, float* v,
-                                           const float* u, bool store) {
+                                           const float* u) {
     const int left = a.N - n < kW ? a.N - n : kW;
-    for (int i = 0; i < left; ++i) {
-        const float o = value_one<GATED>(a, m, n + i, v[i], GATED ? u[i] : 0.0f);
-        v[i] = o;
-        if (!store) continue;
-        if (!a.out2 || m < a.rows0) put_one(a.out, m * a.ldo + n + i, a.out_type, o);
-        else if (m >= a.rows1) put_one(a.out2, (m - a.rows1) * a.ldo2 + n + i, a.out_type, o);
-    }
+    for (int i = 0; i < left; ++i)
+        v[i] = value_one<GATED>(a, m, n + i, v[i], GATED ? u[i] : 0.0f);
 }
 
-// Epilogue of columns n .. n + kW - 1 of row m, all inside and on 16 bytes, v <- their
+// Epilogue of columns n .. n + kW - 1 of row m, all inside, v <- their
 // outputs; raw: the residual's, c: the columns' scales (the gate's) or, without any,
 // biases. GRAD: a backward product, whose output is the sum itself.
 template <bool F8, bool GATED, bool GRAD, int OUT>
@@ -564,11 +558,9 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
         uint8_t* stg = smem + kStages * kStage + (warp - 2) * 4096 * kBufs;
         int filled = 0;  // boxes staged by this warp
         const uint32_t acc_empty0 = tc::map_to(bar_acc_empty, 0);
-        // rows on 16 bytes take the short path
-        const bool fast = (a.vec & kOn16) != 0;
-        const bool whole = !GATED && fast && !a.slab && !a.save[0] && !a.residual;
-        const bool ahead = !GATED && !BT && fast && a.residual;
-        const float* cols = !fast || BT || whole ? nullptr : F8 ? a.col_scale[0] : a.bias;
+        const bool whole = !GATED && !a.slab && !a.save[0] && !a.residual;
+        const bool ahead = !GATED && !BT && a.residual;
+        const float* cols = BT || whole ? nullptr : F8 ? a.col_scale[0] : a.bias;
         int tl = 0;
         for (int w = pair; w < works; w += pairs, ++tl) {
             int m0, n0, k0, k1, split;
@@ -638,7 +630,7 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                             put_row(a.slab + ((long long)split * a.M + m) * a.ldslab + n, v, true);
                         continue;
                     }
-                    if (__builtin_expect(fast && n + kW <= a.N, 1)) {
+                    if (__builtin_expect(n + kW <= a.N, 1)) {
                         if (in)
                             finish_row<F8, GATED, BT, OUT>(a, m, n, v, g, row_scale, now, cnow);
                     } else if (in) {
@@ -648,13 +640,13 @@ gemm_tile_kernel(const __grid_constant__ TileMaps maps, const TileArgs a) {
                         for (int i = 0; i < kW; ++i) tv[i] = v[i];
 #pragma unroll
                         for (int i = 0; i < (GATED ? kW : 1); ++i) tg[i] = g[i];
-                        finish_slowly<GATED>(a, m, n, tv, tg, !fast);
+                        finish_slowly<GATED>(a, m, n, tv, tg);
 #pragma unroll
                         for (int i = 0; i < kW; ++i) v[i] = tv[i];
                     }
-                    if (fast) stage_row<T>(box, lane, c / kW, v);
+                    stage_row<T>(box, lane, c / kW, v);
                 }
-                if (!fast || (!GATED && a.slab)) continue;
+                if (!GATED && a.slab) continue;
                 tc::fence_proxy_async_smem();
                 __syncwarp();
                 const int n = n0 + b * kBox;

@@ -10,7 +10,8 @@
  *    a pointer and a row stride `ld` in elements (>= the columns); its last
  *    axis is contiguous. Pointers are aligned to their element. Rows that
  *    start on 16 bytes (pointer and stride) are read in place; others are
- *    accepted and laid out anew in the workspace first. Outputs of the
+ *    accepted and laid out anew in the workspace first, as are vectors over
+ *    output features (bias, scales) that do not. Outputs of the
  *    products whose rows do not start and end on 16 bytes likewise go through
  *    the workspace. The *_workspace_bytes calls look at the pointers'
  *    alignment, so they take the arguments of the call itself.

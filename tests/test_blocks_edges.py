@@ -249,3 +249,23 @@ def test_neighbouring_columns_of_one_buffer_are_accepted():
         assert rc == EINVAL and need == 0 and "y overlaps x" in err(), (off, ldx)
     rc, need = call(-64)  # before it, in the columns of the row before
     assert rc == EWORKSPACE and need > 0, err()
+
+
+@pytest.mark.parametrize("vector", ["bias", "w_scale", "gate_scale", "up_scale"])
+def test_vectors_off_16_bytes_go_through_the_workspace(vector):
+    """A bias or scales that start on no 16 bytes are laid out anew like rows that do not (in
+    place they would be read one element after the other); few rows read them as they are."""
+    lib = B.blocks_lib
+    if vector in ("gate_scale", "up_scale"):
+        make, name = gated_args, "bvml_gated_linear"
+        kw = dict(in_type=E4M3, x_scale=at(6), gate_scale=at(7), up_scale=at(8))
+    else:
+        make, name = linear_args, "bvml_linear"
+        kw = dict(in_type=E4M3, x_scale=at(6), w_scale=at(7), bias=at(8))
+    size, fn = getattr(lib, name + "_workspace_bytes"), getattr(lib, name)
+    assert size(ctypes.byref(make(T=300, **kw))) == 0
+    kw[vector] += 4
+    a = make(T=300, **kw)
+    assert size(ctypes.byref(a)) == 256  # 32 floats
+    assert fn(ctypes.byref(a), None, 0, None) == EWORKSPACE
+    assert size(ctypes.byref(make(T=7, **kw))) == 0
