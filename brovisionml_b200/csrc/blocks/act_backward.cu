@@ -6,7 +6,10 @@
 // 2048 columns and walks rows, the next rows' loads in flight; a thread keeps eight
 // columns' sums in registers. The sums over a block's rows and over blocks run in
 // a fixed order. What the matrix products read back (dz, dg, du) is rounded to 16
-// bits, the type the tensor cores take; the bias gradient sums the 32-bit values.
+// bits, the type the tensor cores take, which makes the gradients' error against 64 bits 1.41
+// times that of one rounding at the end (fp16 2.1e-4 -> 2.9e-4 of their size, bf16 1.7e-3 ->
+// 2.3e-3); what the rounding leaves over, as a second operand, would double the products.
+// The bias gradient sums the 32-bit values.
 //
 // Bound by HBM where the rows are many (gated, 8191 x 5632: 80 us, 5.8 TB/s), by
 // issuing (26 instructions an element) where L2 holds them (4099 x 2056 fp16: 14 us).

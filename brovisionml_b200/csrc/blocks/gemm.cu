@@ -64,7 +64,9 @@ int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 // column and 0.7 more a tile (57600 x 128 -> 1024: 32.8, 33.8, 34.4 and 38.4 us with 256,
 // 192, 128 and 64 columns; -> 576: 25.9, 20.7, 23.7 and 23.8), any other twice that.
 // Shares of K are written and read once more (6.5 TB/s), which fewer idle pairs have to
-// earn back.
+// earn back. Where it misses (us, its choice and the best): 57600 x 576 -> 128 18.9 and 16.7
+// with 128 columns, 57600 x 64 -> 192 11.3 and 10.3 with 192, 57600 x 128 -> 1024 34.5 and
+// 32.8 with 256.
 double tile_cost(int tiles, int steps, int splits, int bn, double outputs, bool light) {
     const double rate = (128 + bn / 2) / 256.0;
     const long long turns = ((long long)tiles * splits + kPairs - 1) / kPairs;
@@ -108,9 +110,11 @@ Plan plan_of(const GemmLaunch& L) {
 
     p.splits = 1;
     // Few rows: the kernel that streams the weights, up to 64 rows, and up to 128 where
-    // the weights are many or gated. us at 128 rows, bf16, that kernel and the tiles: 512 x 512
-    // 8.7 and 6.0, 1024 x 8192 14.6 and 12.8, 8192 x 1024 12.4 and 10.0, but 4096 x 4096 14.9 and
-    // 17.2 (65 rows), 11264 x 4096 27 and 28, gated 44 and 53.
+    // the weights are many or gated. us, bf16, N x K, that kernel at 64 rows and the tiles at
+    // 65: 512 x 512 6.5 and 5.5, 8192 x 1024 11.2 and 8.9, 1024 x 8192 11.2 and 11.9 (with bias
+    // and residual, for which the tiles share out no K, 11.6 and 22.7); that kernel at 128 and
+    // the tiles at 129: 4096 x 4096 17.1 and 19.6 (bias and residual 17.7 and 17.0; at 65 rows
+    // that kernel takes 14.3), 11264 x 4096 27.1 and 26.9, gated 43.4 and 52.7.
     const bool many = L.gated || (double)L.N * L.k[0] * (double)es > 20e6;
     if (!L.a_t && !L.b_t && L.M <= (many ? 128 : 64)) {
         p.skinny = true;

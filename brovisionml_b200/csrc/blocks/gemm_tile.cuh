@@ -31,7 +31,7 @@
 // Bound by the tensor cores where K is long (87 % busy at 4096 x 4096 x 8192, and then
 // by the power limit: 8192 x 4096 x 8192 bf16 takes 334 us alone, 1.65 PFLOP/s, and 435
 // in a long row of calls), by writing the output where it is short (57600 x 128 -> 576:
-// 21.8 us; filling 66 MB takes 20.8).
+// 21.6 us; filling those 66 MB takes 20.6).
 #pragma once
 
 #include "blocks_common.cuh"
@@ -286,7 +286,7 @@ __device__ __forceinline__ void load_some(const float* p, int at, int end, float
 
 // A whole box (32 rows x 128 bytes of output) of a product that is not gated, adds no
 // residual and keeps nothing, rows on 16 bytes: all its columns at once, without the
-// chunks' loop. us, and by chunks: 57600 x 128 -> 576 21.8 (32), with relu 25 (38.5), gelu
+// chunks' loop. us, and by chunks: 57600 x 128 -> 576 21.6 (32), with relu 25 (38.5), gelu
 // 49 (58). With a residual it is no faster: 55 (57; 49 through shared memory in whole
 // lines, which costs the others 4). read(): called when TMEM has been read.
 template <bool F8, bool GRAD, int OUT, typename Read>

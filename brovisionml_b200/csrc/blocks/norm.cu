@@ -8,16 +8,19 @@
 //
 // Bound by HBM: every row is read once into registers (G threads a row, VPT
 // groups of eight elements a thread), reduced, and written from there. Rows of
-// up to 1024 features belong to a warp or part of one (no block barrier), longer
+// up to 512 features belong to a warp or part of one (no block barrier), longer
 // ones to a block; beyond 16 Ki features a block walks the row twice, the second
-// time out of L2. A block keeps its weights in registers over its rows, and the
+// time out of L2, an element a thread and load. A block keeps its weights in registers over its rows, and the
 // backward pass its sums of dw, which it writes once: the sums over blocks
 // are a second small kernel, in a fixed order (no atomics).
 //
 // us (TB/s): 57600 x 128 fp16 6.6 (4.5; 6.85 with sums of squares and of the residual
-// element by element and not in pairs), 8197 x 4096 bf16 with residual to 8 bits 41 to
-// 45 (5.2 to 5.7; in pairs its quotients took 2 us longer), backward 16384 x 2048 bf16
-// 52.6 (5.1, the second kernel included); one row of 4096 5.0, the launch.
+// element by element and not in pairs), 8197 x 4096 bf16 with residual to 8 bits 40 to
+// 44 (5.3 to 5.9; in pairs its quotients took 2 us longer), backward 16384 x 2048 bf16
+// 52.9 (5.1, the second kernel included); one row of 4096 5.0, the launch. By width, bf16,
+// T K = 33.5 M, forward and backward: 4096 25.7 (5.2) and 41.7 (4.8), 8192 29.4 and 42.8,
+// 12000 27.4 and 125 (four groups a thread do not fit the registers: 536 bytes spilled),
+// 16384 24.7 and 101, 16392 60.9 (2.2) and 157 (1.3), 20000 77.9 and 161.
 #include "blocks_common.cuh"
 #include "blocks_internal.h"
 
@@ -448,7 +451,7 @@ rms_norm_long_kernel(const NormArgs a) {
 }
 
 // Blocks an SM that the backward pass is built for: 64 registers a thread with
-// one group of eight, twice that with two.
+// one group of eight, twice that with two, and no more with four, which spill.
 constexpr int backward_blocks(int G, int VPT) {
     const int threads = G > 32 ? G : kNormThreads;
     const int n = (VPT == 1 ? 1024 : 512) / threads;

@@ -54,6 +54,7 @@ extern "C" {
 #define BVML_ACT_TANH 3
 #define BVML_ACT_SILU 4 /* z sigmoid(z) */
 #define BVML_ACT_GELU 5 /* z Phi(z), Phi the normal distribution function (erf form) */
+/* sigmoid, Phi and their derivatives are zero where they are below 2^-126 */
 
 const char* bvml_blocks_last_error(void);
 int bvml_blocks_version(void);
@@ -115,7 +116,8 @@ int bvml_rms_norm_backward(const void* dy, long long lddy, const void* s, long l
  * residual (T, N); fp32 accumulation on the tensor cores.
  *   in_type F16 or BF16 (x and w alike), out_type the same or F32; or in_type
  *   E4M3 with x_scale (T) and w_scale (N) fp32, the value of x[t, k] being
- *   x[t, k] x_scale[t], and out_type F16, BF16 or F32.
+ *   x[t, k] x_scale[t], and out_type F16, BF16 or F32. The sum is multiplied by
+ *   x_scale[t] w_scale[n], one fp32 number: it has to be within fp32's normal range.
  *   bias (N) fp32 or NULL; residual of out_type or NULL; z, when not NULL,
  *   gets the pre-activation in out_type (the backward pass takes it).
  */

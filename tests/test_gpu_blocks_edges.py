@@ -257,3 +257,23 @@ def test_many_rows_of_few_features(T, K, N, dt):
     (q, s), (v, t) = quantized(T, K, 4), quantized(N, K, 5)
     ref, tol = product(q, v, s, t)
     close(bv.linear(q, v, x_scale=s, w_scale=t, out_dtype=F32), ref, tol + 4 * E * ref.abs())
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("T", [1, 200])
+def test_activations_far_below_zero(act, T):
+    """Down to 2^-126 the activations keep their figures (an argument's rounding counts |z|, or
+    z^2 with gelu, times 2^-24); below, sigmoid and exp(-z^2 / 2) flush to zero, which is off
+    by |z| 2^-126 at most."""
+    z = torch.cat([torch.linspace(-110, 0, 881), torch.linspace(-14, -8, 97)]).cuda().to(BF16)
+    x = torch.zeros(T, 8, device="cuda", dtype=BF16)
+    x[:, 3] = 1
+    w = torch.zeros(z.numel(), 8, device="cuda", dtype=BF16)
+    w[:, 3] = z
+    y = bv.linear(x, w, act=act, out_dtype=F32).double()
+    v = z.double()
+    ref = {"sigmoid": torch.sigmoid(v), "silu": v * torch.sigmoid(v),
+           "gelu": v * torch.special.erfc(-v / 2 ** 0.5) / 2}[act]
+    arg = v * v if act == "gelu" else v.abs()
+    tol = (4 * arg + 32) * E * ref.abs() + (v.abs() + 1) * 2.0 ** -126 * 1.01
+    assert ((y - ref).abs() <= tol).all()
