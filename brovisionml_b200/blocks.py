@@ -54,6 +54,8 @@ class _Unloaded:
 
     def __getattr__(self, name):
         global _binding
+        if name.startswith("__"):  # somebody looking around, not a call
+            raise AttributeError(name)
         _binding = _load_binding()
         return getattr(_binding, name)
 

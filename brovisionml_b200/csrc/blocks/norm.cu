@@ -10,9 +10,9 @@
 // groups of eight elements a thread), reduced, and written from there. Rows of
 // up to 512 features belong to a warp or part of one (no block barrier), longer
 // ones to a block; beyond 16 Ki features a block walks the row twice, the second
-// time out of L2, an element a thread and load. A block keeps its weights in registers over its rows, and the
-// backward pass its sums of dw, which it writes once: the sums over blocks
-// are a second small kernel, in a fixed order (no atomics).
+// time out of L2, an element a thread and load. A block keeps its weights in registers
+// over its rows, and the backward pass its sums of dw, which it writes once: the sums
+// over blocks are a second small kernel, in a fixed order (no atomics).
 //
 // us (TB/s): 57600 x 128 fp16 6.6 (4.5; 6.85 with sums of squares and of the residual
 // element by element and not in pairs), 8197 x 4096 bf16 with residual to 8 bits 40 to
@@ -260,11 +260,11 @@ __device__ __forceinline__ void row_reduce(float& a, float& b, float (*slots)[3]
 }
 // ... and the largest m (not negative; NaN if one is) with the largest c beside it.
 __device__ __forceinline__ float warp_max_nan(float v) {
-    asm("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    asm volatile("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(v));
     return v;
 }
 __device__ __forceinline__ float warp_max(float v) {
-    asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
     return v;
 }
 template <int G>
@@ -444,8 +444,10 @@ rms_norm_long_kernel(const NormArgs a) {
         }
         for (int k = threadIdx.x; k < a.K; k += kLongThreads) {
             const float s = to_f(x[k]) + (r ? to_f(r[k]) : 0.0f);
-            if constexpr (Q) static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(f(s * lift_of(m), wt(k)));
-            else static_cast<T*>(a.y)[t * a.ldy + k] = from_f<T>(s * (wt(k) * rstd));
+            if constexpr (Q)
+                static_cast<uint8_t*>(a.y)[t * a.ldy + k] = to_e4m3(f(s * lift_of(m), wt(k)));
+            else
+                static_cast<T*>(a.y)[t * a.ldy + k] = from_f<T>(s * (wt(k) * rstd));
         }
     }
 }

@@ -70,7 +70,7 @@ int bvml_blocks_status(void* stream);
 /*
  * Attempts of each wait between a matrix product's copies, MMAs and epilogue, for the
  * launches of the process that follow; returns the value before (4194304 at first). For tests of that
- * path: with 1 a wait gives up where what it waits for is not there yet. What is in
+ * path: with 1 (or 0) a wait gives up where what it waits for is not there yet. What is in
  * flight then is waited for all the same before the kernel leaves.
  */
 unsigned bvml_blocks_wait_limit(unsigned attempts);
